@@ -227,6 +227,57 @@ int kdw_fprop_bnrelu_f16(const void* x, const float* scale, const float* shift, 
                          int64_t x_strideW, int64_t y_strideN, int64_t y_strideH, int64_t y_strideW,
                          int prologue_type, int tune, void* stream);
 
+/*
+ * Channel-mixing products of row groups (16-bit operands, fp32 sums, one rounding), the pointwise half that follows a
+ * depthwise convolution; a group per expert, rows sorted by group.  Group e is the rows [ends[e-1], ends[e]) of T, ends
+ * a device array of E cumulative row counts; ends that step back or pass T are clamped.  ends may be NULL with E == 1:
+ * one group of all rows.
+ *   KDW_LINEAR_FWD    out[t,n]   = sum_k a[t,k] * b[e(t),n,k]     a = rows [T][K], b = weights [E][N][K], out [T][N]
+ *   KDW_LINEAR_DGRAD  out[t,k]   = sum_n a[t,n] * b[e(t),n,k]     a = grad [T][N], b = weights [E][N][K], out [T][K]
+ *   KDW_LINEAR_WGRAD  out[e,n,k] = sum_{t in e} a[t,n] * b[t,k]   a = grad [T][N], b = rows [T][K],       out [E][N][K]
+ * Output rows that belong to no group are zero, and so is the weight gradient of a group without rows.  Weights and
+ * outputs are dense; a_stride, b_stride are the elements between the rows of a row operand (b_stride is ignored where
+ * b is the weights).  Rows with a base or stride that is no multiple of 16 bytes, and weights with such a K, are copied
+ * into the workspace first.  1 <= E <= 1024.  The sums are added in a fixed order: same bits every call.
+ *   workspace  256-byte aligned, kdw_linear_f16_workspace_bytes() of the same arguments (0: may be NULL); negative: an
+ *              error.  No initialisation needed; not to be shared by calls that can overlap.
+ */
+#define KDW_LINEAR_FWD 0
+#define KDW_LINEAR_DGRAD 1
+#define KDW_LINEAR_WGRAD 2
+
+/* element types */
+#define KDW_F16 0
+#define KDW_BF16 1
+#define KDW_I8 2
+
+int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int64_t T, int64_t E, int64_t K, int64_t N,
+                                       int64_t a_stride, int64_t b_stride, int dtype);
+int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_t* ends, void* workspace,
+                   int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t a_stride,
+                   int64_t b_stride, int dtype, void* stream);
+
+/*
+ * Rows of 16-bit values as 8-bit integers:  scale[r] = max|x[r,:]| / 127,  q[r,c] = x[r,c] * 127 / max|x[r,:]| rounded to
+ * the nearest integer, halves to even (the exact quotient's rounding).  A row of zeros gives q = 0 and scale 0, a row
+ * with a NaN or an infinity q = 0 and scale NaN.  x: KDW_F16 / KDW_BF16 [rows] x x_stride; q dense [rows][cols].
+ */
+int kdw_quant_rows(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int dtype,
+                   void* stream);
+
+/*
+ * Channel-mixing product in 8-bit integers with a scale per row and per output channel, groups as for kdw_linear_f16:
+ *   y[t,n] = (sum_k x[t,k] * w[e(t),n,k]) * x_scale[t] * w_scale[e(t),n]      y [T][N] KDW_F16 / KDW_BF16 (dtype)
+ * The integer sums are exact (K <= 131071); rows of no group are zero.  x_type KDW_I8: int8 rows with x_scale [T];
+ * KDW_F16 / KDW_BF16: rows that the call quantises as kdw_quant_rows does (x_scale ignored).  w int8 [E][N][K] dense,
+ * w_scale fp32 [E][N].  workspace as for kdw_linear_f16.
+ */
+int64_t kdw_linear_i8_workspace_bytes(const void* x, const void* w, int64_t T, int64_t E, int64_t K, int64_t N,
+                                      int64_t x_stride, int x_type, int dtype);
+int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const float* w_scale, void* y, const int32_t* ends,
+                  void* workspace, int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t x_stride,
+                  int x_type, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

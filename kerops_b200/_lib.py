@@ -42,6 +42,11 @@ SIGNATURES = {
     'kdw_fprop_addstats_f16': (_int, [_ptr] * 5 + [_i64] + [_ptr] * 2 + [_i64] * 5 + [_i64] * 9 + [_int, _ptr]),
     'kdw_fprop_bnrelu_variants': (_int, []),
     'kdw_fprop_bnrelu_f16': (_int, [_ptr] * 5 + [_i64] * 5 + [_i64] * 6 + [_int, _int, _ptr]),
+    'kdw_linear_f16_workspace_bytes': (_i64, [_int, _ptr, _ptr] + [_i64] * 6 + [_int]),
+    'kdw_linear_f16': (_int, [_int] + [_ptr] * 5 + [_i64] + [_i64] * 6 + [_int, _ptr]),
+    'kdw_quant_rows': (_int, [_ptr] * 3 + [_i64] * 3 + [_int, _ptr]),
+    'kdw_linear_i8_workspace_bytes': (_i64, [_ptr, _ptr] + [_i64] * 5 + [_int, _int]),
+    'kdw_linear_i8': (_int, [_ptr] * 7 + [_i64] + [_i64] * 5 + [_int, _int, _ptr]),
     'kdw_allreduce_buffer_bytes': (_i64, [_i64, _int]),
     'kdw_allreduce_push_f32': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _int, _int, ctypes.c_uint32, _i64, _ptr]),
 }

@@ -8,6 +8,7 @@ on all three axes, so it runs on the forward kernel unchanged.
 import torch
 
 from .ops.conv import DWConv, DWConvWGRAD
+from .ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
 
 
 def DWConvDGRAD(grad, weight, *, ACCTYPE='float32'):
@@ -54,3 +55,41 @@ class DepthwiseConv3d(torch.nn.Module):
 
     def forward(self, x):
         return depthwise_conv3d(x, self.weight)
+
+
+class GroupedLinearFunction(torch.autograd.Function):
+    """y = GroupedLinear(x, weight, ends) with gradients for x and weight."""
+
+    @staticmethod
+    def forward(ctx, x, weight, ends):
+        ctx.save_for_backward(x, weight, ends)
+        return GroupedLinear(x, weight, ends)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, weight, ends = ctx.saved_tensors
+        # an expanded or transposed gradient (of a sum, say) has no rows of contiguous channels
+        grad_out = grad_out.contiguous(memory_format=torch.channels_last_3d if grad_out.ndim == 5 else torch.contiguous_format)
+        grad_x = GroupedLinearDGRAD(grad_out, weight, ends) if ctx.needs_input_grad[0] else None
+        grad_w = None
+        if ctx.needs_input_grad[1]:
+            grad_w = GroupedLinearWGRAD(x, grad_out, ends).view(weight.shape)
+        return grad_x, grad_w, None
+
+
+def grouped_linear(x, weight, ends=None):
+    """Differentiable product of row groups with a weight matrix each; see ops.linear.GroupedLinear."""
+    return GroupedLinearFunction.apply(x, weight, ends)
+
+
+class ExpertLinear(torch.nn.Module):
+    """Module form of grouped_linear: `experts` bias-free channel-mixing products, weight [experts, out, in]."""
+
+    def __init__(self, experts, in_channels, out_channels, device=None, dtype=torch.float16):
+        super().__init__()
+        bound = 1.0 / in_channels ** 0.5  # kaiming_uniform_(a=sqrt(5)) on each (out, in) matrix
+        w = (torch.rand(experts, out_channels, in_channels, device=device) * 2 - 1) * bound
+        self.weight = torch.nn.Parameter(w.to(dtype))
+
+    def forward(self, x, ends=None):
+        return grouped_linear(x, self.weight, ends)

@@ -63,12 +63,12 @@ int device_sm_count(int* sms);
 // grid_dependency_wait() before it touches anything the previous kernel wrote - the wait returns when that kernel
 // has completed and its writes are visible; under an ordinary launch the wait returns at once.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_overlapping_previous(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t st,
-                                               Args... args) {
+inline cudaError_t launch_overlapping_previous_smem(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem,
+                                                    cudaStream_t st, const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = 0;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -76,6 +76,11 @@ inline cudaError_t launch_overlapping_previous(void (*kernel)(KArgs...), unsigne
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_overlapping_previous(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t st,
+                                               Args... args) {
+    return launch_overlapping_previous_smem(kernel, grid, block, (size_t)0, st, args...);
 }
 #endif
 

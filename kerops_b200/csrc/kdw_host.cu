@@ -8,6 +8,7 @@
 
 #include "../../include/kdw.h"
 #include "kdw_common.cuh"
+#include "linear_plan.h"
 
 namespace kdw {
 
@@ -197,6 +198,34 @@ int encode_paired_map(CUtensorMap* map, const void* base, int64_t N, int64_t C, 
                     nan_fill ? CU_TENSOR_MAP_FLOAT_OOB_FILL_NAN_REQUEST_ZERO_FMA : CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled (paired d axis) failed with CUresult %d", (int)r);
+        return (int)r;
+    }
+    return 0;
+}
+
+int encode_rows_map(CUtensorMap* map, const void* base, int esize, int64_t cols, int64_t rows, int64_t stride,
+                    int64_t groups, int64_t group_stride, int box_cols, int box_rows) {
+    EncodeTiledFn fn;
+    int rc = get_encode_fn(&fn);
+    if (rc) return rc;
+    if (((uintptr_t)base & 15) != 0 || (stride * esize) % 16 != 0 || (group_stride * esize) % 16 != 0) {
+        set_error("tensor map of rows needs a 16-byte aligned base and strides");
+        return KDW_ERR_ALIGN;
+    }
+    if (box_cols * esize != 128 || box_rows < 1 || box_rows > 256) {  // a box row is one swizzle span
+        set_error("tensor-map box out of range");
+        return KDW_ERR_ARG;
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t strides[2] = {(cuuint64_t)(stride * esize), (cuuint64_t)(group_stride * esize)};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, esize == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, groups > 0 ? 3 : 2,
+                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled (rows) failed with CUresult %d (cols=%lld rows=%lld stride=%lld groups=%lld)", (int)r,
+                  (long long)cols, (long long)rows, (long long)stride, (long long)groups);
         return (int)r;
     }
     return 0;

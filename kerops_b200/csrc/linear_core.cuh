@@ -1,0 +1,261 @@
+// Channel-mixing products on the fifth-generation tensor cores (sm_100a): shared declarations, the work schedule
+// of ragged row groups and the PTX wrappers of tcgen05 and 2-D / 3-D TMA loads.
+//
+//   row products     out[t, :] = a[t, :] * B_g          for the rows t of group g   (forward, input gradient, int8)
+//   weight gradient  out[g]    = sum_t a[t, :]^T b[t, :] over the rows t of group g
+//
+// A UNIT is one output tile of 128 x BN and one share of its contraction.  Row groups end where the device array
+// `ends` says; every CTA scans it once into a table in shared memory (first row and first unit of each group), and a
+// unit index is found in it by bisection, so the host never waits for the row counts.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "kdw_common.cuh"
+
+namespace kdw {
+
+constexpr int kLinMaxGroups = 1024;   // groups of one call: the table of a CTA holds them all
+constexpr int kLinTileM = 128;        // output rows of a tile = lanes of the accumulator
+constexpr int kLinSpan = 128;         // bytes of a shared-memory row = the swizzle span
+
+enum LinOp : int { LIN_FWD = 0, LIN_DGRAD = 1, LIN_WGRAD = 2 };
+
+struct LinParams {
+    const int* ends;        // [E] cumulative row ends, or null: one group of all rows
+    int T, E;               // rows, groups
+    int m_tiles;            // weight gradient: tiles along the output rows; row products: 0 (follows from the group)
+    int n_tiles;            // tiles along the output columns
+    int out_rows, out_cols; // weight gradient: rows of one output matrix; columns of the output
+    int k_blocks;           // row products: blocks of the contraction
+    int splits;             // row products: shares of the contraction
+    int chunk;              // weight gradient: rows of one share (a multiple of 64)
+    void* out;
+    float* partial;         // [unit][BN / 4][128] float4 sums of the shares, or null: every tile has one share
+    int* table;             // copy of the table for the kernel that adds the shares, or null
+    const float* row_scale; // 8-bit operands: [T] and [E][out_cols]
+    const float* col_scale;
+    int out_bf16;
+    int out_vec;            // 1: rows of the output start on 16-byte boundaries
+    uint32_t idesc;
+    int* status;
+    unsigned long long limit_ns;
+    int stop_after;
+};
+
+// First row and first unit of every group (one entry more than there are groups).
+struct LinTable {
+    int row[kLinMaxGroups + 1];
+    int unit[kLinMaxGroups + 1];
+};
+
+struct LinUnit {
+    int g, m0, n0;     // group; first output row (row products: an absolute row of the output) and column
+    int row_end;       // row products: end of the group; weight gradient: rows of the output matrix
+    int kb, ke;        // blocks of the contraction; weight gradient: blocks of 64 rows counted from k_row
+    int k_row;         // weight gradient: first row of the share
+    int k_rows;        // weight gradient: rows of the share (the last block may be partly beyond them)
+    bool whole;        // this unit is the only share of its tile
+};
+
+__host__ __device__ __forceinline__ int lin_ceil(int a, int b) { return (a + b - 1) / b; }
+
+__host__ __device__ __forceinline__ int lin_shares(const LinParams& p, int rows) {
+    if (p.m_tiles == 0) return p.splits;
+    return rows > p.chunk ? lin_ceil(rows, p.chunk) : 1;
+}
+__host__ __device__ __forceinline__ int lin_group_tiles(const LinParams& p, int rows) {
+    return (p.m_tiles ? p.m_tiles : lin_ceil(rows, kLinTileM)) * p.n_tiles;
+}
+
+// Tiles of a group in bands of 16 tile rows, a band's rows fastest: the CTAs that run at the same time then share
+// both operands' tiles in L2 (148 CTAs = 16 tile rows x 9 tile columns).
+constexpr int kLinBand = 16;
+
+__host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const int* row, const int* unit, int u, int BN) {
+    int lo = 0, hi = p.E;  // unit[lo] <= u < unit[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (unit[mid] <= u)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    LinUnit r;
+    r.g = lo;
+    const int rows = row[lo + 1] - row[lo];
+    const int mt = p.m_tiles ? p.m_tiles : lin_ceil(rows, kLinTileM);
+    const int tiles = mt * p.n_tiles;
+    const int v = u - unit[lo];
+    const int share = v / tiles;
+    const int t = v - share * tiles;
+    const int band = t / (kLinBand * p.n_tiles);
+    const int inside = t - band * kLinBand * p.n_tiles;
+    const int high = mt - band * kLinBand < kLinBand ? mt - band * kLinBand : kLinBand;
+    const int nt = inside / high;
+    const int m = band * kLinBand + inside - nt * high;
+    r.n0 = nt * BN;
+    r.k_row = 0;
+    r.k_rows = 0;
+    const int shares = lin_shares(p, rows);
+    r.whole = shares == 1;
+    if (p.m_tiles == 0) {
+        r.m0 = row[lo] + m * kLinTileM;
+        r.row_end = row[lo + 1];
+        r.kb = (int)((long long)p.k_blocks * share / shares);
+        r.ke = (int)((long long)p.k_blocks * (share + 1) / shares);
+    } else {
+        r.m0 = m * kLinTileM;
+        r.row_end = p.out_rows;
+        r.k_row = row[lo] + share * p.chunk;
+        const int left = row[lo + 1] - r.k_row;
+        r.k_rows = left < p.chunk ? left : p.chunk;
+        r.kb = 0;
+        r.ke = lin_ceil(r.k_rows, 64);
+    }
+    return r;
+}
+
+#ifdef __CUDACC__
+
+// Scans `ends` into the table (one warp).  Ends that step back or pass the last row are clamped, so any content
+// gives row ranges inside the tensors.  Returns nothing; the table is complete after the CTA's next barrier.
+__device__ __forceinline__ void lin_build_table(const LinParams& p, int* row, int* unit, int lane) {
+    int rows_before = 0, units_before = 0;
+    if (lane == 0) {
+        row[0] = 0;
+        unit[0] = 0;
+    }
+    for (int base = 0; base < p.E; base += 32) {
+        const int e = base + lane;
+        int end = p.T;
+        if (p.ends) end = e < p.E ? __ldg(p.ends + e) : 0;
+        end = end < 0 ? 0 : (end > p.T ? p.T : end);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, end, d);
+            if (lane >= d && o > end) end = o;
+        }
+        if (end < rows_before) end = rows_before;
+        int begin = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) begin = rows_before;
+        const int rows = end - begin;
+        int units = e < p.E ? lin_group_tiles(p, rows) * lin_shares(p, rows) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, units, d);
+            if (lane >= d) units += o;
+        }
+        units += units_before;
+        if (e < p.E) {
+            row[e + 1] = end;
+            unit[e + 1] = units;
+        }
+        rows_before = __shfl_sync(0xffffffffu, end, 31);
+        units_before = __shfl_sync(0xffffffffu, units, 31);
+    }
+}
+
+__device__ __forceinline__ void tma_load_2d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
+    if ((dst & 1023u) != 0) {
+        atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
+        return;
+    }
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(tm), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1,
+                                            int c2) {
+    if ((dst & 1023u) != 0) {
+        atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
+        return;
+    }
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives on `bar` when the tensor-core work issued so far by this thread has finished.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+template <bool I8>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if constexpr (I8)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+}
+
+// 32 accumulator columns of the calling warp's 32 lanes.
+__device__ __forceinline__ void tmem_load_32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory matrix descriptors, 128-byte swizzle.
+//   contraction contiguous: rows of 128 bytes, groups of 8 rows 1024 bytes apart; a step of 32 bytes along the
+//                           contraction advances the start address by 32 bytes
+//   rows contiguous:        panels of 64 rows (128 bytes) x 64 contraction steps, panels 8192 bytes apart, groups of 8
+//                           steps 1024 bytes apart; 16 steps advance the start address by 2048 bytes
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool row_contiguous) {
+    const uint64_t lead = row_contiguous ? 8192 >> 4 : 1, stride = 1024 >> 4;
+    return (uint64_t)((addr & 0x3ffff) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+    uint32_t r;
+    if (bf16)
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace kdw

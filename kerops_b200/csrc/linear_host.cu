@@ -1,0 +1,283 @@
+// C entry points of the channel-mixing products: argument checks, the plan and the workspace layout.
+#include <algorithm>
+
+#include "../../include/kdw.h"
+#include "linear_core.cuh"
+#include "linear_plan.h"
+
+namespace kdw {
+
+static inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
+    const bool wgrad = a.op == LIN_WGRAD;
+    pl->esize = a.esize;
+    const int64_t con = a.op == LIN_FWD ? a.K : a.op == LIN_DGRAD ? a.N : a.T;  // length of the contraction
+    pl->out_cols = (int)(a.op == LIN_FWD ? a.N : a.K);
+    pl->out_rows = wgrad ? (int)a.N : 0;
+    pl->a_rows = a.T;
+    pl->a_cols = a.op == LIN_FWD ? a.K : a.N;
+    pl->b_rows = wgrad ? a.T : a.E * a.N;
+    pl->b_cols = a.K;
+    // TMA wants 16-byte bases and pitches
+    const int64_t per16 = 16 / a.esize;
+    pl->pack_a = ((uintptr_t)a.a & 15) != 0 || a.a_stride % per16 != 0 || a.a_stride < pl->a_cols;
+    pl->pack_b = ((uintptr_t)a.b & 15) != 0 || a.b_stride % per16 != 0 || a.b_stride < pl->b_cols;
+    pl->a_pitch = round_up(pl->a_cols, per16);
+    pl->b_pitch = round_up(pl->b_cols, per16);
+
+    const int64_t k_elems = 128 / a.esize;
+    pl->k_blocks = wgrad ? 0 : (int)ceil_div(con, k_elems);
+    pl->splits = 1;
+    pl->chunk = 0;
+    // Groups are rounded up to whole tiles: at most one tile row more per group than the rows fill.
+    const int64_t m_tiles = wgrad ? ceil_div(a.N, kLinTileM) : ceil_div(a.T, kLinTileM) + std::min(a.E, a.T) - 1;
+    pl->bn = 64;
+    double best = 1e300;
+    for (int bn : {256, 128, 64}) {
+        const int64_t n_tiles = ceil_div(pl->out_cols, bn);
+        const int64_t tiles = m_tiles * n_tiles * (wgrad ? a.E : 1);
+        // time of a CTA: its tiles times what a tile costs, in columns (a narrow tile re-reads the other operand)
+        const double cost = (double)ceil_div(tiles, sms) * (bn + 64);
+        if (cost < best) {
+            best = cost;
+            pl->bn = bn;
+        }
+    }
+    pl->n_tiles = (int)ceil_div(pl->out_cols, pl->bn);
+    pl->m_tiles = wgrad ? (int)m_tiles : 0;
+    const int64_t tiles = m_tiles * pl->n_tiles * (wgrad ? a.E : 1);
+    pl->max_tiles = tiles;
+    pl->max_units = tiles;
+    bool split = false;
+    if (wgrad) {
+        // shares of the rows so that every SM has work
+        int64_t chunk = round_up(std::max<int64_t>(a.T, 1), 64);
+        if (tiles < 2 * sms && a.T > 512) {
+            const int64_t per_tile = std::max<int64_t>(1, 2 * sms / tiles);
+            chunk = std::max<int64_t>(256, round_up(ceil_div(a.T, per_tile), 64));
+        }
+        pl->chunk = (int)std::min<int64_t>(chunk, 1 << 30);
+        split = pl->chunk < a.T;
+        if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
+    } else if (tiles * 2 <= sms && pl->k_blocks >= 8) {
+        pl->splits = (int)std::min<int64_t>(sms / tiles, pl->k_blocks / 4);
+        split = pl->splits > 1;
+        pl->max_units = tiles * pl->splits;
+    }
+    int64_t off = 0;
+    pl->off_a = pl->off_b = pl->off_table = 0;
+    pl->off_partial = -1;
+    if (pl->pack_a) {
+        pl->off_a = off;
+        off = round_up(off + pl->a_rows * pl->a_pitch * a.esize, 256);
+    }
+    if (pl->pack_b) {
+        pl->off_b = off;
+        off = round_up(off + pl->b_rows * pl->b_pitch * a.esize, 256);
+    }
+    if (split) {
+        pl->off_table = off;
+        off = round_up(off + 2 * (a.E + 1) * 4, 256);
+        pl->off_partial = off;
+        off += pl->max_units * kLinTileM * pl->bn * 4;
+    }
+    pl->bytes = off;
+    if (pl->max_units > INT32_MAX) {
+        set_error("linear: %lld tiles are more than one call takes", (long long)pl->max_units);
+        return KDW_ERR_ARG;
+    }
+    return 0;
+}
+
+static int check_sizes(const char* what, int64_t T, int64_t E, int64_t K, int64_t N) {
+    const int64_t most = INT32_MAX - 1024;
+    if (T < 1 || E < 1 || K < 1 || N < 1 || T > most || K > most || N > most) {
+        set_error("%s: T=%lld E=%lld K=%lld N=%lld out of range", what, (long long)T, (long long)E, (long long)K,
+                  (long long)N);
+        return KDW_ERR_ARG;
+    }
+    if (E > kLinMaxGroups) {
+        set_error("%s: %lld groups, at most %d", what, (long long)E, kLinMaxGroups);
+        return KDW_ERR_ARG;
+    }
+    if (E * N > most) {
+        set_error("%s: E*N=%lld out of range", what, (long long)(E * N));
+        return KDW_ERR_ARG;
+    }
+    return 0;
+}
+
+static int f16_args(LinArgs* a, int op, const void* pa, const void* pb, int64_t T, int64_t E, int64_t K, int64_t N,
+                    int64_t a_stride, int64_t b_stride, int dtype) {
+    int rc = check_sizes("linear_f16", T, E, K, N);
+    if (rc) return rc;
+    if (op < LIN_FWD || op > LIN_WGRAD || (dtype != KDW_F16 && dtype != KDW_BF16)) {
+        set_error("linear_f16: op=%d dtype=%d unknown", op, dtype);
+        return KDW_ERR_ARG;
+    }
+    const int64_t a_cols = op == LIN_FWD ? K : N;
+    if (a_stride < a_cols || (op == LIN_WGRAD && b_stride < K)) {
+        set_error("linear_f16: row strides %lld, %lld are shorter than the rows", (long long)a_stride, (long long)b_stride);
+        return KDW_ERR_ARG;
+    }
+    *a = LinArgs();
+    a->op = op;
+    a->a = pa;
+    a->b = pb;
+    a->T = T;
+    a->E = E;
+    a->K = K;
+    a->N = N;
+    a->a_stride = a_stride;
+    a->b_stride = op == LIN_WGRAD ? b_stride : K;
+    a->esize = 2;
+    a->in_bf16 = a->out_bf16 = dtype == KDW_BF16;
+    return 0;
+}
+
+// The 8-bit product: the rows are int8 with their scales, or 16-bit rows that are quantised into the workspace first.
+struct I8Layout {
+    int64_t q_pitch, off_scale, off_rest;  // bytes; quantised rows at 0
+};
+static int i8_args(LinArgs* a, I8Layout* l, const void* x, const void* w, int64_t T, int64_t E, int64_t K, int64_t N,
+                   int64_t x_stride, int x_type, int dtype) {
+    int rc = check_sizes("linear_i8", T, E, K, N);
+    if (rc) return rc;
+    if ((x_type != KDW_I8 && x_type != KDW_F16 && x_type != KDW_BF16) || (dtype != KDW_F16 && dtype != KDW_BF16)) {
+        set_error("linear_i8: x_type=%d dtype=%d unknown", x_type, dtype);
+        return KDW_ERR_ARG;
+    }
+    if (K > 131071) {  // 2^14 (K - 1) < 2^31 - 2^14: no sum leaves 32 bits
+        set_error("linear_i8: K=%lld, at most 131071 (32-bit sums)", (long long)K);
+        return KDW_ERR_ARG;
+    }
+    if (x_stride < K) {
+        set_error("linear_i8: row stride %lld is shorter than the rows", (long long)x_stride);
+        return KDW_ERR_ARG;
+    }
+    *a = LinArgs();
+    l->q_pitch = l->off_scale = l->off_rest = 0;
+    a->op = LIN_FWD;
+    a->a = x;
+    a->a_stride = x_stride;
+    if (x_type != KDW_I8) {
+        l->q_pitch = round_up(K, 16);
+        l->off_scale = round_up(T * l->q_pitch, 256);
+        l->off_rest = round_up(l->off_scale + 4 * T, 256);
+        a->a = nullptr;  // its copy in the workspace is aligned
+        a->a_stride = l->q_pitch;
+    }
+    a->b = w;
+    a->b_stride = K;
+    a->T = T;
+    a->E = E;
+    a->K = K;
+    a->N = N;
+    a->esize = 1;
+    a->out_bf16 = dtype == KDW_BF16;
+    return 0;
+}
+
+static int plan_and_run(LinArgs* a, void* workspace, int64_t workspace_bytes, void* stream) {
+    LinPlan pl;
+    int sms = 0;
+    int rc = device_sm_count(&sms);
+    if (!rc) rc = linear_plan(&pl, *a, sms);
+    if (rc) return rc;
+    if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || ((uintptr_t)workspace & 255) != 0)) {
+        set_error("linear: workspace of %lld bytes (256-byte aligned) needed, %lld given", (long long)pl.bytes,
+                  (long long)(workspace ? workspace_bytes : 0));
+        return KDW_ERR_WORKSPACE;
+    }
+    return linear_run(pl, *a, workspace, (cudaStream_t)stream);
+}
+
+}  // namespace kdw
+
+extern "C" {
+
+int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int64_t T, int64_t E, int64_t K, int64_t N,
+                                       int64_t a_stride, int64_t b_stride, int dtype) {
+    using namespace kdw;
+    LinArgs args;
+    LinPlan pl;
+    int sms = 0;
+    int rc = f16_args(&args, op, a, b, T, E, K, N, a_stride, b_stride, dtype);
+    if (!rc) rc = device_sm_count(&sms);
+    if (!rc) rc = linear_plan(&pl, args, sms);
+    return rc ? (rc < 0 ? rc : -rc) : pl.bytes;
+}
+
+int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_t* ends, void* workspace,
+                   int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t a_stride,
+                   int64_t b_stride, int dtype, void* stream) {
+    using namespace kdw;
+    if (!a || !b || !out || (!ends && E != 1)) {
+        set_error("linear_f16: null pointer (ends may be null only with one group)");
+        return KDW_ERR_ARG;
+    }
+    LinArgs args;
+    int rc = f16_args(&args, op, a, b, T, E, K, N, a_stride, b_stride, dtype);
+    if (rc) return rc;
+    if (((uintptr_t)a & 1) || ((uintptr_t)b & 1) || ((uintptr_t)out & 1) || ((uintptr_t)ends & 3)) {
+        set_error("linear_f16: a pointer is not aligned to its elements");
+        return KDW_ERR_ALIGN;
+    }
+    args.out = out;
+    args.ends = ends;
+    return plan_and_run(&args, workspace, workspace_bytes, stream);
+}
+
+int64_t kdw_linear_i8_workspace_bytes(const void* x, const void* w, int64_t T, int64_t E, int64_t K, int64_t N,
+                                      int64_t x_stride, int x_type, int dtype) {
+    using namespace kdw;
+    LinArgs args;
+    LinPlan pl;
+    I8Layout l;
+    int sms = 0;
+    int rc = i8_args(&args, &l, x, w, T, E, K, N, x_stride, x_type, dtype);
+    if (!rc) rc = device_sm_count(&sms);
+    if (!rc) rc = linear_plan(&pl, args, sms);
+    return rc ? (rc < 0 ? rc : -rc) : l.off_rest + pl.bytes;
+}
+
+int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const float* w_scale, void* y, const int32_t* ends,
+                  void* workspace, int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t x_stride,
+                  int x_type, int dtype, void* stream) {
+    using namespace kdw;
+    if (!x || !w || !w_scale || !y || (!ends && E != 1) || (x_type == KDW_I8 && !x_scale)) {
+        set_error("linear_i8: null pointer (x_scale may be null only with 16-bit x, ends only with one group)");
+        return KDW_ERR_ARG;
+    }
+    LinArgs args;
+    I8Layout l;
+    int rc = i8_args(&args, &l, x, w, T, E, K, N, x_stride, x_type, dtype);
+    if (rc) return rc;
+    if ((x_type != KDW_I8 && ((uintptr_t)x & 1)) || ((uintptr_t)x_scale & 3) || ((uintptr_t)w_scale & 3) || ((uintptr_t)y & 1) ||
+        ((uintptr_t)ends & 3)) {
+        set_error("linear_i8: a pointer is not aligned to its elements");
+        return KDW_ERR_ALIGN;
+    }
+    args.out = y;
+    args.ends = ends;
+    args.row_scale = x_scale;
+    args.col_scale = w_scale;
+    char* ws = (char*)workspace;
+    if (x_type != KDW_I8) {
+        if (!workspace || workspace_bytes < l.off_rest || ((uintptr_t)workspace & 255) != 0) {
+            set_error("linear_i8: workspace of at least %lld bytes (256-byte aligned) needed", (long long)l.off_rest);
+            return KDW_ERR_WORKSPACE;
+        }
+        args.a = ws;
+        args.row_scale = (const float*)(ws + l.off_scale);
+        rc = quant_rows(x, ws, (float*)(ws + l.off_scale), T, K, x_stride, l.q_pitch, x_type == KDW_BF16, true,
+                        (cudaStream_t)stream);
+        if (rc) return rc;
+        ws += l.off_rest;
+    }
+    return plan_and_run(&args, ws, workspace_bytes - l.off_rest, stream);
+}
+
+}  // extern "C"

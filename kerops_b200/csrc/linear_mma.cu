@@ -1,0 +1,541 @@
+// Channel-mixing products of ragged row groups: forward, input gradient, weight gradient (16-bit operands) and the
+// 8-bit integer product with a scale per row and per output channel.
+#include <string.h>
+
+#include "../../include/kdw.h"
+#include "linear_core.cuh"
+#include "linear_plan.h"
+
+namespace kdw {
+
+// ------------------------------------------------------------------------------------------------------------------
+// The product kernel.  One persistent CTA per SM: warp 0 loads operand tiles with TMA into a ring of stages, warp 1
+// issues the tensor-core products into one of two accumulators in tensor memory, warps 4-7 bring finished accumulators
+// to memory while the next tile is being multiplied, warps 2-3 clear the output rows behind the last group.
+//   A_ROWS / B_ROWS: the operand is stored with its output index contiguous (the contraction runs along memory rows)
+// ------------------------------------------------------------------------------------------------------------------
+template <bool I8_, bool A_ROWS_, bool B_ROWS_, int BN_>
+struct LCfg {
+    static constexpr bool I8 = I8_, A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, WGRAD = A_ROWS_;
+    static constexpr int BN = BN_;
+    static constexpr int THREADS = 256;
+    static constexpr int A_BYTES = kLinTileM * kLinSpan;
+    static constexpr int B_BYTES = BN * kLinSpan;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 196608 / STAGE;
+    static constexpr int PITCH = 144;  // staged output rows: 64 values and 16 bytes more, free of bank conflicts
+    static constexpr int STAGING = 4 * 32 * PITCH;
+    static constexpr int TMEM_COLS = 2 * BN;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + (int)sizeof(LinTable) + (2 * STAGES + 5) * 8 + 16;
+    static constexpr int K_ELEMS = I8 ? 128 : 64;  // contraction steps of a stage
+    static_assert(TMEM_COLS >= 32 && TMEM_COLS <= 512, "");
+    static_assert(SMEM <= 232448, "");
+};
+
+// Writes `rows` x `cols` (<= 64) staged 16-bit values of one warp to memory.
+__device__ __forceinline__ void store_staged(const char* stage, int pitch, char* dst, long long dst_pitch, int rows, int cols,
+                                             bool vec, int lane) {
+    if (vec) {  // 16-byte pieces, eight lanes to a row of 64 values
+        const int c = lane & 7;
+        if (c * 8 < cols) {
+#pragma unroll
+            for (int r = lane >> 3; r < 32; r += 4) {
+                if (r < rows)
+                    *reinterpret_cast<uint4*>(dst + r * dst_pitch + c * 16) =
+                        *reinterpret_cast<const uint4*>(stage + r * pitch + c * 16);
+            }
+        }
+    } else {
+        for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < cols; c += 32)
+                *reinterpret_cast<uint16_t*>(dst + r * dst_pitch + c * 2) =
+                    *reinterpret_cast<const uint16_t*>(stage + r * pitch + c * 2);
+    }
+}
+
+// Clears the output rows that belong to no group: every CTA takes its share.
+__device__ __forceinline__ void clear_rows(const LinParams& p, int first_row, int tid, int nthreads) {
+    const long long begin = (long long)first_row * p.out_cols * 2, end = (long long)p.T * p.out_cols * 2;
+    char* out = reinterpret_cast<char*>(p.out);
+    const long long head = begin + ((16 - ((uintptr_t)(out + begin) & 15)) & 15);
+    const long long id = (long long)blockIdx.x * nthreads + tid, n = (long long)gridDim.x * nthreads;
+    if (head >= end) {
+        for (long long i = begin + 2 * id; i < end; i += 2 * n) *reinterpret_cast<uint16_t*>(out + i) = 0;
+        return;
+    }
+    const long long tail = head + (end - head) / 16 * 16;
+    for (long long i = begin + 2 * id; i < head; i += 2 * n) *reinterpret_cast<uint16_t*>(out + i) = 0;
+    for (long long i = head + 16 * id; i < tail; i += 16 * n) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+    for (long long i = tail + 2 * id; i < end; i += 2 * n) *reinterpret_cast<uint16_t*>(out + i) = 0;
+}
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                               const __grid_constant__ CUtensorMap map_b,
+                                                               const __grid_constant__ LinParams p) {
+    extern __shared__ char smem_raw[];
+    char* const base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    char* const staging = base + C::STAGES * C::STAGE;
+    LinTable* const tab = reinterpret_cast<LinTable*>(staging + C::STAGING);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(
+        reinterpret_cast<char*>(tab) + (sizeof(LinTable) + 7) / 8 * 8);
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 5);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES,
+                   acc_empty = acc_full + 16, drain = acc_empty + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&map_a);
+        prefetch_tmap(&map_b);
+        for (int i = 0; i < C::STAGES; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full + 8 * i, 1);
+            mbar_init(acc_empty + 8 * i, 4);
+        }
+        mbar_init(drain, 1);
+        mbar_fence_init();
+    } else if (warp == 1) {
+        tmem_alloc(smem_u32(s_tmem), C::TMEM_COLS);
+    }
+    // operands, scales and `ends` may be the work of the kernel before this one
+    grid_dependency_wait();
+    if (warp == 2) lin_build_table(p, tab->row, tab->unit, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    const int units = tab->unit[p.E];
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int loads = 0, stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+                for (int k = w.kb; k < w.ke; ++k) {
+                    if (p.stop_after >= 0 && loads >= p.stop_after) {
+                        ok = false;
+                        break;
+                    }
+                    if (!mbar_wait_bounded(empty + 8 * stage, phase ^ 1, p.limit_ns)) {
+                        atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES, bar = full + 8 * stage;
+                    mbar_expect_tx(bar, C::STAGE);
+                    if constexpr (C::WGRAD) {
+                        const int r = w.k_row + k * 64;
+#pragma unroll
+                        for (int j = 0; j < kLinTileM / 64; ++j)
+                            tma_load_2d(p.status, a + j * 8192, &map_a, bar, w.m0 + j * 64, r);
+#pragma unroll
+                        for (int j = 0; j < C::BN / 64; ++j)
+                            tma_load_2d(p.status, b + j * 8192, &map_b, bar, w.n0 + j * 64, r);
+                    } else {
+                        tma_load_2d(p.status, a, &map_a, bar, k * C::K_ELEMS, w.m0);
+                        if constexpr (C::B_ROWS) {
+#pragma unroll
+                            for (int j = 0; j < C::BN / 64; ++j)
+                                tma_load_3d(p.status, b + j * 8192, &map_b, bar, w.n0 + j * 64, k * 64, w.g);
+                        } else {
+                            tma_load_3d(p.status, b, &map_b, bar, k * C::K_ELEMS, w.n0, w.g);
+                        }
+                    }
+                    ++loads;
+                    if (++stage == C::STAGES) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+            // a CTA leaves only when its last copies have landed
+            const int last = loads < C::STAGES ? loads : C::STAGES;
+            for (int i = 0; i < last; ++i) {
+                if (stage == 0) {
+                    stage = C::STAGES;
+                    phase ^= 1;
+                }
+                --stage;
+                if (!mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+            if (w.kb == w.ke) continue;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * C::BN;
+            for (int k = w.kb; k < w.ke; ++k) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns));
+                if (!ok) break;
+                char* const sa = base + stage * C::STAGE;
+                if constexpr (C::WGRAD) {
+                    // rows beyond the share are another group's (or of no group): their products must vanish even
+                    // where one of the factors is a NaN or an infinity, so both operands are cleared
+                    const int valid = w.k_rows - k * 64;
+                    if (valid < 64) {
+                        for (int i = valid * 8 + lane; i < 512; i += 32)
+#pragma unroll
+                            for (int j = 0; j < C::STAGE / 8192; ++j)
+                                *reinterpret_cast<uint4*>(sa + j * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t da = smem_desc(smem_u32(sa), C::A_ROWS);
+                    const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ROWS);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma<C::I8>(d, da + i * (C::A_ROWS ? 2048 >> 4 : 32 >> 4), db + i * (C::B_ROWS ? 2048 >> 4 : 32 >> 4),
+                                      p.idesc, k > w.kb || i > 0);
+                    tc_commit(empty + 8 * stage);
+                    if (k + 1 == w.ke) tc_commit(acc_full + 8 * acc);
+                }
+                __syncwarp();
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1;
+            }
+        }
+        if (!ok && lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        // products in flight still read shared memory and write tensor memory
+        if (elect_one()) {
+            tc_commit(drain);
+            if (!mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        if (!C::WGRAD) clear_rows(p, tab->row[p.E], threadIdx.x - 64, 64);
+        if (p.table && blockIdx.x == 0)
+            for (int i = threadIdx.x - 64; i <= p.E; i += 64) {
+                p.table[i] = tab->row[i];
+                p.table[p.E + 1 + i] = tab->unit[i];
+            }
+    } else {
+        const int q = warp & 3;
+        char* const stg = staging + q * 32 * C::PITCH;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+            const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+            const bool any = w.ke > w.kb;
+            if (any) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * acc, acc_phase, p.limit_ns))) {
+                    if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+                    break;
+                }
+                tc_fence_after();
+            }
+            const uint32_t d = tmem + acc * C::BN + ((uint32_t)(q * 32) << 16);
+            const int row0 = w.m0 + q * 32;
+            int rows = w.row_end - row0;
+            rows = rows > 32 ? 32 : rows;
+            if (w.whole || !p.partial) {
+                char* out = reinterpret_cast<char*>(p.out);
+                const long long pitch = (long long)p.out_cols * 2;
+                if (C::WGRAD) out += (long long)w.g * p.out_rows * pitch;
+                float rs = 1.f;
+                if (C::I8) rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.f;
+                const float* cs = C::I8 ? p.col_scale + (long long)w.g * p.out_cols : nullptr;
+#pragma unroll 1
+                for (int c0 = 0; c0 < C::BN; c0 += 64) {
+                    int cols = p.out_cols - w.n0 - c0;
+                    if (cols <= 0 || rows <= 0) break;
+                    cols = cols > 64 ? 64 : cols;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[32];
+                        if (any) {
+                            tmem_load_32(d + c0 + h * 32, v);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            float f[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if constexpr (C::I8) {
+                                    // one rounding of the exact sum and of each factor; the row's scale first, so
+                                    // that two small scales do not underflow in a product of their own
+                                    const int c = w.n0 + c0 + h * 32 + i + j;
+                                    f[j] = (float)(int)v[i + j] * rs * (c < p.out_cols ? __ldg(cs + c) : 0.f);
+                                } else {
+                                    f[j] = __uint_as_float(v[i + j]);
+                                }
+                            }
+                            uint4 o;
+                            o.x = pack2(f[0], f[1], p.out_bf16);
+                            o.y = pack2(f[2], f[3], p.out_bf16);
+                            o.z = pack2(f[4], f[5], p.out_bf16);
+                            o.w = pack2(f[6], f[7], p.out_bf16);
+                            *reinterpret_cast<uint4*>(stg + lane * C::PITCH + h * 64 + i * 2) = o;
+                        }
+                    }
+                    __syncwarp();
+                    store_staged(stg, C::PITCH, out + row0 * pitch + (long long)(w.n0 + c0) * 2, pitch, rows, cols,
+                                 p.out_vec, lane);
+                    __syncwarp();
+                }
+            } else {
+                // a share of a tile: column quadruples of a row side by side over the rows
+                uint4* out = reinterpret_cast<uint4*>(p.partial) + (long long)u * (C::BN / 4) * kLinTileM + q * 32 + lane;
+#pragma unroll 1
+                for (int c0 = 0; c0 < C::BN; c0 += 32) {
+                    uint32_t v[32];
+                    tmem_load_32(d + c0, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        out[(long long)((c0 + i) / 4) * kLinTileM] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            if (any) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_free(tmem, C::TMEM_COLS);
+}
+
+// Adds the shares of the tiles that have several, in their order, and rounds once.  A CTA takes 32 columns of one tile.
+template <bool I8>
+__global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__ LinParams p, int BN) {
+    __shared__ float s[kLinTileM][33];
+    grid_dependency_wait();
+    const int slices = BN / 32;
+    const int* row = p.table;
+    const int* unit = p.table + p.E + 1;
+    const int tid = threadIdx.x;
+    for (int i = blockIdx.x;; i += gridDim.x) {
+        // tile i / slices, counted over the groups
+        int t = i / slices, g = 0, shares = 0, tiles = 0;
+        for (; g < p.E; ++g) {
+            const int rows = row[g + 1] - row[g];
+            tiles = lin_group_tiles(p, rows);
+            shares = lin_shares(p, rows);
+            if (t < tiles) break;
+            t -= tiles;
+        }
+        if (g == p.E) return;
+        if (shares == 1) continue;
+        const int u = unit[g] + t;
+        const LinUnit w = lin_unit(p, row, unit, u, BN);
+        const int c0 = (i % slices) * 32;
+        int cols = p.out_cols - w.n0 - c0;
+        cols = cols > 32 ? 32 : cols;
+        if (cols <= 0) continue;
+        const int r = tid & 127, half = tid >> 7;  // the thread's row and which 16 of the 32 columns
+        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + (long long)u * (BN / 4) * kLinTileM +
+                           (long long)(c0 / 4 + half * 4) * kLinTileM + r;
+        const long long step = (long long)tiles * (BN / 4) * kLinTileM;
+        float f[16];
+        int n[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            f[j] = 0.f;
+            n[j] = 0;
+        }
+        for (int k = 0; k < shares; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 v = __ldcg(src + k * step + (long long)j * kLinTileM);
+                if (I8) {
+                    n[4 * j] += (int)v.x;
+                    n[4 * j + 1] += (int)v.y;
+                    n[4 * j + 2] += (int)v.z;
+                    n[4 * j + 3] += (int)v.w;
+                } else {
+                    f[4 * j] += __uint_as_float(v.x);
+                    f[4 * j + 1] += __uint_as_float(v.y);
+                    f[4 * j + 2] += __uint_as_float(v.z);
+                    f[4 * j + 3] += __uint_as_float(v.w);
+                }
+            }
+        int rows = w.row_end - w.m0;
+        rows = rows > kLinTileM ? kLinTileM : rows;
+        if (I8) {
+            const float rs = r < rows ? __ldg(p.row_scale + w.m0 + r) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int c = w.n0 + c0 + half * 16 + j;
+                f[j] = (float)n[j] * rs * (c < p.out_cols ? __ldg(p.col_scale + (long long)w.g * p.out_cols + c) : 0.f);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[r][half * 16 + j] = f[j];
+        __syncthreads();
+        char* out = reinterpret_cast<char*>(p.out) + (p.m_tiles ? (long long)w.g * p.out_rows * p.out_cols * 2 : 0);
+        const int c = tid & 31;
+        if (c < cols)
+            for (int rr = tid >> 5; rr < rows; rr += 8) {
+                const uint32_t v = pack2(s[rr][c], 0.f, p.out_bf16);
+                *reinterpret_cast<uint16_t*>(out + ((long long)(w.m0 + rr) * p.out_cols + w.n0 + c0 + c) * 2) = (uint16_t)v;
+            }
+    }
+}
+
+// Copies rows whose pitch or base TMA cannot address to rows of a 16-byte pitch; what lies between the columns and
+// the pitch is never read (the tensor maps end at the columns).
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols,
+                                                        long long src_stride, int dst_stride) {
+    constexpr int V = 16 / sizeof(T);
+    grid_dependency_wait();
+    const int per_row = (cols + V - 1) / V;
+    const long long n = rows * per_row;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long r = i / per_row;
+        const int c = (int)(i - r * per_row) * V;
+        union {
+            uint4 u;
+            T t[V];
+        } v;
+        v.u = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j < cols) v.t[j] = src[r * src_stride + c + j];
+        *reinterpret_cast<uint4*>(dst + r * dst_stride + c) = v.u;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------------------------
+template <class C>
+static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const LinParams& p,
+                          cudaStream_t st) {
+    static KernelSetup setup;
+    int sms = 0, occ = 0;
+    int rc = setup.get((const void*)linear_kernel<C>, C::THREADS, C::SMEM, &sms, &occ);
+    if (rc) return rc;
+    const int grid = pl.max_units < sms ? (pl.max_units > 0 ? (int)pl.max_units : 1) : sms;
+    KDW_CUDA(launch_overlapping_previous_smem(linear_kernel<C>, (unsigned)grid, (unsigned)C::THREADS, (size_t)C::SMEM, st, ma,
+                                              mb, p));
+    if (p.partial) {
+        const long long blocks = pl.max_tiles * (C::BN / 32);
+        KDW_CUDA(launch_overlapping_previous(linear_sum_kernel<C::I8>, (unsigned)(blocks < 4 * sms ? blocks : 4 * sms), 256u,
+                                             st, p, C::BN));
+    }
+    return 0;
+}
+
+template <bool I8, bool AR, bool BR>
+static int launch_width(const LinPlan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const LinParams& p,
+                        cudaStream_t st) {
+    switch (pl.bn) {
+        case 64: return launch_product<LCfg<I8, AR, BR, 64>>(pl, ma, mb, p, st);
+        case 128: return launch_product<LCfg<I8, AR, BR, 128>>(pl, ma, mb, p, st);
+        default: return launch_product<LCfg<I8, AR, BR, 256>>(pl, ma, mb, p, st);
+    }
+}
+
+template <typename T>
+static int pack_rows(const void* src, void* dst, int64_t rows, int64_t cols, int64_t src_stride, int64_t dst_stride,
+                     cudaStream_t st) {
+    const int64_t pieces = rows * ((cols * (int64_t)sizeof(T) + 15) / 16);
+    int sms = 0;
+    int rc = device_sm_count(&sms);
+    if (rc) return rc;
+    const int64_t want = (pieces + 255) / 256;
+    KDW_CUDA(launch_overlapping_previous(pack_rows_kernel<T>, (unsigned)(want < 8 * sms ? want : 8 * sms), 256u, st,
+                                         (const T*)src, (T*)dst, (long long)rows, (int)cols, (long long)src_stride,
+                                         (int)dst_stride));
+    return 0;
+}
+
+int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
+    int* status = nullptr;
+    int rc = status_ptr(&status);
+    if (rc) return rc;
+    char* w = (char*)ws;
+    const void* pa = a.a;
+    const void* pb = a.b;
+    int64_t sa = a.a_stride, sb = a.b_stride;
+    if (pl.pack_a) {
+        pa = w + pl.off_a;
+        rc = pl.esize == 2 ? pack_rows<uint16_t>(a.a, w + pl.off_a, pl.a_rows, pl.a_cols, a.a_stride, pl.a_pitch, st)
+                           : pack_rows<uint8_t>(a.a, w + pl.off_a, pl.a_rows, pl.a_cols, a.a_stride, pl.a_pitch, st);
+        if (rc) return rc;
+        sa = pl.a_pitch;
+    }
+    if (pl.pack_b) {
+        pb = w + pl.off_b;
+        rc = pl.esize == 2 ? pack_rows<uint16_t>(a.b, w + pl.off_b, pl.b_rows, pl.b_cols, a.b_stride, pl.b_pitch, st)
+                           : pack_rows<uint8_t>(a.b, w + pl.off_b, pl.b_rows, pl.b_cols, a.b_stride, pl.b_pitch, st);
+        if (rc) return rc;
+        sb = pl.b_pitch;
+    }
+    LinParams p;
+    memset(&p, 0, sizeof(p));
+    p.ends = a.ends;
+    p.T = (int)a.T;
+    p.E = (int)a.E;
+    p.m_tiles = pl.m_tiles;
+    p.n_tiles = pl.n_tiles;
+    p.out_rows = pl.out_rows;
+    p.out_cols = pl.out_cols;
+    p.k_blocks = pl.k_blocks;
+    p.splits = pl.splits;
+    p.chunk = pl.chunk;
+    p.out = a.out;
+    p.partial = pl.off_partial >= 0 ? (float*)(w + pl.off_partial) : nullptr;
+    p.table = pl.off_partial >= 0 ? (int*)(w + pl.off_table) : nullptr;
+    p.row_scale = a.row_scale;
+    p.col_scale = a.col_scale;
+    p.out_bf16 = a.out_bf16;
+    p.out_vec = (pl.out_cols % 8 == 0) && ((uintptr_t)a.out & 15) == 0;
+    p.status = status;
+    const WaitTest wt = wait_test();
+    p.limit_ns = wt.limit_ns;
+    p.stop_after = wt.stop_after;
+    const bool wgrad = a.op == LIN_WGRAD, b_rows = a.op != LIN_FWD;
+    // accumulator fp32 (1) or int32 (2); operands fp16 (0) / bf16 (1) / int8 (1); which are stored by output index
+    const uint32_t fmt = pl.esize == 1 ? 1u : (uint32_t)a.in_bf16;
+    p.idesc = (pl.esize == 1 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)wgrad << 15 | (uint32_t)b_rows << 16 |
+              (uint32_t)(pl.bn >> 3) << 17 | (uint32_t)(kLinTileM >> 4) << 24;
+    CUtensorMap ma, mb;
+    const int span = kLinSpan / pl.esize;
+    rc = encode_rows_map(&ma, pa, pl.esize, pl.a_cols, pl.a_rows, sa, 0, 0, span, wgrad ? 64 : kLinTileM);
+    if (rc) return rc;
+    if (wgrad)
+        rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows, sb, 0, 0, 64, 64);
+    else
+        rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows / a.E, sb, a.E, pl.b_rows / a.E * sb, span,
+                             b_rows ? 64 : pl.bn);
+    if (rc) return rc;
+    if (pl.esize == 1) return launch_width<true, false, false>(pl, ma, mb, p, st);
+    if (wgrad) return launch_width<false, true, true>(pl, ma, mb, p, st);
+    if (b_rows) return launch_width<false, false, true>(pl, ma, mb, p, st);
+    return launch_width<false, false, false>(pl, ma, mb, p, st);
+}
+
+}  // namespace kdw

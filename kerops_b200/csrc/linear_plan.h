@@ -1,0 +1,45 @@
+// Host-side plan of one channel-mixing product: tile width, shares of the contraction, packed copies and the
+// layout of the workspace.  The workspace query and the launch both build it from the same arguments.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace kdw {
+
+struct LinArgs {
+    int op;               // LinOp
+    const void *a, *b;    // rows [T][.] and: weights [E][N][K] (row products) or rows [T][K] (weight gradient)
+    void* out;
+    const int* ends;
+    int64_t T, E, K, N;
+    int64_t a_stride, b_stride;  // elements between rows; of the weights: K
+    int esize;            // bytes of an operand element (2 or 1)
+    int in_bf16, out_bf16;
+    const float *row_scale, *col_scale;
+};
+
+struct LinPlan {
+    int esize, bn;
+    int m_tiles, n_tiles, out_rows, out_cols, k_blocks, splits, chunk;
+    bool pack_a, pack_b;
+    int64_t a_rows, a_cols, a_pitch, b_rows, b_cols, b_pitch;  // pitches of the packed copies, in elements
+    int64_t off_a, off_b, off_table, off_partial;              // off_partial < 0: no tile has several shares
+    int64_t bytes;
+    int64_t max_tiles, max_units;                              // over all row distributions
+};
+
+int linear_plan(LinPlan* pl, const LinArgs& a, int sms);
+int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st);
+
+// Quantises rows of 16-bit values (see quant_rows.cu); q_padded: what lies between `cols` and q_stride may be written.
+int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride, int bf16,
+               bool q_padded, cudaStream_t st);
+
+// Rows of `cols` elements (1 or 2 bytes each) `stride` elements apart, in `groups` matrices `group_stride` elements
+// apart (0 groups: one matrix, a 2-D map); a box of `box_cols` x `box_rows`, 128-byte swizzle, zeros outside.
+int encode_rows_map(CUtensorMap* map, const void* base, int esize, int64_t cols, int64_t rows, int64_t stride,
+                    int64_t groups, int64_t group_stride, int box_cols, int box_rows);
+
+}  // namespace kdw

@@ -1,0 +1,90 @@
+"""Argument marshalling of the channel-mixing products between torch tensors and the C-ABI (include/kdw.h)."""
+import torch
+
+from ... import _lib
+from ..conv._launch import _on, _stream_ptr
+
+# torch dtype -> KDW_F16 / KDW_BF16 (include/kdw.h)
+TYPES = {torch.float16: 0, torch.bfloat16: 1}
+INT8 = 2  # KDW_I8
+FWD, DGRAD, WGRAD = 0, 1, 2
+MAX_GROUPS = 1024
+
+
+def as_rows(t, name):
+    """The [rows, channels] matrix of `t`: `t` itself, or the voxels of a channels_last_3d (N, C, H, W, D) volume."""
+    if t.ndim == 5:
+        assert t.is_contiguous(memory_format=torch.channels_last_3d), f'{name}: channels_last_3d volume expected'
+        return t.permute(0, 2, 3, 4, 1).reshape(-1, t.shape[1])
+    assert t.ndim == 2, f'{name}: [rows, channels] matrix or (N, C, H, W, D) volume expected'
+    assert t.stride(1) == 1 or t.shape[1] == 1, f'{name}: the channels of a row must be contiguous'
+    assert t.stride(0) >= t.shape[1] or t.shape[0] <= 1, f'{name}: rows must not overlap'
+    return t
+
+
+def like_rows(rows, t):
+    """`rows` [T, C'] in the form of `t`: the matrix itself, or a channels_last_3d volume of t's extents."""
+    if t.ndim == 2:
+        return rows
+    n, _, h, w, d = t.shape
+    return rows.view(n, h, w, d, rows.shape[1]).permute(0, 4, 1, 2, 3)
+
+
+def row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def check_ends(ends, groups, device):
+    if ends is None:
+        assert groups == 1, 'ends is needed with more than one group'
+        return
+    assert ends.dtype == torch.int32 and ends.ndim == 1 and ends.is_contiguous(), 'ends: contiguous int32 vector expected'
+    assert ends.shape[0] == groups, 'ends: one cumulative row count per group expected'
+    assert ends.device == device, 'ends must be on the device of the rows'
+
+
+def product(op, a, b, out, ends, T, E, K, N):
+    """Enqueues one product (FWD | DGRAD | WGRAD) of 16-bit operands on a's device / current stream."""
+    lib = _lib.load()
+    dtype = TYPES[a.dtype]
+    sa, sb = row_stride(a), row_stride(b) if op == WGRAD else K
+    pa, pb = a.data_ptr(), b.data_ptr()
+    with _on(a.device):
+        nbytes = lib.kdw_linear_f16_workspace_bytes(op, pa, pb, T, E, K, N, sa, sb, dtype)
+        if nbytes < 0:
+            _lib.check(int(nbytes))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+        rc = lib.kdw_linear_f16(
+            op, pa, pb, out.data_ptr(), ends.data_ptr() if ends is not None else None,
+            ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sa, sb, dtype, _stream_ptr(a.device),
+        )
+    _lib.check(rc)
+    return out
+
+
+def int8_product(x, x_scale, weight, w_scale, y, ends, T, E, K, N):
+    """Enqueues y = Int8Linear(x); x is int8 with x_scale, or 16-bit (x_scale None)."""
+    lib = _lib.load()
+    x_type, dtype, sx = TYPES.get(x.dtype, INT8), TYPES[y.dtype], row_stride(x)
+    px, pw = x.data_ptr(), weight.data_ptr()
+    with _on(x.device):
+        nbytes = lib.kdw_linear_i8_workspace_bytes(px, pw, T, E, K, N, sx, x_type, dtype)
+        if nbytes < 0:
+            _lib.check(int(nbytes))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        rc = lib.kdw_linear_i8(
+            px, x_scale.data_ptr() if x_scale is not None else None, pw, w_scale.data_ptr(), y.data_ptr(),
+            ends.data_ptr() if ends is not None else None, ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx,
+            x_type, dtype, _stream_ptr(x.device),
+        )
+    _lib.check(rc)
+    return y
+
+
+def quant_rows(x, q, scale):
+    """Enqueues q, scale = QuantRows(x) for a [rows, channels] matrix."""
+    lib = _lib.load()
+    with _on(x.device):
+        rc = lib.kdw_quant_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), x.shape[0], x.shape[1], row_stride(x),
+                                TYPES[x.dtype], _stream_ptr(x.device))
+    _lib.check(rc)

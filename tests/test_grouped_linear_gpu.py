@@ -1,0 +1,331 @@
+"""Products of row groups (forward, input gradient, weight gradient) against a plain 64-bit form.  The inputs are small
+whole numbers wherever possible: their sums are exact in fp32 in any order, so the comparison is bit for bit."""
+import pytest
+import torch
+
+from tests import _linear as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _check(T, K, N, ends, dtype, seed=0):
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    spec = ends
+    ends = [T] if spec is None else spec
+    E = len(ends)
+    x, g = ref.integers((T, K), dtype, seed), ref.integers((T, N), dtype, seed + 1)
+    w = ref.integers((E, N, K), dtype, seed + 2)
+    e = None if spec is None else ref.tensor_ends(ends)
+    y, dx = GroupedLinear(x, w, e), GroupedLinearDGRAD(g, w, e)
+    dw = GroupedLinearWGRAD(x, g, e)
+    assert dw.shape == ((N, K) if e is None else (E, N, K))
+    assert torch.equal(y, ref.fwd(x, w, ends).to(dtype))
+    assert torch.equal(dx, ref.dgrad(g, w, ends).to(dtype))
+    assert torch.equal(dw.view(E, N, K), ref.wgrad(x, g, ends).to(dtype))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T', [1, 2, 9, 17, 33, 64, 127, 128, 129, 300])
+@pytest.mark.parametrize('K,N', [(1, 1), (8, 8), (16, 264), (37, 5), (64, 64), (100, 63), (200, 136), (264, 520)])
+def test_one_group(T, K, N, dtype):
+    _check(T, K, N, None, dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T,ends', [
+    (1, [0, 1, 1]),
+    (5, [1, 2, 3, 4, 5]),
+    (300, [0, 0, 300]),
+    (300, [300, 300, 300]),
+    (300, [1, 130, 131, 259]),           # rows behind the last group
+    (300, [0, 0, 0]),                    # no group has rows
+    (300, [200, 100, 250]),              # an end that steps back: an empty group
+    (300, [100, 400, 200]),              # ends past the last row
+    (300, [-5, 128, 256]),
+    (1000, [64, 128, 500, 513, 514, 999]),
+])
+@pytest.mark.parametrize('K,N', [(64, 72), (33, 130), (320, 64)])
+def test_groups(T, ends, K, N, dtype):
+    _check(T, K, N, ends, dtype)
+
+
+@pytest.mark.parametrize('E', [33, 1000, 1024])
+def test_many_groups(E):
+    g = torch.Generator().manual_seed(E)
+    ends = torch.cumsum(torch.randint(0, 4, (E,), generator=g), 0).tolist()
+    _check(ends[-1] + 3, 40, 24, ends, torch.bfloat16)
+
+
+@pytest.mark.parametrize('T,K,N,ends', [
+    (4096, 512, 768, None),              # wide tiles
+    (3000, 1024, 512, [1000, 1700, 2990]),
+    (16, 4096, 512, None),               # a long contraction over few rows: shares that are added afterwards
+    (40, 4104, 512, [3, 30]),
+    (150, 2048, 130, None),
+    (30000, 64, 96, None),               # a long contraction of the weight gradient
+    (30011, 40, 72, [29000, 29000, 30000]),
+])
+def test_larger(T, K, N, ends):
+    _check(T, K, N, ends, torch.float16)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_normal_values_within_the_rounding(dtype):
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, K, N, ends = 700, 328, 200, [100, 100, 650]
+    gen = torch.Generator(device='cuda').manual_seed(4)
+    x = torch.randn(T, K, generator=gen, device='cuda').to(dtype)
+    g = torch.randn(T, N, generator=gen, device='cuda').to(dtype)
+    w = (torch.randn(3, N, K, generator=gen, device='cuda') / K ** 0.5).to(dtype)
+    e = ref.tensor_ends(ends)
+    # half a step of the result, and for each of the n fp32 additions at most a step of fp32 (2^-23) of the sum of
+    # magnitudes; the last term is half the smallest subnormal of fp16
+    for got, f, args, n in ((GroupedLinear(x, w, e), ref.fwd, (x, w), K), (GroupedLinearDGRAD(g, w, e), ref.dgrad, (g, w), N),
+                            (GroupedLinearWGRAD(x, g, e), ref.wgrad, (x, g), T)):
+        want, size = f(*args, ends), f(*(a.abs() for a in args), ends)
+        err = (got.double() - want).abs()
+        assert (err <= torch.finfo(dtype).eps / 2 * want.abs() + n * 2.0 ** -23 * size + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_a_group_sees_only_its_rows(bad):
+    """NaN and infinities in one group, and in rows of no group, change no other group's results."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, K, N, ends = 500, 72, 136, [100, 230, 400]
+    x, g = ref.integers((T, K), torch.float16, 1), ref.integers((T, N), torch.float16, 2)
+    w = ref.integers((3, N, K), torch.float16, 3)
+    e = ref.tensor_ends(ends)
+    y, dx, dw = ref.fwd(x, w, ends).half(), ref.dgrad(g, w, ends).half(), ref.wgrad(x, g, ends).half()
+    x[100:230], g[100:230], x[400:], g[400:] = bad, bad, bad, bad
+    gy, gdx, gdw = GroupedLinear(x, w, e), GroupedLinearDGRAD(g, w, e), GroupedLinearWGRAD(x, g, e)
+    keep = [*range(100), *range(230, 500)]
+    assert torch.equal(gy[keep], y[keep]) and torch.equal(gdx[keep], dx[keep])
+    assert torch.equal(gdw[[0, 2]], dw[[0, 2]])
+    assert not torch.isfinite(gdw[1]).any()
+    assert torch.isnan(gy[100:230]).all() or torch.isinf(gy[100:230]).any()
+
+
+@pytest.mark.parametrize('offset,stride', [(0, 80), (8, 88), (1, 80), (0, 73), (3, 91)])
+def test_row_strides_and_bases(offset, stride):
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, C, N, ends = 333, 72, 72, [10, 300]
+    wide_x, wide_g = ref.integers((T, stride + 8), torch.bfloat16, 1), ref.integers((T, stride + 8), torch.bfloat16, 2)
+    wide_x, wide_g = wide_x.flatten()[:T * stride + 8], wide_g.flatten()[:T * stride + 8]
+    before = wide_x.clone(), wide_g.clone()
+    x, g = (torch.as_strided(t, (T, C), (stride, 1), offset) for t in (wide_x, wide_g))
+    w = ref.integers((2, N, C), torch.bfloat16, 3)
+    e = ref.tensor_ends(ends)
+    assert torch.equal(GroupedLinear(x, w, e), ref.fwd(x, w, ends).bfloat16())
+    assert torch.equal(GroupedLinearDGRAD(g, w, e), ref.dgrad(g, w, ends).bfloat16())
+    assert torch.equal(GroupedLinearWGRAD(x, g, e), ref.wgrad(x, g, ends).bfloat16())
+    assert torch.equal(wide_x, before[0]) and torch.equal(wide_g, before[1])
+
+
+@pytest.mark.parametrize('K', [64, 33])
+@pytest.mark.parametrize('rows', [12, 400])
+def test_nothing_beyond_the_outputs_is_written(K, rows):
+    from kerops_b200.ops.linear import _launch
+
+    N, ends, guard = 72, [rows // 4, rows - 5], 4096
+    x, g = ref.integers((rows, K), torch.float16, 1), ref.integers((rows, N), torch.float16, 2)
+    w = ref.integers((2, N, K), torch.float16, 3)
+    e = ref.tensor_ends(ends)
+    for op, a, b, shape, want in ((0, x, w, (rows, N), ref.fwd(x, w, ends)), (1, g, w, (rows, K), ref.dgrad(g, w, ends)),
+                                  (2, g, x, (2, N, K), ref.wgrad(x, g, ends))):
+        n = torch.Size(shape).numel()
+        for shift in (0, 1):  # an aligned output and one that only scalar stores reach
+            buf = torch.full((n + 2 * guard,), 7.0, dtype=torch.float16, device='cuda')
+            out = buf[guard + shift:guard + shift + n].view(shape)
+            _launch.product(op, a, b, out, e, rows, 2, K, N)
+            assert torch.equal(out, want.half())
+            assert (buf[:guard + shift] == 7).all() and (buf[guard + shift + n:] == 7).all()
+
+
+def test_volumes_and_empty_inputs():
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    x = ref.integers((2, 3, 5, 7, 16), torch.float16, 1).permute(0, 4, 1, 2, 3)
+    g = ref.integers((2, 3, 5, 7, 24), torch.float16, 2).permute(0, 4, 1, 2, 3)
+    w = ref.integers((2, 24, 16), torch.float16, 3)
+    e = ref.tensor_ends([105, 210])  # a group per sample
+    xr, gr = x.permute(0, 2, 3, 4, 1).reshape(210, 16), g.permute(0, 2, 3, 4, 1).reshape(210, 24)
+    y, dx = GroupedLinear(x, w, e), GroupedLinearDGRAD(g, w, e)
+    assert y.shape == g.shape and y.stride() == g.stride() and dx.shape == x.shape and dx.stride() == x.stride()
+    assert torch.equal(y.permute(0, 2, 3, 4, 1).reshape(210, 24), ref.fwd(xr, w, [105, 210]).half())
+    assert torch.equal(dx.permute(0, 2, 3, 4, 1).reshape(210, 16), ref.dgrad(gr, w, [105, 210]).half())
+    assert torch.equal(GroupedLinearWGRAD(x, g, e), ref.wgrad(xr, gr, [105, 210]).half())
+    none = torch.empty(0, 16, dtype=torch.float16, device='cuda')
+    assert GroupedLinear(none, w, e).shape == (0, 24)
+    assert torch.equal(GroupedLinearWGRAD(none, torch.empty(0, 24, dtype=torch.float16, device='cuda'), e), torch.zeros_like(w))
+
+
+def test_offsets_beyond_32_bits():
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, K, N = 17_000_100, 136, 136  # 2.3e9 values per operand
+    ends = [16_999_000, 17_000_050]
+    x = torch.zeros(T, K, dtype=torch.float16, device='cuda')
+    tail = ref.integers((2000, K), torch.float16, 1)
+    x[-2000:] = tail
+    w = ref.integers((2, N, K), torch.float16, 2)
+    e = ref.tensor_ends(ends)
+    local = [t - (T - 2000) for t in ends]
+    want = ref.fwd(tail, w, local).half()
+    y = GroupedLinear(x, w, e)
+    assert torch.equal(y[-2000:], want) and not y[:-2000].any()
+    del y
+    dx = GroupedLinearDGRAD(x, w, e)
+    assert torch.equal(dx[-2000:], ref.dgrad(tail, w, local).half()) and not dx[:-2000].any()
+    del dx
+    assert torch.equal(GroupedLinearWGRAD(x, x, e), ref.wgrad(tail, tail, local).half())
+
+
+def test_same_bits_every_call_and_on_any_stream():
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearWGRAD
+
+    T, K, N = 20000, 96, 160
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    x = torch.randn(T, K, generator=gen, device='cuda', dtype=torch.float16)
+    g = torch.randn(T, N, generator=gen, device='cuda', dtype=torch.float16)
+    w = torch.randn(3, N, K, generator=gen, device='cuda', dtype=torch.float16)
+    e = ref.tensor_ends([3000, 15000, 20000])
+    first = GroupedLinear(x, w, e), GroupedLinearWGRAD(x, g, e)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((GroupedLinear(x, w, e), GroupedLinearWGRAD(x, g, e)))
+    torch.cuda.synchronize()
+    for y, dw in got:
+        assert torch.equal(y, first[0]) and torch.equal(dw, first[1])
+
+
+def test_capture_and_replay():
+    """The row counts are read on the device: a captured step replays on other rows, weights and ends."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, K, N = 600, 72, 200
+    x, g = ref.integers((T, K), torch.float16, 1), ref.integers((T, N), torch.float16, 2)
+    w, e = ref.integers((3, N, K), torch.float16, 3), ref.tensor_ends([100, 400, 600])
+
+    def step():
+        return GroupedLinear(x, w, e), GroupedLinearDGRAD(g, w, e), GroupedLinearWGRAD(x, g, e)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):  # two graphs do not share a workspace
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for seed, ends in ((10, [1, 1, 590]), (20, [600, 600, 600]), (30, [0, 300, 301])):
+        x.copy_(ref.integers((T, K), torch.float16, seed))
+        w.copy_(ref.integers((3, N, K), torch.float16, seed + 1))
+        e.copy_(ref.tensor_ends(ends))
+        for o in outs:
+            for t in o:
+                t.fill_(float('nan'))
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for y, dx, dw in outs:
+            assert torch.equal(y, ref.fwd(x, w, ends).half())
+            assert torch.equal(dx, ref.dgrad(g, w, ends).half())
+            assert torch.equal(dw, ref.wgrad(x, g, ends).half())
+
+
+@pytest.mark.parametrize('shape', ['matrix', 'volume'])
+def test_autograd_formula_and_differences(shape):
+    from kerops_b200.autograd import ExpertLinear, grouped_linear
+
+    T, K, N, ends = 210, 16, 24, [50, 50, 200]
+    e = ref.tensor_ends(ends)
+
+    def form(t):
+        return t if shape == 'matrix' else t.view(2, 3, 5, 7, -1).permute(0, 4, 1, 2, 3)
+
+    def rows(t):
+        return t if shape == 'matrix' else t.permute(0, 2, 3, 4, 1).reshape(T, -1)
+
+    x, w = form(ref.integers((T, K), torch.float16, 1)).requires_grad_(True), ref.integers((3, N, K), torch.float16, 2).requires_grad_(True)
+    g = form(ref.integers((T, N), torch.float16, 3))
+    y = grouped_linear(x, w, e)
+    y.backward(g)
+    assert torch.equal(rows(x.grad), ref.dgrad(rows(g), w.detach(), ends).half())
+    assert torch.equal(w.grad, ref.wgrad(rows(x.detach()), rows(g), ends).half())
+    # the product is linear in each argument: a difference quotient is exact, whatever the step
+    dx, dw = form(ref.integers((T, K), torch.float16, 4)), ref.integers((3, N, K), torch.float16, 5)
+    with torch.no_grad():
+        along_x = grouped_linear(x + dx, w, e).double() - y.double()
+        along_w = grouped_linear(x, w + dw, e).double() - y.double()
+    assert (along_x * g.double()).sum() == (x.grad.double() * dx.double()).sum()
+    assert (along_w * g.double()).sum() == (w.grad.double() * dw.double()).sum()
+    # a gradient that is one value expanded, only one of the gradients wanted, and the module
+    m = ExpertLinear(3, K, N, device='cuda')
+    m(x.detach(), e).sum().backward()
+    assert torch.equal(m.weight.grad, ref.wgrad(rows(x.detach()), torch.ones(T, N, device='cuda'), ends).half())
+    x.grad = None
+    m.weight.requires_grad_(False)
+    m(x, e).sum().backward()
+    err = (rows(x.grad).double() - ref.dgrad(torch.ones(T, N, device='cuda'), m.weight, ends)).abs()
+    assert (err <= 2.0 ** -11 * rows(x.grad).abs() + N * 2.0 ** -23 * N / 4).all()  # |w| <= 1/4
+
+
+def test_depthwise_then_pointwise_step():
+    """The products behind a depthwise convolution, as a layer uses them: y = experts(dwconv(x)) and all gradients."""
+    from kerops_b200.autograd import DepthwiseConv3d, ExpertLinear
+    from kerops_b200.ops.conv import DWConv, DWConvWGRAD
+    from kerops_b200.autograd import DWConvDGRAD
+
+    C, N = 16, 40
+    x = ref.integers((2, 6, 8, 12, C), torch.float16, 1).permute(0, 4, 1, 2, 3).requires_grad_(True)
+    conv, mix = DepthwiseConv3d(C, device='cuda'), ExpertLinear(2, C, N, device='cuda')
+    conv.weight.data.copy_(ref.integers((3, 3, 3, C), torch.float16, 2, top=1))
+    mix.weight.data.copy_(ref.integers((2, N, C), torch.float16, 3, top=1))
+    e = ref.tensor_ends([576, 1152])
+    g = ref.integers((2, 6, 8, 12, N), torch.float16, 4, top=1).permute(0, 4, 1, 2, 3)
+    mix(conv(x), e).backward(g)
+
+    def rows(t):
+        return t.permute(0, 2, 3, 4, 1).reshape(1152, -1)
+
+    h = DWConv(x.detach(), conv.weight.detach())
+    gh = ref.dgrad(rows(g), mix.weight.detach(), [576, 1152]).half().view(2, 6, 8, 12, C).permute(0, 4, 1, 2, 3)
+    assert torch.equal(mix.weight.grad, ref.wgrad(rows(h), rows(g), [576, 1152]).half())
+    assert torch.equal(conv.weight.grad, DWConvWGRAD(x.detach(), gh))
+    assert torch.equal(x.grad, DWConvDGRAD(gh, conv.weight.detach()))
+
+
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable():
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearWGRAD
+
+    x, w = ref.integers((600, 512), torch.float16, 1), ref.integers((1, 256, 512), torch.float16, 2)
+    g = ref.integers((600, 256), torch.float16, 3)
+    lib = _lib.load()
+    want = GroupedLinear(x, w), GroupedLinearWGRAD(x, g)
+    assert _lib.device_status() == 0
+    try:
+        for stop in (0, 3):
+            assert lib.kdw_test_wait_limits(50_000_000, stop) == 0
+            GroupedLinear(x, w)
+            assert _lib.device_status() == 1
+            GroupedLinearWGRAD(x, g)
+            assert _lib.device_status() == 1
+    finally:
+        lib.kdw_test_wait_limits(2_000_000_000, -1)
+    assert torch.equal(GroupedLinear(x, w), want[0]) and torch.equal(GroupedLinearWGRAD(x, g), want[1])
+    assert _lib.device_status() == 0

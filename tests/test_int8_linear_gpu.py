@@ -1,0 +1,231 @@
+"""The row quantiser and the 8-bit integer product.  Both are defined to the bit: the quantised values are the exactly
+rounded quotients, the integer sums are exact, and the two scales are applied in fp32 one after the other."""
+import numpy as np
+import pytest
+import torch
+
+from tests import _linear as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _quant(x):
+    """64-bit form; a quotient that is no half misses every half by 2^-20 and more, one that is comes out exactly."""
+    f = x.double().cpu().numpy()
+    top = np.abs(f).max(axis=1, keepdims=True)
+    with np.errstate(invalid='ignore', divide='ignore'):
+        q = np.where(top > 0, np.rint(f * 127 / top), 0)
+    scale = (torch.from_numpy(top[:, 0]).float() / 127).to(x.device)
+    return torch.from_numpy(q).to(torch.int8).to(x.device), scale
+
+
+def _all_values(dtype):
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    return bits[torch.isfinite(bits)].cuda()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_quant_every_value_against_many_maxima(dtype):
+    from kerops_b200.ops.linear import QuantRows
+
+    values = _all_values(dtype)
+    g = torch.Generator(device='cuda').manual_seed(0)
+    some = values[torch.randint(len(values), (60,), generator=g, device='cuda')].abs()
+    edge = torch.tensor([1.0, 127.0, 254.0, 127 * 1.5, 2.0 ** -10, torch.finfo(dtype).max, torch.finfo(dtype).tiny], device='cuda').to(dtype)
+    smallest = values[values > 0].min()
+    for top in [*some, *edge, smallest]:
+        row = torch.where(values.abs() <= top, values, torch.zeros_like(values))
+        row = torch.cat([row, top.view(1)])[None]
+        q, s = QuantRows(row)
+        qr, sr = _quant(row)
+        assert torch.equal(q, qr) and torch.equal(s, sr), float(top)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T,K', [(1, 1), (3, 7), (5, 8), (2, 1000), (9, 1024), (7, 1025), (3, 4096), (2, 8200), (1, 40003), (300, 33)])
+def test_quant_shapes(T, K, dtype):
+    from kerops_b200.ops.linear import QuantRows
+
+    x = torch.randn(T, K, generator=torch.Generator(device='cuda').manual_seed(K), device='cuda').to(dtype)
+    x[0] = 0 if T > 1 else x[0]
+    q, s = QuantRows(x)
+    qr, sr = _quant(x)
+    assert q.shape == x.shape and torch.equal(q, qr) and torch.equal(s, sr)
+    wide = torch.zeros(T, K + 11, dtype=dtype, device='cuda')
+    wide[:, 3:3 + K] = x
+    q, s = QuantRows(wide[:, 3:3 + K])
+    assert torch.equal(q, qr) and torch.equal(s, sr)
+
+
+@pytest.mark.parametrize('K', [40, 2000])
+def test_quant_rows_that_are_not_finite(K):
+    from kerops_b200.ops.linear import QuantRows
+
+    x = torch.randn(6, K, device='cuda').half()
+    x[1, K // 2], x[3, 0], x[4, K - 1] = float('nan'), float('inf'), float('-inf')
+    q, s = QuantRows(x)
+    bad = torch.tensor([False, True, False, True, True, False], device='cuda')
+    assert torch.equal(torch.isnan(s), bad) and not q[bad].any()
+    qr, sr = _quant(x[~bad])
+    assert torch.equal(q[~bad], qr) and torch.equal(s[~bad], sr)
+
+
+def _int8(T, K, N, E, seed):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    x = torch.randint(-128, 128, (T, K), generator=g, device='cuda', dtype=torch.int8)
+    w = torch.randint(-128, 128, (E, N, K), generator=g, device='cuda', dtype=torch.int8)
+    return x, torch.rand(T, generator=g, device='cuda') + 0.01, w, (torch.rand(E, N, generator=g, device='cuda') + 0.01) / K
+
+
+def _product(x, xs, w, ws, ends, dtype):
+    sums = ref.fwd(x, w, ends)  # exact in 64 bits
+    y = torch.zeros(sums.shape, dtype=dtype, device=x.device)
+    for e, (a, b) in enumerate(ref.spans(ends, x.shape[0])):
+        y[a:b] = (sums[a:b].float() * xs[a:b, None] * ws[e]).to(dtype)
+    return y
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T,K,N,ends', [
+    *[(T, K, N, None) for T in (1, 2, 8, 9, 31, 64, 129, 300) for K, N in ((1, 1), (16, 16), (33, 70), (128, 64), (272, 200))],
+    (1, 4096, 1000, None), (3, 4100, 264, None), (16, 8192, 512, None), (60, 4096, 384, None), (1000, 512, 640, None),
+    (300, 144, 136, [0, 100, 100, 290]), (300, 144, 136, [0, 0, 0]), (300, 70, 33, [200, 100, 400]),
+    (12, 2048, 256, [0, 3, 3, 4, 12, 12]), (12, 100, 30, [0, 3, 3, 4, 9, 9]),
+])
+def test_product_to_the_bit(T, K, N, ends, dtype):
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import Int8Linear
+
+    E = 1 if ends is None else len(ends)
+    x, xs, w, ws = _int8(T, K, N, E, T + K + N)
+    e = None if ends is None else ref.tensor_ends(ends)
+    y = Int8Linear(x, w, ws, e, x_scale=xs, dtype=dtype)
+    assert torch.equal(y, _product(x, xs, w, ws, ends or [T], dtype))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T,K,N,ends', [
+    (1, 1, 1, None), (1, 4096, 512, None), (1, 1001, 333, None), (5, 2056, 72, None), (8, 64, 64, None), (33, 256, 100, None),
+    (200, 1000, 130, None), (64, 4096, 1024, None), (1000, 520, 264, [10, 10, 900]), (7, 640, 128, [1, 1, 4, 6]),
+    (16, 9000, 40, None),
+])
+def test_float_rows_are_quantised_within_the_call(T, K, N, ends, dtype):
+    from kerops_b200.ops.linear import Int8Linear
+
+    E = 1 if ends is None else len(ends)
+    _, _, w, ws = _int8(T, K, N, E, 1)
+    x = torch.randn(T, K, generator=torch.Generator(device='cuda').manual_seed(2), device='cuda').to(dtype)
+    if T > 4:
+        x[2] = 0
+        x[3, 0] = float('inf')
+    e = None if ends is None else ref.tensor_ends(ends)
+    y = Int8Linear(x, w, ws, e)
+    fine = torch.isfinite(x).all(1)
+    q, s = _quant(torch.where(fine[:, None], x, torch.zeros_like(x)))
+    s = torch.where(fine, s, torch.full_like(s, float('nan')))
+    want = _product(q, s, w, ws, ends or [T], dtype)
+    assert y.dtype == dtype and torch.equal(y.nan_to_num(7.0), want.nan_to_num(7.0))
+    other = torch.bfloat16 if dtype == torch.float16 else torch.float16
+    y = Int8Linear(x, w, ws, e, dtype=other)
+    assert torch.equal(y.nan_to_num(7.0), _product(q, s, w, ws, ends or [T], other).nan_to_num(7.0))
+
+
+def test_the_longest_sum_stays_inside_32_bits():
+    from kerops_b200.ops.linear import Int8Linear
+    from kerops_b200.ops.linear.int8_linear import MAX_K
+
+    for T in (1, 130):
+        x = torch.full((T, MAX_K), -128, dtype=torch.int8, device='cuda')
+        w = torch.full((1, 24, MAX_K), -128, dtype=torch.int8, device='cuda')
+        one = torch.full((T,), 2.0 ** -16, device='cuda')
+        y = Int8Linear(x, w, torch.ones(1, 24, device='cuda'), x_scale=one, dtype=torch.float16)
+        assert (y == 32768.0).all()  # 2^14 * 131071 / 2^16 = 32767.75, rounded
+
+
+@pytest.mark.parametrize('T', [3, 200])
+def test_small_scales_do_not_underflow_in_a_product_of_their_own(T):
+    from kerops_b200.ops.linear import Int8Linear
+
+    x = torch.full((T, 64), 100, dtype=torch.int8, device='cuda')
+    w = torch.full((1, 8, 64), 100, dtype=torch.int8, device='cuda')
+    y = Int8Linear(x, w, torch.full((1, 8), 1e-22, device='cuda'), x_scale=torch.full((T,), 1e-22, device='cuda'), dtype=torch.bfloat16)
+    want = 640000 * 1e-44
+    assert torch.all((y.double() - want).abs() <= want * 2 ** -7)
+
+
+def test_strides_volumes_and_guard_bands():
+    from kerops_b200.ops.linear import Int8Linear, QuantRows, _launch
+
+    for T, K, N, pad in ((50, 64, 40, 16), (50, 64, 40, 3), (4, 96, 40, 16), (4, 96, 40, 5), (4, 30, 33, 0)):
+        x, xs, w, ws = _int8(T, K + pad, N, 1, 3)
+        view, w = x[:, pad // 2:pad // 2 + K], w[:, :, :K].contiguous()
+        want = _product(view, xs, w, ws, [T], torch.float16)
+        buf = torch.full((T * N + 8192,), 7.0, dtype=torch.float16, device='cuda')
+        for shift in (4096, 4097):
+            buf.fill_(7.0)
+            out = buf[shift:shift + T * N].view(T, N)
+            _launch.int8_product(view, xs, w, ws, out, None, T, 1, K, N)
+            assert torch.equal(out, want) and (buf[:shift] == 7).all() and (buf[shift + T * N:] == 7).all()
+    v = torch.randn(2, 3, 4, 5, 16, device='cuda').half().permute(0, 4, 1, 2, 3)
+    wq, ws = QuantRows(torch.randn(2, 24, 16, device='cuda').half())
+    e = ref.tensor_ends([60, 120])
+    y = Int8Linear(v, wq, ws, e)
+    rows = v.permute(0, 2, 3, 4, 1).reshape(120, 16)
+    assert y.shape == (2, 24, 3, 4, 5) and y.is_contiguous(memory_format=torch.channels_last_3d)
+    assert torch.equal(y.permute(0, 2, 3, 4, 1).reshape(120, 24), Int8Linear(rows, wq, ws, e))
+    q, s = QuantRows(v)
+    assert torch.equal(Int8Linear(q, wq, ws, e, x_scale=s, dtype=torch.float16), y)
+    assert Int8Linear(rows[:0], wq, ws, e).shape == (0, 24)
+
+
+@pytest.mark.parametrize('T', [2, 300])
+def test_streams_and_capture(T):
+    from kerops_b200.ops.linear import Int8Linear
+
+    K, N = 1024, 200
+    x = torch.randn(T, K, device='cuda').half()
+    _, _, w, ws = _int8(1, K, N, 2, 1)
+    e = ref.tensor_ends([1, T])
+    want = Int8Linear(x, w, ws, e)
+    torch.cuda.synchronize()
+    got = []
+    for s in [torch.cuda.Stream() for _ in range(3)]:
+        with torch.cuda.stream(s):
+            got += [Int8Linear(x, w, ws, e) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = Int8Linear(x, w, ws, e)
+    x.copy_(torch.randn(T, K, device='cuda').half())
+    e.copy_(ref.tensor_ends([0, T - 1]))
+    y.fill_(float('nan'))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, Int8Linear(x, w, ws, e)) and not y[T - 1].any()
+
+
+def test_trained_in_16_bits_then_answering_in_8():
+    """The weights that GroupedLinear trains, quantised per output channel and used by Int8Linear: every output is off
+    by what the two roundings of its factors allow."""
+    from kerops_b200.autograd import ExpertLinear
+    from kerops_b200.ops.linear import Int8Linear, QuantRows
+
+    m = ExpertLinear(3, 128, 96, device='cuda', dtype=torch.bfloat16)
+    x = torch.randn(100, 128, generator=torch.Generator(device='cuda').manual_seed(1), device='cuda').bfloat16()
+    ends = [30, 30, 90]
+    e = ref.tensor_ends(ends)
+    w = m.weight.detach()
+    y = Int8Linear(x, *QuantRows(w), e)
+    # a value is off by half a step s/2 = max/254: |x w - x' w'| <= |x| dw + |w| dx + dx dw, summed over K; then half
+    # a step of bf16 for the result and 2^-22 of it for the fp32 scales
+    dx = x.double().abs().amax(1, keepdim=True) / 254
+    want = ref.fwd(x, w, ends)
+    dw = w.double().abs().amax(2) / 254
+    for e_, (a, b) in enumerate(ref.spans(ends, 100)):
+        slack = x[a:b].double().abs().sum(1, keepdim=True) * dw[e_] + dx[a:b] * w[e_].double().abs().sum(1) + 128 * dx[a:b] * dw[e_]
+        assert ((y[a:b].double() - want[a:b]).abs() <= slack + (2.0 ** -8 + 2.0 ** -22) * (want[a:b].abs() + slack)).all()
+    assert not y[90:].any()
