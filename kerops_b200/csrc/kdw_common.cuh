@@ -64,23 +64,26 @@ int device_sm_count(int* sms);
 // has completed and its writes are visible; under an ordinary launch the wait returns at once.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_overlapping_previous_smem(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem,
-                                                    cudaStream_t st, const Args&... args) {
+                                                    cudaStream_t st, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_overlapping_previous(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t st,
                                                Args... args) {
-    return launch_overlapping_previous_smem(kernel, grid, block, (size_t)0, st, args...);
+    return launch_overlapping_previous_smem(kernel, grid, block, (size_t)0, st, 1, args...);
 }
 #endif
 

@@ -4,7 +4,7 @@
 //   row products     out[t, :] = a[t, :] * B_g          for the rows t of group g   (forward, input gradient, int8)
 //   weight gradient  out[g]    = sum_t a[t, :]^T b[t, :] over the rows t of group g
 //
-// A UNIT is one output tile of 128 x BN and one share of its contraction.  Row groups end where the device array
+// A UNIT is one output tile of 128 x BN (a CTA) or 256 x BN (a pair of CTAs) and one share of its contraction.  Row groups end where the device array
 // `ends` says; every CTA scans it once into a table in shared memory (first row and first unit of each group), and a
 // unit index is found in it by bisection, so the host never waits for the row counts.
 #pragma once
@@ -16,7 +16,7 @@
 namespace kdw {
 
 constexpr int kLinMaxGroups = 1024;   // groups of one call: the table of a CTA holds them all
-constexpr int kLinTileM = 128;        // output rows of a tile = lanes of the accumulator
+constexpr int kLinTileM = 128;        // output rows of a CTA's tile = lanes of the accumulator
 constexpr int kLinSpan = 128;         // bytes of a shared-memory row = the swizzle span
 
 enum LinOp : int { LIN_FWD = 0, LIN_DGRAD = 1, LIN_WGRAD = 2 };
@@ -24,6 +24,7 @@ enum LinOp : int { LIN_FWD = 0, LIN_DGRAD = 1, LIN_WGRAD = 2 };
 struct LinParams {
     const int* ends;        // [E] cumulative row ends, or null: one group of all rows
     int T, E;               // rows, groups
+    int tile_m;             // output rows of a tile: 128, or 256 for a pair of CTAs
     int m_tiles;            // weight gradient: tiles along the output rows; row products: 0 (follows from the group)
     int n_tiles;            // tiles along the output columns
     int out_rows, out_cols; // weight gradient: rows of one output matrix; columns of the output
@@ -31,7 +32,7 @@ struct LinParams {
     int splits;             // row products: shares of the contraction
     int chunk;              // weight gradient: rows of one share (a multiple of 64)
     void* out;
-    float* partial;         // [unit][BN / 4][128] float4 sums of the shares, or null: every tile has one share
+    float* partial;         // [unit][tile_m / 128][BN / 4][128] float4 sums of the shares, or null: every tile has one share
     int* table;             // copy of the table for the kernel that adds the shares, or null
     const float* row_scale; // 8-bit operands: [T] and [E][out_cols]
     const float* col_scale;
@@ -65,7 +66,7 @@ __host__ __device__ __forceinline__ int lin_shares(const LinParams& p, int rows)
     return rows > p.chunk ? lin_ceil(rows, p.chunk) : 1;
 }
 __host__ __device__ __forceinline__ int lin_group_tiles(const LinParams& p, int rows) {
-    return (p.m_tiles ? p.m_tiles : lin_ceil(rows, kLinTileM)) * p.n_tiles;
+    return (p.m_tiles ? p.m_tiles : lin_ceil(rows, p.tile_m)) * p.n_tiles;
 }
 
 // Tiles of a group in bands of 16 tile rows, a band's rows fastest: the CTAs that run at the same time then share
@@ -84,28 +85,32 @@ __host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const i
     LinUnit r;
     r.g = lo;
     const int rows = row[lo + 1] - row[lo];
-    const int mt = p.m_tiles ? p.m_tiles : lin_ceil(rows, kLinTileM);
-    const int tiles = mt * p.n_tiles;
-    const int v = u - unit[lo];
-    const int share = v / tiles;
-    const int t = v - share * tiles;
-    const int band = t / (kLinBand * p.n_tiles);
-    const int inside = t - band * kLinBand * p.n_tiles;
-    const int high = mt - band * kLinBand < kLinBand ? mt - band * kLinBand : kLinBand;
-    const int nt = inside / high;
-    const int m = band * kLinBand + inside - nt * high;
+    const int mt = p.m_tiles ? p.m_tiles : lin_ceil(rows, p.tile_m);
+    const int shares = lin_shares(p, rows);
+    int share = 0, nt = 0, m = u - unit[lo];
+    if (shares > 1) {
+        const int tiles = mt * p.n_tiles;
+        share = m / tiles;
+        m -= share * tiles;
+    }
+    if (p.n_tiles > 1) {
+        const int band = m / (kLinBand * p.n_tiles);
+        const int inside = m - band * kLinBand * p.n_tiles;
+        const int high = mt - band * kLinBand < kLinBand ? mt - band * kLinBand : kLinBand;
+        nt = inside / high;
+        m = band * kLinBand + inside - nt * high;
+    }
     r.n0 = nt * BN;
     r.k_row = 0;
     r.k_rows = 0;
-    const int shares = lin_shares(p, rows);
     r.whole = shares == 1;
     if (p.m_tiles == 0) {
-        r.m0 = row[lo] + m * kLinTileM;
+        r.m0 = row[lo] + m * p.tile_m;
         r.row_end = row[lo + 1];
         r.kb = (int)((long long)p.k_blocks * share / shares);
         r.ke = (int)((long long)p.k_blocks * (share + 1) / shares);
     } else {
-        r.m0 = m * kLinTileM;
+        r.m0 = m * p.tile_m;
         r.row_end = p.out_rows;
         r.k_row = row[lo] + share * p.chunk;
         const int left = row[lo + 1] - r.k_row;
@@ -156,27 +161,42 @@ __device__ __forceinline__ void lin_build_table(const LinParams& p, int* row, in
     }
 }
 
+// Loads of a box; PAIR: the barrier may be the other CTA's (a shared::cluster address), as the two CTAs of a pair
+// report to one of them.
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_2d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
     if ((dst & 1023u) != 0) {
         atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
         return;
     }
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(tm), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+            ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(bar)
+            : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_3d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1,
                                             int c2) {
     if ((dst & 1023u) != 0) {
         atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
         return;
     }
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            dst),
-        "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+            "[%5];" ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+            ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+            : "memory");
 }
 
 // One lane of a converged warp.
@@ -190,37 +210,107 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+// Shared-memory address of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
 }
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrivals on another CTA's barrier.  Only the first makes this thread's writes to memory visible to the CTA that waits
+// (a fence of some 1500 cycles); the second follows tensor-memory loads, which tcgen05.fence orders, the third announces
+// bytes and has nothing to make visible.
+__device__ __forceinline__ void cluster_release_arrive(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void cluster_expect_tx(uint32_t cluster_bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
+                 : "memory");
+}
+// Bounded wait like mbar_wait_bounded; PAIR: also orders what the other CTA of the pair did before it arrived.
+template <bool PAIR>
+__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+    if constexpr (true) {
+        return mbar_wait_bounded(bar, parity, limit_ns);
+    } else {
+        unsigned long long t0 = 0;
+        for (uint32_t it = 0;; ++it) {
+            uint32_t ok;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(ok)
+                : "r"(bar), "r"(parity)
+                : "memory");
+            if (ok) return true;
+            if (it == 0) t0 = global_ns();
+            if ((it & 63u) == 63u && global_ns() - t0 > limit_ns) return false;
+        }
+    }
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Arrives on `bar` when the tensor-core work issued so far by this thread has finished.
+// Arrives on `bar` (PAIR: on that barrier of both CTAs) when the tensor-core work issued so far by this thread has
+// finished.
+template <bool PAIR>
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-template <bool I8>
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    if constexpr (I8)
+    if constexpr (PAIR)
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
             : "memory");
     else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-            : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+
+#define KDW_TC_MMA(group, kind)                                                              \
+    asm volatile(                                                                            \
+        "{\n\t.reg .pred p;\n\t"                                                             \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                          \
+        "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)                                       \
+        : "memory")
+template <bool I8, bool PAIR>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if constexpr (I8 && PAIR)
+        KDW_TC_MMA("2", "i8");
+    else if constexpr (I8)
+        KDW_TC_MMA("1", "i8");
+    else if constexpr (PAIR)
+        KDW_TC_MMA("2", "f16");
+    else
+        KDW_TC_MMA("1", "f16");
+}
+#undef KDW_TC_MMA
 
 // 32 accumulator columns of the calling warp's 32 lanes.
 __device__ __forceinline__ void tmem_load_32(uint32_t addr, uint32_t (&v)[32]) {

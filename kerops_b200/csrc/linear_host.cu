@@ -1,5 +1,8 @@
 // C entry points of the channel-mixing products: argument checks, the plan and the workspace layout.
+#include <stdlib.h>
+
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
@@ -31,20 +34,33 @@ int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
     pl->k_blocks = wgrad ? 0 : (int)ceil_div(con, k_elems);
     pl->splits = 1;
     pl->chunk = 0;
-    // Groups are rounded up to whole tiles: at most one tile row more per group than the rows fill.
-    const int64_t m_tiles = wgrad ? ceil_div(a.N, kLinTileM) : ceil_div(a.T, kLinTileM) + std::min(a.E, a.T) - 1;
-    pl->bn = 64;
+    // Tile and shares.  LINEAR_TILE (a build for measurements) fixes the tile.
+    const int64_t groups = std::min(a.E, a.T);
     double best = 1e300;
-    for (int bn : {256, 128, 64}) {
-        const int64_t n_tiles = ceil_div(pl->out_cols, bn);
-        const int64_t tiles = m_tiles * n_tiles * (wgrad ? a.E : 1);
-        // time of a CTA: its tiles times what a tile costs, in columns (a narrow tile re-reads the other operand)
-        const double cost = (double)ceil_div(tiles, sms) * (bn + 64);
-        if (cost < best) {
-            best = cost;
-            pl->bn = bn;
+    for (int tile_m : {256, 128})
+        for (int bn : {256, 128, 64}) {
+            if (tile_m == 256 && bn == 64) continue;
+            const int slots = tile_m == 256 ? sms / 2 : sms;
+            // Groups are rounded up to whole tiles: at most one tile row more per group than the rows fill, half of
+            // one on average.
+            const double m_tiles = wgrad ? (double)ceil_div(a.N, tile_m) * a.E
+                                         : std::max<double>((double)ceil_div(a.T, tile_m), (double)a.T / tile_m + 0.5 * groups);
+            const double tiles = m_tiles * ceil_div(pl->out_cols, bn);
+            // time of a CTA in columns: its tiles times what a tile costs
+            const double per_tile = tile_m == 256 ? bn + 32 : bn + (bn == 256 ? 96 : 64);
+            const double cost = std::ceil(tiles / slots) * per_tile;
+            if (cost < best) {
+                best = cost;
+                pl->bn = bn;
+                pl->tile_m = tile_m;
+            }
         }
+    if (const char* force = getenv("KDW_LINEAR_TILE")) {
+        pl->tile_m = atoi(force) / 1000;
+        pl->bn = atoi(force) % 1000;
     }
+    const int slots = pl->tile_m == 256 ? sms / 2 : sms;
+    const int64_t m_tiles = wgrad ? ceil_div(a.N, pl->tile_m) : ceil_div(a.T, pl->tile_m) + groups - 1;
     pl->n_tiles = (int)ceil_div(pl->out_cols, pl->bn);
     pl->m_tiles = wgrad ? (int)m_tiles : 0;
     const int64_t tiles = m_tiles * pl->n_tiles * (wgrad ? a.E : 1);
@@ -54,15 +70,15 @@ int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
     if (wgrad) {
         // shares of the rows so that every SM has work
         int64_t chunk = round_up(std::max<int64_t>(a.T, 1), 64);
-        if (tiles < 2 * sms && a.T > 512) {
-            const int64_t per_tile = std::max<int64_t>(1, 2 * sms / tiles);
+        if (tiles < 2 * slots && a.T > 512) {
+            const int64_t per_tile = std::max<int64_t>(1, 2 * slots / tiles);
             chunk = std::max<int64_t>(256, round_up(ceil_div(a.T, per_tile), 64));
         }
         pl->chunk = (int)std::min<int64_t>(chunk, 1 << 30);
         split = pl->chunk < a.T;
         if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
-    } else if (tiles * 2 <= sms && pl->k_blocks >= 8) {
-        pl->splits = (int)std::min<int64_t>(sms / tiles, pl->k_blocks / 4);
+    } else if (tiles * 2 <= slots && pl->k_blocks >= 8) {
+        pl->splits = (int)std::min<int64_t>(slots / tiles, pl->k_blocks / 4);
         split = pl->splits > 1;
         pl->max_units = tiles * pl->splits;
     }
@@ -81,7 +97,7 @@ int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
         pl->off_table = off;
         off = round_up(off + 2 * (a.E + 1) * 4, 256);
         pl->off_partial = off;
-        off += pl->max_units * kLinTileM * pl->bn * 4;
+        off += pl->max_units * pl->tile_m * pl->bn * 4;
     }
     pl->bytes = off;
     if (pl->max_units > INT32_MAX) {

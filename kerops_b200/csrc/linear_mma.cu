@@ -10,46 +10,56 @@ namespace kdw {
 
 // ------------------------------------------------------------------------------------------------------------------
 // The product kernel.  One persistent CTA per SM: warp 0 loads operand tiles with TMA into a ring of stages, warp 1
-// issues the tensor-core products into one of two accumulators in tensor memory, warps 4-7 bring finished accumulators
-// to memory while the next tile is being multiplied, warps 2-3 clear the output rows behind the last group.
+// issues the tensor-core products into accumulators in tensor memory, warps 4-7 and 8-11 take finished accumulators in
+// turn and bring them to memory while the next tiles are being multiplied, warps 2-3 clear the output rows behind the
+// last group.
 //   A_ROWS / B_ROWS: the operand is stored with its output index contiguous (the contraction runs along memory rows)
+//   PAIR: two CTAs of a cluster share a 256 x BN tile.  Each loads its 128 rows of A and half of B's columns; the tensor
+//         cores of both read both halves of B, so a byte that enters shared memory is used for twice the products.  CTA 0
+//         waits for the loads of both and issues the products.
 // ------------------------------------------------------------------------------------------------------------------
-template <bool I8_, bool A_ROWS_, bool B_ROWS_, int BN_>
+template <bool I8_, bool A_ROWS_, bool B_ROWS_, int BN_, bool PAIR_>
 struct LCfg {
-    static constexpr bool I8 = I8_, A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, WGRAD = A_ROWS_;
+    static constexpr bool I8 = I8_, A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, WGRAD = A_ROWS_, PAIR = PAIR_;
     static constexpr int BN = BN_;
-    static constexpr int THREADS = 256;
+    static constexpr int LOAD_N = PAIR ? BN / 2 : BN;  // columns of B that a CTA loads
+    static constexpr int THREADS = 384;
     static constexpr int A_BYTES = kLinTileM * kLinSpan;
-    static constexpr int B_BYTES = BN * kLinSpan;
+    static constexpr int B_BYTES = LOAD_N * kLinSpan;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 196608 / STAGE;
-    static constexpr int PITCH = 144;  // staged output rows: 64 values and 16 bytes more, free of bank conflicts
-    static constexpr int STAGING = 4 * 32 * PITCH;
-    static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + (int)sizeof(LinTable) + (2 * STAGES + 5) * 8 + 16;
+    static constexpr int SCOLS = BN == 256 ? 32 : 64;  // output columns staged at a time
+    static constexpr int PITCH = SCOLS * 2 + 16;       // bytes of a staged row: free of bank conflicts
+    static constexpr int STAGING = 8 * 32 * PITCH;
+    static constexpr int STAGES = (232448 - 1024 - STAGING - (int)sizeof(LinTable) - 512) / STAGE;
+    static constexpr int ACCS = BN == 256 ? 2 : 4;
+    static constexpr int TMEM_COLS = ACCS * BN;
+    static constexpr int BARS = 3 * STAGES + 2 * ACCS + 1;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + (int)sizeof(LinTable) + BARS * 8 + 16;
     static constexpr int K_ELEMS = I8 ? 128 : 64;  // contraction steps of a stage
-    static_assert(TMEM_COLS >= 32 && TMEM_COLS <= 512, "");
-    static_assert(SMEM <= 232448, "");
+    static_assert(LOAD_N >= 64 && TMEM_COLS >= 32 && TMEM_COLS <= 512, "");
+    static_assert(SMEM <= 232448 && BARS * 8 + 16 <= 512, "");
 };
 
-// Writes `rows` x `cols` (<= 64) staged 16-bit values of one warp to memory.
-__device__ __forceinline__ void store_staged(const char* stage, int pitch, char* dst, long long dst_pitch, int rows, int cols,
-                                             bool vec, int lane) {
-    if (vec) {  // 16-byte pieces, eight lanes to a row of 64 values
-        const int c = lane & 7;
+// Writes `rows` x `cols` (<= SCOLS) staged 16-bit values of one warp to memory.
+template <int SCOLS, int PITCH>
+__device__ __forceinline__ void store_staged(const char* stage, char* dst, long long dst_pitch, int rows, int cols, bool vec,
+                                             int lane) {
+    if (vec) {  // 16-byte pieces, SCOLS / 8 lanes to a row
+        constexpr int LPR = SCOLS / 8;
+        const int c = lane % LPR;
         if (c * 8 < cols) {
 #pragma unroll
-            for (int r = lane >> 3; r < 32; r += 4) {
+            for (int r = lane / LPR; r < 32; r += 32 / LPR) {
                 if (r < rows)
                     *reinterpret_cast<uint4*>(dst + r * dst_pitch + c * 16) =
-                        *reinterpret_cast<const uint4*>(stage + r * pitch + c * 16);
+                        *reinterpret_cast<const uint4*>(stage + r * PITCH + c * 16);
             }
         }
     } else {
         for (int r = 0; r < rows; ++r)
             for (int c = lane; c < cols; c += 32)
                 *reinterpret_cast<uint16_t*>(dst + r * dst_pitch + c * 2) =
-                    *reinterpret_cast<const uint16_t*>(stage + r * pitch + c * 2);
+                    *reinterpret_cast<const uint16_t*>(stage + r * PITCH + c * 2);
     }
 }
 
@@ -77,34 +87,37 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     char* const base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     char* const staging = base + C::STAGES * C::STAGE;
     LinTable* const tab = reinterpret_cast<LinTable*>(staging + C::STAGING);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(
-        reinterpret_cast<char*>(tab) + (sizeof(LinTable) + 7) / 8 * 8);
-    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 5);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(tab + 1);
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + C::BARS);
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES,
-                   acc_empty = acc_full + 16, drain = acc_empty + 16;
+                   acc_empty = acc_full + 8 * C::ACCS, drain = acc_empty + 8 * C::ACCS, partly = drain + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = C::PAIR ? cluster_rank() : 0;
+    const int first = C::PAIR ? blockIdx.x >> 1 : blockIdx.x, step = C::PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&map_a);
         prefetch_tmap(&map_b);
         for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(full + 8 * i, 1);
+            mbar_init(full + 8 * i, C::PAIR ? 2 : 1);
             mbar_init(empty + 8 * i, 1);
+            mbar_init(partly + 8 * i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < C::ACCS; ++i) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, 4);
+            mbar_init(acc_empty + 8 * i, C::PAIR ? 8 : 4);
         }
         mbar_init(drain, 1);
         mbar_fence_init();
     } else if (warp == 1) {
-        tmem_alloc(smem_u32(s_tmem), C::TMEM_COLS);
+        tmem_alloc<C::PAIR>(smem_u32(s_tmem), C::TMEM_COLS);
     }
     // operands, scales and `ends` may be the work of the kernel before this one
     grid_dependency_wait();
     if (warp == 2) lin_build_table(p, tab->row, tab->unit, lane);
     tc_fence_before();
     __syncthreads();
+    if (C::PAIR) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     const int units = tab->unit[p.E];
@@ -114,36 +127,46 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             int loads = 0, stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            for (int u = first; u < units && ok; u += step) {
                 const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+                const int m0 = w.m0 + (int)rank * kLinTileM, n0 = w.n0 + (int)rank * C::LOAD_N;
                 for (int k = w.kb; k < w.ke; ++k) {
                     if (p.stop_after >= 0 && loads >= p.stop_after) {
                         ok = false;
                         break;
                     }
-                    if (!mbar_wait_bounded(empty + 8 * stage, phase ^ 1, p.limit_ns)) {
+                    if (!lin_wait<C::PAIR>(empty + 8 * stage, phase ^ 1, p.limit_ns)) {
                         atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                         ok = false;
                         break;
                     }
-                    const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES, bar = full + 8 * stage;
-                    mbar_expect_tx(bar, C::STAGE);
+                    const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES;
+                    uint32_t bar = full + 8 * stage;
+                    if (rank == 0) {
+                        mbar_expect_tx(bar, C::STAGE);
+                    } else if (C::WGRAD && w.k_rows - k * 64 < 64) {
+                        bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
+                        mbar_expect_tx(bar, C::STAGE);
+                    } else {
+                        bar = cluster_addr(bar, 0);  // CTA 0 waits for the loads of both
+                        cluster_expect_tx(bar, C::STAGE);
+                    }
                     if constexpr (C::WGRAD) {
                         const int r = w.k_row + k * 64;
 #pragma unroll
                         for (int j = 0; j < kLinTileM / 64; ++j)
-                            tma_load_2d(p.status, a + j * 8192, &map_a, bar, w.m0 + j * 64, r);
+                            tma_load_2d<C::PAIR>(p.status, a + j * 8192, &map_a, bar, m0 + j * 64, r);
 #pragma unroll
-                        for (int j = 0; j < C::BN / 64; ++j)
-                            tma_load_2d(p.status, b + j * 8192, &map_b, bar, w.n0 + j * 64, r);
+                        for (int j = 0; j < C::LOAD_N / 64; ++j)
+                            tma_load_2d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, r);
                     } else {
-                        tma_load_2d(p.status, a, &map_a, bar, k * C::K_ELEMS, w.m0);
+                        tma_load_2d<C::PAIR>(p.status, a, &map_a, bar, k * C::K_ELEMS, m0);
                         if constexpr (C::B_ROWS) {
 #pragma unroll
-                            for (int j = 0; j < C::BN / 64; ++j)
-                                tma_load_3d(p.status, b + j * 8192, &map_b, bar, w.n0 + j * 64, k * 64, w.g);
+                            for (int j = 0; j < C::LOAD_N / 64; ++j)
+                                tma_load_3d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, k * 64, w.g);
                         } else {
-                            tma_load_3d(p.status, b, &map_b, bar, k * C::K_ELEMS, w.n0, w.g);
+                            tma_load_3d<C::PAIR>(p.status, b, &map_b, bar, k * C::K_ELEMS, n0, w.g);
                         }
                     }
                     ++loads;
@@ -153,73 +176,86 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                     }
                 }
             }
-            // a CTA leaves only when its last copies have landed
-            const int last = loads < C::STAGES ? loads : C::STAGES;
-            for (int i = 0; i < last; ++i) {
-                if (stage == 0) {
-                    stage = C::STAGES;
-                    phase ^= 1;
+            // a CTA (a pair) leaves only when its last copies have landed
+            if (rank == 0) {
+                const int last = loads < C::STAGES ? loads : C::STAGES;
+                for (int i = 0; i < last; ++i) {
+                    if (stage == 0) {
+                        stage = C::STAGES;
+                        phase ^= 1;
+                    }
+                    --stage;
+                    if (!lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns))
+                        atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                 }
-                --stage;
-                if (!mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         int stage = 0, acc = 0;
-        uint32_t phase = 0, acc_phase = 0;
+        uint32_t phase = 0, acc_phase = 0, partly_phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int u = first; u < units && ok; u += step) {
             const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
             if (w.kb == w.ke) continue;
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
-            if (!ok) break;
-            tc_fence_after();
+            if (rank == 0) {
+                ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
+                if (!ok) break;
+                tc_fence_after();
+            }
             const uint32_t d = tmem + acc * C::BN;
             for (int k = w.kb; k < w.ke; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns));
-                if (!ok) break;
                 char* const sa = base + stage * C::STAGE;
-                if constexpr (C::WGRAD) {
-                    // rows beyond the share are another group's (or of no group): their products must vanish even
-                    // where one of the factors is a NaN or an infinity, so both operands are cleared
-                    const int valid = w.k_rows - k * 64;
-                    if (valid < 64) {
-                        for (int i = valid * 8 + lane; i < 512; i += 32)
+                // rows beyond the share are another group's (or of no group): their products must vanish even where
+                // one of the factors is a NaN or an infinity, so both operands are cleared
+                const int valid = C::WGRAD ? w.k_rows - k * 64 : 64;
+                if (rank == 0 || valid < 64) {
+                    ok = rank == 0 ? lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns)
+                                   : lin_wait<C::PAIR>(partly + 8 * stage, partly_phase >> stage & 1, p.limit_ns);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
+                if (C::WGRAD && valid < 64) {
+                    for (int i = valid * 8 + lane; i < 512; i += 32)
 #pragma unroll
-                            for (int j = 0; j < C::STAGE / 8192; ++j)
-                                *reinterpret_cast<uint4*>(sa + j * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
-                        fence_proxy_async_smem();
-                        __syncwarp();
+                        for (int j = 0; j < C::STAGE / 8192; ++j)
+                            *reinterpret_cast<uint4*>(sa + j * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (rank != 0) {
+                        partly_phase ^= 1u << stage;  // one parity bit per stage
+                        if (lane == 0) cluster_release_arrive(cluster_addr(full + 8 * stage, 0));
                     }
                 }
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t da = smem_desc(smem_u32(sa), C::A_ROWS);
-                    const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ROWS);
+                if (rank == 0) {
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t da = smem_desc(smem_u32(sa), C::A_ROWS);
+                        const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ROWS);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc_mma<C::I8>(d, da + i * (C::A_ROWS ? 2048 >> 4 : 32 >> 4), db + i * (C::B_ROWS ? 2048 >> 4 : 32 >> 4),
-                                      p.idesc, k > w.kb || i > 0);
-                    tc_commit(empty + 8 * stage);
-                    if (k + 1 == w.ke) tc_commit(acc_full + 8 * acc);
+                        for (int i = 0; i < 4; ++i)
+                            tc_mma<C::I8, C::PAIR>(d, da + i * (C::A_ROWS ? 2048 >> 4 : 32 >> 4),
+                                                   db + i * (C::B_ROWS ? 2048 >> 4 : 32 >> 4), p.idesc, k > w.kb || i > 0);
+                        tc_commit<C::PAIR>(empty + 8 * stage);
+                        if (k + 1 == w.ke) tc_commit<C::PAIR>(acc_full + 8 * acc);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 if (++stage == C::STAGES) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
-            if (++acc == 2) {
+            if (++acc == C::ACCS) {
                 acc = 0;
                 acc_phase ^= 1;
             }
         }
         if (!ok && lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         // products in flight still read shared memory and write tensor memory
-        if (elect_one()) {
-            tc_commit(drain);
-            if (!mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        if (rank == 0 && elect_one()) {
+            tc_commit<C::PAIR>(drain);
+            if (!lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         }
         __syncwarp();
     } else if (warp < 4) {
@@ -230,22 +266,31 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 p.table[p.E + 1 + i] = tab->unit[i];
             }
     } else {
-        const int q = warp & 3;
-        char* const stg = staging + q * 32 * C::PITCH;
-        int acc = 0;
+        const int q = warp & 3, turn = (warp >> 2) - 1;
+        char* const stg = staging + (warp - 4) * 32 * C::PITCH;
+        int acc = 0, count = 0;  // accumulators used so far: the two groups of warps take them in turn
         uint32_t acc_phase = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        for (int u = first; u < units; u += step) {
             const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
             const bool any = w.ke > w.kb;
+            const bool mine = (count & 1) == turn;
+            if (any) ++count;
+            if (!mine) {
+                if (any && ++acc == C::ACCS) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
+                continue;
+            }
             if (any) {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * acc, acc_phase, p.limit_ns))) {
+                if (!__all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_full + 8 * acc, acc_phase, p.limit_ns))) {
                     if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                     break;
                 }
                 tc_fence_after();
             }
             const uint32_t d = tmem + acc * C::BN + ((uint32_t)(q * 32) << 16);
-            const int row0 = w.m0 + q * 32;
+            const int row0 = w.m0 + (int)rank * kLinTileM + q * 32;
             int rows = w.row_end - row0;
             rows = rows > 32 ? 32 : rows;
             if (w.whole || !p.partial) {
@@ -256,12 +301,12 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 if (C::I8) rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.f;
                 const float* cs = C::I8 ? p.col_scale + (long long)w.g * p.out_cols : nullptr;
 #pragma unroll 1
-                for (int c0 = 0; c0 < C::BN; c0 += 64) {
+                for (int c0 = 0; c0 < C::BN; c0 += C::SCOLS) {
                     int cols = p.out_cols - w.n0 - c0;
                     if (cols <= 0 || rows <= 0) break;
-                    cols = cols > 64 ? 64 : cols;
+                    cols = cols > C::SCOLS ? C::SCOLS : cols;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < C::SCOLS / 32; ++h) {
                         uint32_t v[32];
                         if (any) {
                             tmem_load_32(d + c0 + h * 32, v);
@@ -292,13 +337,14 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         }
                     }
                     __syncwarp();
-                    store_staged(stg, C::PITCH, out + row0 * pitch + (long long)(w.n0 + c0) * 2, pitch, rows, cols,
-                                 p.out_vec, lane);
+                    store_staged<C::SCOLS, C::PITCH>(stg, out + row0 * pitch + (long long)(w.n0 + c0) * 2, pitch, rows, cols,
+                                                     p.out_vec, lane);
                     __syncwarp();
                 }
             } else {
                 // a share of a tile: column quadruples of a row side by side over the rows
-                uint4* out = reinterpret_cast<uint4*>(p.partial) + (long long)u * (C::BN / 4) * kLinTileM + q * 32 + lane;
+                uint4* out = reinterpret_cast<uint4*>(p.partial) +
+                             ((long long)u * (C::PAIR ? 2 : 1) + rank) * (C::BN / 4) * kLinTileM + q * 32 + lane;
 #pragma unroll 1
                 for (int c0 = 0; c0 < C::BN; c0 += 32) {
                     uint32_t v[32];
@@ -311,8 +357,13 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             if (any) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8 * acc);
-                if (++acc == 2) {
+                if (lane == 0) {
+                    if (C::PAIR)
+                        cluster_arrive(cluster_addr(acc_empty + 8 * acc, 0));
+                    else
+                        mbar_arrive(acc_empty + 8 * acc);
+                }
+                if (++acc == C::ACCS) {
                     acc = 0;
                     acc_phase ^= 1;
                 }
@@ -321,8 +372,9 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     }
     tc_fence_before();
     __syncthreads();
+    if (C::PAIR) cluster_sync();
     tc_fence_after();
-    if (warp == 1) tmem_free(tmem, C::TMEM_COLS);
+    if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
 }
 
 // Adds the shares of the tiles that have several, in their order, and rounds once.  A CTA takes 32 columns of one tile.
@@ -330,7 +382,7 @@ template <bool I8>
 __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__ LinParams p, int BN) {
     __shared__ float s[kLinTileM][33];
     grid_dependency_wait();
-    const int slices = BN / 32;
+    const int halves = p.tile_m / kLinTileM, slices = BN / 32 * halves;
     const int* row = p.table;
     const int* unit = p.table + p.E + 1;
     const int tid = threadIdx.x;
@@ -347,15 +399,17 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
         if (g == p.E) return;
         if (shares == 1) continue;
         const int u = unit[g] + t;
-        const LinUnit w = lin_unit(p, row, unit, u, BN);
-        const int c0 = (i % slices) * 32;
+        LinUnit w = lin_unit(p, row, unit, u, BN);
+        const int half_m = (i % slices) / (BN / 32);
+        w.m0 += half_m * kLinTileM;
+        const int c0 = (i % (BN / 32)) * 32;
         int cols = p.out_cols - w.n0 - c0;
         cols = cols > 32 ? 32 : cols;
         if (cols <= 0) continue;
         const int r = tid & 127, half = tid >> 7;  // the thread's row and which 16 of the 32 columns
-        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + (long long)u * (BN / 4) * kLinTileM +
+        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + ((long long)u * halves + half_m) * (BN / 4) * kLinTileM +
                            (long long)(c0 / 4 + half * 4) * kLinTileM + r;
-        const long long step = (long long)tiles * (BN / 4) * kLinTileM;
+        const long long step = (long long)tiles * halves * (BN / 4) * kLinTileM;
         float f[16];
         int n[16];
 #pragma unroll
@@ -380,6 +434,7 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
                 }
             }
         int rows = w.row_end - w.m0;
+        if (rows <= 0) continue;
         rows = rows > kLinTileM ? kLinTileM : rows;
         if (I8) {
             const float rs = r < rows ? __ldg(p.row_scale + w.m0 + r) : 0.f;
@@ -437,11 +492,12 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     int sms = 0, occ = 0;
     int rc = setup.get((const void*)linear_kernel<C>, C::THREADS, C::SMEM, &sms, &occ);
     if (rc) return rc;
-    const int grid = pl.max_units < sms ? (pl.max_units > 0 ? (int)pl.max_units : 1) : sms;
-    KDW_CUDA(launch_overlapping_previous_smem(linear_kernel<C>, (unsigned)grid, (unsigned)C::THREADS, (size_t)C::SMEM, st, ma,
-                                              mb, p));
+    const int slots = C::PAIR ? sms / 2 : sms;
+    const int grid = (pl.max_units < slots ? (pl.max_units > 0 ? (int)pl.max_units : 1) : slots) * (C::PAIR ? 2 : 1);
+    KDW_CUDA(launch_overlapping_previous_smem(linear_kernel<C>, (unsigned)grid, (unsigned)C::THREADS, (size_t)C::SMEM, st,
+                                              C::PAIR ? 2 : 1, ma, mb, p));
     if (p.partial) {
-        const long long blocks = pl.max_tiles * (C::BN / 32);
+        const long long blocks = pl.max_tiles * (C::BN / 32) * (p.tile_m / kLinTileM);
         KDW_CUDA(launch_overlapping_previous(linear_sum_kernel<C::I8>, (unsigned)(blocks < 4 * sms ? blocks : 4 * sms), 256u,
                                              st, p, C::BN));
     }
@@ -451,10 +507,13 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
 template <bool I8, bool AR, bool BR>
 static int launch_width(const LinPlan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const LinParams& p,
                         cudaStream_t st) {
+    if (pl.tile_m == 256)
+        return pl.bn == 128 ? launch_product<LCfg<I8, AR, BR, 128, true>>(pl, ma, mb, p, st)
+                            : launch_product<LCfg<I8, AR, BR, 256, true>>(pl, ma, mb, p, st);
     switch (pl.bn) {
-        case 64: return launch_product<LCfg<I8, AR, BR, 64>>(pl, ma, mb, p, st);
-        case 128: return launch_product<LCfg<I8, AR, BR, 128>>(pl, ma, mb, p, st);
-        default: return launch_product<LCfg<I8, AR, BR, 256>>(pl, ma, mb, p, st);
+        case 64: return launch_product<LCfg<I8, AR, BR, 64, false>>(pl, ma, mb, p, st);
+        case 128: return launch_product<LCfg<I8, AR, BR, 128, false>>(pl, ma, mb, p, st);
+        default: return launch_product<LCfg<I8, AR, BR, 256, false>>(pl, ma, mb, p, st);
     }
 }
 
@@ -499,6 +558,7 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     p.ends = a.ends;
     p.T = (int)a.T;
     p.E = (int)a.E;
+    p.tile_m = pl.tile_m;
     p.m_tiles = pl.m_tiles;
     p.n_tiles = pl.n_tiles;
     p.out_rows = pl.out_rows;
@@ -521,7 +581,7 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     // accumulator fp32 (1) or int32 (2); operands fp16 (0) / bf16 (1) / int8 (1); which are stored by output index
     const uint32_t fmt = pl.esize == 1 ? 1u : (uint32_t)a.in_bf16;
     p.idesc = (pl.esize == 1 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)wgrad << 15 | (uint32_t)b_rows << 16 |
-              (uint32_t)(pl.bn >> 3) << 17 | (uint32_t)(kLinTileM >> 4) << 24;
+              (uint32_t)(pl.bn >> 3) << 17 | (uint32_t)(pl.tile_m >> 4) << 24;
     CUtensorMap ma, mb;
     const int span = kLinSpan / pl.esize;
     rc = encode_rows_map(&ma, pa, pl.esize, pl.a_cols, pl.a_rows, sa, 0, 0, span, wgrad ? 64 : kLinTileM);
@@ -530,7 +590,7 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
         rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows, sb, 0, 0, 64, 64);
     else
         rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows / a.E, sb, a.E, pl.b_rows / a.E * sb, span,
-                             b_rows ? 64 : pl.bn);
+                             b_rows ? 64 : pl.tile_m == 256 ? pl.bn / 2 : pl.bn);
     if (rc) return rc;
     if (pl.esize == 1) return launch_width<true, false, false>(pl, ma, mb, p, st);
     if (wgrad) return launch_width<false, true, true>(pl, ma, mb, p, st);

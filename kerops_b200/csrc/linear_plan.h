@@ -21,7 +21,7 @@ struct LinArgs {
 };
 
 struct LinPlan {
-    int esize, bn;
+    int esize, bn, tile_m;  // tile_m 256: a pair of CTAs to a tile
     int m_tiles, n_tiles, out_rows, out_cols, k_blocks, splits, chunk;
     bool pack_a, pack_b;
     int64_t a_rows, a_cols, a_pitch, b_rows, b_cols, b_pitch;  // pitches of the packed copies, in elements
