@@ -63,11 +63,11 @@ int device_sm_count(int* sms);
 // grid_dependency_wait() before it touches anything the previous kernel wrote - the wait returns when that kernel
 // has completed and its writes are visible; under an ordinary launch the wait returns at once.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_overlapping_previous_smem(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem,
+inline cudaError_t launch_overlapping_previous_grid(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                                     cudaStream_t st, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2] = {};
@@ -83,7 +83,7 @@ inline cudaError_t launch_overlapping_previous_smem(void (*kernel)(KArgs...), un
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_overlapping_previous(void (*kernel)(KArgs...), unsigned grid, unsigned block, cudaStream_t st,
                                                Args... args) {
-    return launch_overlapping_previous_smem(kernel, grid, block, (size_t)0, st, 1, args...);
+    return launch_overlapping_previous_grid(kernel, dim3(grid), dim3(block), (size_t)0, st, 1, args...);
 }
 #endif
 

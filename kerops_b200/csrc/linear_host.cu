@@ -153,6 +153,8 @@ static int f16_args(LinArgs* a, int op, const void* pa, const void* pb, int64_t 
     return 0;
 }
 
+static bool is_few(const LinArgs& a) { return a.op == LIN_FWD && a.T <= kFewRows; }
+
 // The 8-bit product: the rows are int8 with their scales, or 16-bit rows that are quantised into the workspace first.
 struct I8Layout {
     int64_t q_pitch, off_scale, off_rest;  // bytes; quantised rows at 0
@@ -196,6 +198,11 @@ static int i8_args(LinArgs* a, I8Layout* l, const void* x, const void* w, int64_
     return 0;
 }
 
+// Few 16-bit rows that every CTA of the product quantises itself.
+static bool quant_inside(const LinArgs& a, int x_type) {
+    return x_type != KDW_I8 && a.T <= kFewQuantRows && (a.K + 127) / 128 * 128 + 64 <= kFewQuantPitch;
+}
+
 static int plan_and_run(LinArgs* a, void* workspace, int64_t workspace_bytes, void* stream) {
     LinPlan pl;
     int sms = 0;
@@ -222,6 +229,7 @@ int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int
     int sms = 0;
     int rc = f16_args(&args, op, a, b, T, E, K, N, a_stride, b_stride, dtype);
     if (!rc) rc = device_sm_count(&sms);
+    if (!rc && is_few(args)) return 0;
     if (!rc) rc = linear_plan(&pl, args, sms);
     return rc ? (rc < 0 ? rc : -rc) : pl.bytes;
 }
@@ -243,6 +251,7 @@ int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_
     }
     args.out = out;
     args.ends = ends;
+    if (is_few(args)) return linear_few(args, dtype, (cudaStream_t)stream);
     return plan_and_run(&args, workspace, workspace_bytes, stream);
 }
 
@@ -255,6 +264,7 @@ int64_t kdw_linear_i8_workspace_bytes(const void* x, const void* w, int64_t T, i
     int sms = 0;
     int rc = i8_args(&args, &l, x, w, T, E, K, N, x_stride, x_type, dtype);
     if (!rc) rc = device_sm_count(&sms);
+    if (!rc && is_few(args)) return quant_inside(args, x_type) ? 0 : l.off_rest;
     if (!rc) rc = linear_plan(&pl, args, sms);
     return rc ? (rc < 0 ? rc : -rc) : l.off_rest + pl.bytes;
 }
@@ -281,6 +291,11 @@ int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const fl
     args.row_scale = x_scale;
     args.col_scale = w_scale;
     char* ws = (char*)workspace;
+    if (is_few(args) && quant_inside(args, x_type)) {
+        args.a = x;
+        args.a_stride = x_stride;
+        return linear_few(args, x_type, (cudaStream_t)stream);
+    }
     if (x_type != KDW_I8) {
         if (!workspace || workspace_bytes < l.off_rest || ((uintptr_t)workspace & 255) != 0) {
             set_error("linear_i8: workspace of at least %lld bytes (256-byte aligned) needed", (long long)l.off_rest);
@@ -293,6 +308,7 @@ int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const fl
         if (rc) return rc;
         ws += l.off_rest;
     }
+    if (is_few(args)) return linear_few(args, KDW_I8, (cudaStream_t)stream);
     return plan_and_run(&args, ws, workspace_bytes - l.off_rest, stream);
 }
 

@@ -494,7 +494,7 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     if (rc) return rc;
     const int slots = C::PAIR ? sms / 2 : sms;
     const int grid = (pl.max_units < slots ? (pl.max_units > 0 ? (int)pl.max_units : 1) : slots) * (C::PAIR ? 2 : 1);
-    KDW_CUDA(launch_overlapping_previous_smem(linear_kernel<C>, (unsigned)grid, (unsigned)C::THREADS, (size_t)C::SMEM, st,
+    KDW_CUDA(launch_overlapping_previous_grid(linear_kernel<C>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, st,
                                               C::PAIR ? 2 : 1, ma, mb, p));
     if (p.partial) {
         const long long blocks = pl.max_tiles * (C::BN / 32) * (p.tile_m / kLinTileM);

@@ -33,6 +33,11 @@ struct LinPlan {
 int linear_plan(LinPlan* pl, const LinArgs& a, int sms);
 int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st);
 
+// Products of few rows, without a workspace (linear_few.cu).  x_type: KDW_I8, or 16-bit rows to quantise within the kernel.
+constexpr int kFewRows = 32;
+constexpr int kFewQuantRows = 8, kFewQuantPitch = 128 * 96 + 64;  // rows and bytes of a row that a CTA quantises itself
+int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
+
 // Quantises rows of 16-bit values (see quant_rows.cu); q_padded: what lies between `cols` and q_stride may be written.
 int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride, int bf16,
                bool q_padded, cudaStream_t st);

@@ -1,14 +1,18 @@
 """Argument marshalling of the channel-mixing products between torch tensors and the C-ABI (include/kdw.h)."""
+import functools
+
 import torch
 
 from ... import _lib
-from ..conv._launch import _on, _stream_ptr
+from ..conv._launch import _on
 
 # torch dtype -> KDW_F16 / KDW_BF16 (include/kdw.h)
 TYPES = {torch.float16: 0, torch.bfloat16: 1}
 INT8 = 2  # KDW_I8
 FWD, DGRAD, WGRAD = 0, 1, 2
 MAX_GROUPS = 1024
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index; torch.cuda.current_stream costs 2 us more
 
 
 def as_rows(t, name):
@@ -43,41 +47,59 @@ def check_ends(ends, groups, device):
     assert ends.device == device, 'ends must be on the device of the rows'
 
 
+# The workspace depends on sizes and on the operands' alignment to 16 bytes alone; asking the library costs more than the
+# rest of a small call.
+@functools.lru_cache(maxsize=4096)
+def _product_workspace(device, op, a_align, b_align, T, E, K, N, sa, sb, dtype):
+    n = _lib.load().kdw_linear_f16_workspace_bytes(op, 4096 + a_align, 4096 + b_align, T, E, K, N, sa, sb, dtype)
+    if n < 0:
+        _lib.check(int(n))
+    return n
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_workspace(device, x_align, w_align, T, E, K, N, sx, x_type, dtype):
+    n = _lib.load().kdw_linear_i8_workspace_bytes(4096 + x_align, 4096 + w_align, T, E, K, N, sx, x_type, dtype)
+    if n < 0:
+        _lib.check(int(n))
+    return n
+
+
 def product(op, a, b, out, ends, T, E, K, N):
     """Enqueues one product (FWD | DGRAD | WGRAD) of 16-bit operands on a's device / current stream."""
     lib = _lib.load()
+    device = a.device
     dtype = TYPES[a.dtype]
     sa, sb = row_stride(a), row_stride(b) if op == WGRAD else K
     pa, pb = a.data_ptr(), b.data_ptr()
-    with _on(a.device):
-        nbytes = lib.kdw_linear_f16_workspace_bytes(op, pa, pb, T, E, K, N, sa, sb, dtype)
-        if nbytes < 0:
-            _lib.check(int(nbytes))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    with _on(device):
+        nbytes = _product_workspace(device.index, op, pa & 15, pb & 15, T, E, K, N, sa, sb, dtype)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = lib.kdw_linear_f16(
-            op, pa, pb, out.data_ptr(), ends.data_ptr() if ends is not None else None,
-            ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sa, sb, dtype, _stream_ptr(a.device),
+            op, pa, pb, out.data_ptr(), None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None,
+            nbytes, T, E, K, N, sa, sb, dtype, _raw_stream(device.index),
         )
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
     return out
 
 
 def int8_product(x, x_scale, weight, w_scale, y, ends, T, E, K, N):
     """Enqueues y = Int8Linear(x); x is int8 with x_scale, or 16-bit (x_scale None)."""
     lib = _lib.load()
+    device = x.device
     x_type, dtype, sx = TYPES.get(x.dtype, INT8), TYPES[y.dtype], row_stride(x)
     px, pw = x.data_ptr(), weight.data_ptr()
-    with _on(x.device):
-        nbytes = lib.kdw_linear_i8_workspace_bytes(px, pw, T, E, K, N, sx, x_type, dtype)
-        if nbytes < 0:
-            _lib.check(int(nbytes))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    with _on(device):
+        nbytes = _int8_workspace(device.index, px & 15, pw & 15, T, E, K, N, sx, x_type, dtype)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = lib.kdw_linear_i8(
-            px, x_scale.data_ptr() if x_scale is not None else None, pw, w_scale.data_ptr(), y.data_ptr(),
-            ends.data_ptr() if ends is not None else None, ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx,
-            x_type, dtype, _stream_ptr(x.device),
+            px, None if x_scale is None else x_scale.data_ptr(), pw, w_scale.data_ptr(), y.data_ptr(),
+            None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx, x_type,
+            dtype, _raw_stream(device.index),
         )
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
     return y
 
 
@@ -86,5 +108,5 @@ def quant_rows(x, q, scale):
     lib = _lib.load()
     with _on(x.device):
         rc = lib.kdw_quant_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr(), x.shape[0], x.shape[1], row_stride(x),
-                                TYPES[x.dtype], _stream_ptr(x.device))
+                                TYPES[x.dtype], _raw_stream(x.device.index))
     _lib.check(rc)

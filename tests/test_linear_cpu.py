@@ -90,7 +90,7 @@ def test_c_entry_points_refuse_bad_arguments(kdw_lib):
                dict(dt=2), dict(sx=15), dict(T=0)):
         assert call8(**kw) == -1, kw
     assert call8(xs=P + 2) == call8(ws=P + 1) == call8(y=P + 1) == call8(xt=0, x=P + 1) == -2
-    assert call8(xt=0) == -3 and b'workspace' in kdw_lib.kdw_last_error()
+    assert call8(xt=0, T=400) == -3 and b'workspace' in kdw_lib.kdw_last_error()
     assert q(None, P, P, 1, 8, 8, 0, None) == q(P, P, P, 0, 8, 8, 0, None) == q(P, P, P, 1, 8, 7, 0, None) == -1
     assert q(P, P, P, 1, 8, 8, 2, None) == -1 and q(P + 1, P, P, 1, 8, 8, 0, None) == -2
     assert kdw_lib.kdw_linear_f16_workspace_bytes(0, P, P, 0, 1, 8, 8, 8, 8, 0) == -1
