@@ -16,7 +16,7 @@ CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'include')
 LIB = os.path.join(CSRC, 'libkdw.so')
 SOURCES = ['kdw_host.cu', 'dwconv_fprop.cu', 'dwconv_fprop_mma.cu', 'dwconv_wgrad.cu', 'dwconv_wgrad_mma.cu', 'grad_allreduce.cu', 'dwconv_fprop_addstats.cu', 'dwconv_fprop_bnrelu.cu',
-           'linear_host.cu', 'linear_mma.cu', 'linear_few.cu', 'quant_rows.cu']
+           'linear_host.cu', 'linear_mma.cu', 'linear_few.cu', 'linear_narrow.cu', 'quant_rows.cu']
 HEADERS = [os.path.join(CSRC, h) for h in (
     'kdw_common.cuh', 'mma_patch.cuh', 'fprop_core.cuh', 'wgrad_core.cuh', 'fprop_variants.inc', 'wgrad_variants.inc',
     'linear_core.cuh', 'linear_plan.h', 'quant_core.cuh')] + [os.path.join(INCLUDE, 'kdw.h')]

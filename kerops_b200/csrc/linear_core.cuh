@@ -33,6 +33,7 @@ struct LinParams {
     int chunk;              // weight gradient: rows of one share (a multiple of 64)
     void* out;
     float* partial;         // [unit][tile_m / 128][BN / 4][128] float4 sums of the shares, or null: every tile has one share
+    int fold;               // weight gradient: > 1, all tiles go to `partial`
     int* table;             // copy of the table for the kernel that adds the shares, or null
     const float* row_scale; // 8-bit operands: [T] and [E][out_cols]
     const float* col_scale;

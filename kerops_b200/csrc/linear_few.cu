@@ -5,18 +5,17 @@
 // contraction inside a fragment is free as long as both operands agree, so the four words of such a piece are, as they
 // come, the operands of two products.  The weights go from memory to registers to the tensor pipe, without shared memory;
 // the tensor pipe is idle almost always.  A CTA takes 16 output channels of one group and splits the contraction over its
-// eight warps in pieces of 64 bytes, so that the CTA reads runs of 512 bytes; the warps' sums are added in shared memory.
+// four or eight warps in pieces of 64 bytes, so that the CTA reads runs of 256 or 512 bytes; the warps' sums are added in shared memory.
 //
 // 8-bit products of 16-bit rows: with at most eight rows every CTA quantises the rows it needs itself (they come from L2),
 // which is cheaper than a kernel in front.
+#include <stdlib.h>
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
 #include "quant_core.cuh"
 
 namespace kdw {
-
-constexpr int kFewWarps = 8;
 
 struct FewParams {
     const char *x, *w;        // rows and weights
@@ -95,10 +94,11 @@ __device__ __forceinline__ void few_group(const FewParams& p, int slot, int lane
     int before = 0, seen = 0;
     *g = -1;
     *begin = *end = 0;
+    int next = lane < p.E ? __ldg(p.ends + lane) : 0;
     for (int base = 0; base < p.E; base += 32) {
         const int e = base + lane;
-        int stop = p.T;
-        if (p.ends) stop = e < p.E ? __ldg(p.ends + e) : 0;
+        int stop = next;
+        next = e + 32 < p.E ? __ldg(p.ends + e + 32) : 0;
         stop = stop < 0 ? 0 : (stop > p.T ? p.T : stop);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -123,14 +123,13 @@ __device__ __forceinline__ void few_group(const FewParams& p, int slot, int lane
 }
 
 // NT: tiles of eight rows that share one pass over the weights.  QUANT: x holds 16-bit rows (NT == 1).
-template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
-__global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid_constant__ FewParams p) {
+template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U>
+__global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_constant__ FewParams p) {
     extern __shared__ __align__(16) char s_q[];
-    __shared__ uint32_t s_sum[kFewWarps][NT * 8][17];
+    __shared__ uint32_t s_sum[WARPS][NT * 8][17];
     __shared__ int s_group[4];
     __shared__ uint32_t s_max[8];
     __shared__ float s_scale[8];
-    constexpr int U = NT <= 2 ? 4 : 2;  // pieces in flight per lane and weight row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const int n0 = blockIdx.x * 16;
     grid_dependency_wait();
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
     }
     uint16_t* const y = reinterpret_cast<uint16_t*>(p.y);
     if (blockIdx.y == 0)
-        for (int i = threadIdx.x; i < (p.T - last) * 16; i += 32 * kFewWarps)
+        for (int i = threadIdx.x; i < (p.T - last) * 16; i += 32 * WARPS)
             if (n0 + (i & 15) < p.N) y[(long long)(last + (i >> 4)) * p.N + n0 + (i & 15)] = 0;
     if (end <= begin) return;
 
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) wv[u][h] = load_piece<VEC, true>(wr[h], (c + u * kFewWarps) * 64 + tig * 16, wlen[h]);
+                for (int h = 0; h < 2; ++h) wv[u][h] = load_piece<VEC, true>(wr[h], (c + u * WARPS) * 64 + tig * 16, wlen[h]);
         };
         load_weights(warp);
         if constexpr (QUANT) {
@@ -185,7 +184,7 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
             for (int r = 0; r < rows; ++r) {
                 const char* row = p.x + (t0 + r) * p.x_pitch;
                 uint32_t m = 0;
-                for (int i = threadIdx.x; i < vecs; i += 32 * kFewWarps)
+                for (int i = threadIdx.x; i < vecs; i += 32 * WARPS)
                     m = max_bits(load_piece<VEC, false>(row, i * 16, 2 * p.len), m);
                 m = __reduce_max_sync(0xffffffffu, m);
                 if (lane == 0 && m) atomicMax(&s_max[r], m);
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
                 const char* row = p.x + (t0 + r) * p.x_pitch;
                 const QuantRow q = quant_row(s_max[r], p.x_bf16);
                 if (threadIdx.x == 0) s_scale[r] = q.scale;
-                for (int i = threadIdx.x; i < p.q_pitch / 8; i += 32 * kFewWarps) {
+                for (int i = threadIdx.x; i < p.q_pitch / 8; i += 32 * WARPS) {
                     uint2 o = make_uint2(0, 0);
                     if (i < vecs) o = quant8(load_piece<VEC, false>(row, i * 16, 2 * p.len), q, p.x_bf16);
                     *reinterpret_cast<uint2*>(s_q + r * p.q_pitch + i * 8) = o;
@@ -216,14 +215,14 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
             xlen[j] = t < end ? p.len : 0;
             xr[j] = QUANT ? s_q + gid * p.q_pitch : p.x + (t < end ? t : t0) * p.x_pitch;
         }
-        for (int c = warp; c < pieces; c += U * kFewWarps) {
+        for (int c = warp; c < pieces; c += U * WARPS) {
             if (c != warp) load_weights(c);
             uint4 xv[U][NT];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const int at = (c + u * kFewWarps) * 64 + tig * 16;
+                    const int at = (c + u * WARPS) * 64 + tig * 16;
                     if constexpr (QUANT)
                         xv[u][j] = at < xlen[j] ? *reinterpret_cast<const uint4*>(xr[j] + at) : make_uint4(0, 0, 0, 0);
                     else
@@ -243,18 +242,18 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 4; ++i) s_sum[warp][j * 8 + tig * 2 + (i & 1)][gid + 8 * (i >> 1)] = acc[j][i];
         __syncthreads();
-        for (int i = threadIdx.x; i < NT * 8 * 16; i += 32 * kFewWarps) {
+        for (int i = threadIdx.x; i < NT * 8 * 16; i += 32 * WARPS) {
             const int r = i >> 4, c = i & 15, t = t0 + r, n = n0 + c;
             if (t >= end || n >= p.N) continue;
             float v = 0.f;
             if constexpr (I8) {
                 int s = 0;
 #pragma unroll
-                for (int k = 0; k < kFewWarps; ++k) s += (int)s_sum[k][r][c];
+                for (int k = 0; k < WARPS; ++k) s += (int)s_sum[k][r][c];
                 v = (float)s * (QUANT ? s_scale[r] : __ldg(p.x_scale + t)) * __ldg(p.w_scale + (long long)g * p.N + n);
             } else {
 #pragma unroll
-                for (int k = 0; k < kFewWarps; ++k) v += __uint_as_float(s_sum[k][r][c]);
+                for (int k = 0; k < WARPS; ++k) v += __uint_as_float(s_sum[k][r][c]);
             }
             y[(long long)t * p.N + n] = (uint16_t)pack2(v, 0.f, p.y_bf16);
         }
@@ -262,19 +261,30 @@ __global__ __launch_bounds__(32 * kFewWarps) void linear_few_kernel(const __grid
     }
 }
 
-template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
-static int few_launch(const FewParams& p, cudaStream_t st) {
-    static KernelSetup setup;
-    const int smem = QUANT ? p.q_pitch * 8 : 0;
+template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U>
+static int few_warps(const FewParams& p, dim3 grid, cudaStream_t st) {
     if (QUANT) {
+        static KernelSetup setup;
         int sms = 0, occ = 0;
-        int rc = setup.get((const void*)linear_few_kernel<I8, BF16, QUANT, NT, VEC>, 32 * kFewWarps, 8 * kFewQuantPitch, &sms, &occ);
+        int rc = setup.get((const void*)linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U>, 32 * WARPS, 8 * kFewQuantPitch, &sms, &occ);
         if (rc) return rc;
     }
-    const int slots = p.ends ? (p.E < p.T ? p.E : p.T) : 1;
-    KDW_CUDA(launch_overlapping_previous_grid(linear_few_kernel<I8, BF16, QUANT, NT, VEC>, dim3((unsigned)((p.N + 15) / 16), (unsigned)slots),
-                                              dim3(32 * kFewWarps), (size_t)smem, st, 1, p));
+    KDW_CUDA(launch_overlapping_previous_grid(linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U>, grid, dim3(32 * WARPS),
+                                              (size_t)(QUANT ? p.q_pitch * 8 : 0), st, 1, p));
     return 0;
+}
+template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
+static int few_launch(const FewParams& p, cudaStream_t st) {
+    const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)(p.ends ? (p.E < p.T ? p.E : p.T) : 1));
+    constexpr int U0 = NT == 1 ? 8 : NT == 2 ? 4 : 2;
+    const char* f = getenv("KDW_FEW");
+    switch (f ? atoi(f) : 0) {
+        case 1: return few_warps<I8, BF16, QUANT, NT, VEC, 4, U0>(p, grid, st);
+        case 2: return few_warps<I8, BF16, QUANT, NT, VEC, 8, U0>(p, grid, st);
+        case 3: return few_warps<I8, BF16, QUANT, NT, VEC, 4, U0 / 2>(p, grid, st);
+        case 4: return few_warps<I8, BF16, QUANT, NT, VEC, 16, U0 / 2>(p, grid, st);
+        default: return few_warps<I8, BF16, QUANT, NT, VEC, 8, U0 / 2>(p, grid, st);
+    }
 }
 template <bool I8, bool BF16, bool VEC>
 static int few_rows(const FewParams& p, cudaStream_t st) {

@@ -13,8 +13,28 @@ namespace kdw {
 static inline int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
+// Rows of few channels are short, and the TMA unit moves rows at a fixed rate.  In the weight gradient of one group of dense
+// rows, f neighbouring rows can be read as one of f times the channels: the product of the folded operands holds f x f
+// blocks, of which those on the diagonal are summed and the others, which mix rows, are left.  (In a row product the
+// others would multiply zeros with other rows' values, which may be infinite.)
+static int fold_of(const LinArgs& a) {
+    if (a.op != LIN_WGRAD || a.ends || a.E != 1 || a.a_stride != a.N || a.b_stride != a.K || a.K % 8 || a.N % 8) return 1;
+    if (((uintptr_t)a.a & 15) || ((uintptr_t)a.b & 15) || a.T < 8192) return 1;
+    const int64_t narrow = std::min(a.K, a.N);
+    int f = 1;
+    while (f < 8 && narrow * f * 2 <= 64 && a.T % (f * 2) == 0) f *= 2;
+    return f;
+}
+
+int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
+    LinArgs a = given;
     const bool wgrad = a.op == LIN_WGRAD;
+    pl->fold = fold_of(a);
+    a.T /= pl->fold;
+    a.K *= wgrad ? pl->fold : 1;
+    a.N *= wgrad ? pl->fold : 1;
+    a.a_stride *= pl->fold;
+    a.b_stride *= pl->fold;
     pl->esize = a.esize;
     const int64_t con = a.op == LIN_FWD ? a.K : a.op == LIN_DGRAD ? a.N : a.T;  // length of the contraction
     pl->out_cols = (int)(a.op == LIN_FWD ? a.N : a.K);
@@ -75,7 +95,7 @@ int linear_plan(LinPlan* pl, const LinArgs& a, int sms) {
             chunk = std::max<int64_t>(256, round_up(ceil_div(a.T, per_tile), 64));
         }
         pl->chunk = (int)std::min<int64_t>(chunk, 1 << 30);
-        split = pl->chunk < a.T;
+        split = pl->chunk < a.T || pl->fold > 1;  // the folded product's blocks are summed from the shares
         if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
     } else if (tiles * 2 <= slots && pl->k_blocks >= 8) {
         pl->splits = (int)std::min<int64_t>(slots / tiles, pl->k_blocks / 4);
@@ -229,7 +249,7 @@ int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int
     int sms = 0;
     int rc = f16_args(&args, op, a, b, T, E, K, N, a_stride, b_stride, dtype);
     if (!rc) rc = device_sm_count(&sms);
-    if (!rc && is_few(args)) return 0;
+    if (!rc && (is_few(args) || is_narrow(args))) return 0;
     if (!rc) rc = linear_plan(&pl, args, sms);
     return rc ? (rc < 0 ? rc : -rc) : pl.bytes;
 }
@@ -252,6 +272,8 @@ int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_
     args.out = out;
     args.ends = ends;
     if (is_few(args)) return linear_few(args, dtype, (cudaStream_t)stream);
+    // 16-byte stores: an output that does not allow them takes the other path, whose workspace must then be given
+    if (is_narrow(args) && ((uintptr_t)out & 15) == 0) return linear_narrow(args, (cudaStream_t)stream);
     return plan_and_run(&args, workspace, workspace_bytes, stream);
 }
 

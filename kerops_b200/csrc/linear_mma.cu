@@ -79,6 +79,12 @@ __device__ __forceinline__ void clear_rows(const LinParams& p, int first_row, in
     for (long long i = tail + 2 * id; i < end; i += 2 * n) *reinterpret_cast<uint16_t*>(out + i) = 0;
 }
 
+// Panels of 64 columns of a tile `width` wide that hold any of the `left` columns from its first on.
+__device__ __forceinline__ int boxes_inside(int left, int width) {
+    const int n = (left + 63) >> 6;
+    return n < 0 ? 0 : n > width / 64 ? width / 64 : n;
+}
+
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                const __grid_constant__ CUtensorMap map_b,
@@ -141,29 +147,29 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         break;
                     }
                     const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES;
+                    // Boxes wholly beyond the output are not loaded: what is left in their place reaches only rows and
+                    // columns of the accumulator that are not stored.
+                    const int a_boxes = C::WGRAD ? boxes_inside(p.out_rows - m0, kLinTileM) : 1;
+                    const int b_boxes = C::B_ROWS ? boxes_inside(p.out_cols - n0, C::LOAD_N) : 1;
+                    const uint32_t bytes = (C::WGRAD ? a_boxes * 8192 : C::A_BYTES) + (C::B_ROWS ? b_boxes * 8192 : C::B_BYTES);
                     uint32_t bar = full + 8 * stage;
                     if (rank == 0) {
-                        mbar_expect_tx(bar, C::STAGE);
+                        mbar_expect_tx(bar, bytes);
                     } else if (C::WGRAD && w.k_rows - k * 64 < 64) {
                         bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
-                        mbar_expect_tx(bar, C::STAGE);
+                        mbar_expect_tx(bar, bytes);
                     } else {
                         bar = cluster_addr(bar, 0);  // CTA 0 waits for the loads of both
-                        cluster_expect_tx(bar, C::STAGE);
+                        cluster_expect_tx(bar, bytes);
                     }
                     if constexpr (C::WGRAD) {
                         const int r = w.k_row + k * 64;
-#pragma unroll
-                        for (int j = 0; j < kLinTileM / 64; ++j)
-                            tma_load_2d<C::PAIR>(p.status, a + j * 8192, &map_a, bar, m0 + j * 64, r);
-#pragma unroll
-                        for (int j = 0; j < C::LOAD_N / 64; ++j)
-                            tma_load_2d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, r);
+                        for (int j = 0; j < a_boxes; ++j) tma_load_2d<C::PAIR>(p.status, a + j * 8192, &map_a, bar, m0 + j * 64, r);
+                        for (int j = 0; j < b_boxes; ++j) tma_load_2d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, r);
                     } else {
                         tma_load_2d<C::PAIR>(p.status, a, &map_a, bar, k * C::K_ELEMS, m0);
                         if constexpr (C::B_ROWS) {
-#pragma unroll
-                            for (int j = 0; j < C::LOAD_N / 64; ++j)
+                            for (int j = 0; j < b_boxes; ++j)
                                 tma_load_3d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, k * 64, w.g);
                         } else {
                             tma_load_3d<C::PAIR>(p.status, b, &map_b, bar, k * C::K_ELEMS, n0, w.g);
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             const int row0 = w.m0 + (int)rank * kLinTileM + q * 32;
             int rows = w.row_end - row0;
             rows = rows > 32 ? 32 : rows;
-            if (w.whole || !p.partial) {
+            if (!p.partial || (w.whole && p.fold == 1)) {
                 char* out = reinterpret_cast<char*>(p.out);
                 const long long pitch = (long long)p.out_cols * 2;
                 if (C::WGRAD) out += (long long)w.g * p.out_rows * pitch;
@@ -377,18 +383,19 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
 }
 
-// Adds the shares of the tiles that have several, in their order, and rounds once.  A CTA takes 32 columns of one tile.
-template <bool I8>
+// Adds the shares of the tiles that have several, and rounds once.  A CTA takes four columns of 256 / L rows of a tile; L
+// threads to a row add every L-th share each, and their sums are added in order: the same bits every call.
+template <bool I8, int L>
 __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__ LinParams p, int BN) {
-    __shared__ float s[kLinTileM][33];
-    grid_dependency_wait();
-    const int halves = p.tile_m / kLinTileM, slices = BN / 32 * halves;
+    constexpr int R = 256 / L;  // rows at a time
+    __shared__ uint4 s[L][R];
+    const int r = threadIdx.x % R, l = threadIdx.x / R;
+    const int quads = BN / 4, blocks = p.tile_m / R * quads;  // of a tile
     const int* row = p.table;
     const int* unit = p.table + p.E + 1;
-    const int tid = threadIdx.x;
+    grid_dependency_wait();
     for (int i = blockIdx.x;; i += gridDim.x) {
-        // tile i / slices, counted over the groups
-        int t = i / slices, g = 0, shares = 0, tiles = 0;
+        int t = i / blocks, g = 0, shares = 0, tiles = 0;  // the tile, counted over the groups
         for (; g < p.E; ++g) {
             const int rows = row[g + 1] - row[g];
             tiles = lin_group_tiles(p, rows);
@@ -399,62 +406,91 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
         if (g == p.E) return;
         if (shares == 1) continue;
         const int u = unit[g] + t;
-        LinUnit w = lin_unit(p, row, unit, u, BN);
-        const int half_m = (i % slices) / (BN / 32);
-        w.m0 += half_m * kLinTileM;
-        const int c0 = (i % (BN / 32)) * 32;
-        int cols = p.out_cols - w.n0 - c0;
-        cols = cols > 32 ? 32 : cols;
-        if (cols <= 0) continue;
-        const int r = tid & 127, half = tid >> 7;  // the thread's row and which 16 of the 32 columns
-        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + ((long long)u * halves + half_m) * (BN / 4) * kLinTileM +
-                           (long long)(c0 / 4 + half * 4) * kLinTileM + r;
-        const long long step = (long long)tiles * halves * (BN / 4) * kLinTileM;
-        float f[16];
-        int n[16];
+        const LinUnit w = lin_unit(p, row, unit, u, BN);
+        const int part = i % blocks, quad = part % quads, m = part / quads * R + r;  // row of the tile
+        const int c0 = w.n0 + quad * 4;
+        if (c0 >= p.out_cols) continue;
+        const long long halves = p.tile_m / kLinTileM, step = tiles * halves * quads * kLinTileM;
+        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + ((u * halves + m / kLinTileM) * quads + quad) * kLinTileM + m % kLinTileM;
+        uint4 sum = make_uint4(0, 0, 0, 0);
+        auto add = [&](const uint4& v) {
+            if (I8) {
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            } else {
+                sum.x = __float_as_uint(__uint_as_float(sum.x) + __uint_as_float(v.x));
+                sum.y = __float_as_uint(__uint_as_float(sum.y) + __uint_as_float(v.y));
+                sum.z = __float_as_uint(__uint_as_float(sum.z) + __uint_as_float(v.z));
+                sum.w = __float_as_uint(__uint_as_float(sum.w) + __uint_as_float(v.w));
+            }
+        };
+#pragma unroll 8
+        for (int k = l; k < shares; k += L) add(__ldcg(src + k * step));
+        __syncthreads();
+        s[l][r] = sum;
+        __syncthreads();
+        if (l != 0 || w.m0 + m >= w.row_end) continue;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            f[j] = 0.f;
-            n[j] = 0;
+        for (int k = 1; k < L; ++k) add(s[k][r]);
+        const uint32_t v[4] = {sum.x, sum.y, sum.z, sum.w};
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) +
+                        ((p.m_tiles ? (long long)w.g * p.out_rows : 0) + w.m0 + m) * p.out_cols + c0;
+        const float rs = I8 ? __ldg(p.row_scale + w.m0 + m) : 1.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c0 + j < p.out_cols) {
+                float f;
+                if (I8)
+                    f = (float)(int)v[j] * rs * __ldg(p.col_scale + (long long)w.g * p.out_cols + c0 + j);
+                else
+                    f = __uint_as_float(v[j]);
+                out[j] = (uint16_t)pack2(f, 0.f, p.out_bf16);
+            }
+    }
+}
+
+// The weight gradient from a folded product (see linear_plan): the sum over the shares and over the f blocks on the
+// diagonal.  A CTA adds four neighbouring values of a row, its threads the (share, block) pairs, in a fixed order.
+__global__ __launch_bounds__(256) void linear_fold_kernel(const __grid_constant__ LinParams p, int BN, int N, int K) {
+    __shared__ float4 s[8];
+    const int lane = threadIdx.x & 31, quads = K / 4, tiles = p.m_tiles * p.n_tiles;
+    grid_dependency_wait();
+    const int shares = p.table[p.E + 1 + p.E] / tiles;
+    for (int i = blockIdx.x; i < N * quads; i += gridDim.x) {
+        const int n = i / quads, k = (i - n * quads) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int j = threadIdx.x; j < shares * p.fold; j += 256) {
+            const int share = j / p.fold, block = j - share * p.fold;
+            const int m = block * N + n, c = block * K + k;
+            const int mt = m / p.tile_m, nt = c / BN, band = mt / kLinBand;
+            const int high = p.m_tiles - band * kLinBand < kLinBand ? p.m_tiles - band * kLinBand : kLinBand;
+            const long long u = (long long)share * tiles + band * kLinBand * p.n_tiles + nt * high + mt - band * kLinBand;
+            const long long half = u * (p.tile_m / kLinTileM) + (m % p.tile_m) / kLinTileM;
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial) + (half * (BN / 4) + (c % BN) / 4) * kLinTileM + m % kLinTileM);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
         }
-        for (int k = 0; k < shares; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint4 v = __ldcg(src + k * step + (long long)j * kLinTileM);
-                if (I8) {
-                    n[4 * j] += (int)v.x;
-                    n[4 * j + 1] += (int)v.y;
-                    n[4 * j + 2] += (int)v.z;
-                    n[4 * j + 3] += (int)v.w;
-                } else {
-                    f[4 * j] += __uint_as_float(v.x);
-                    f[4 * j + 1] += __uint_as_float(v.y);
-                    f[4 * j + 2] += __uint_as_float(v.z);
-                    f[4 * j + 3] += __uint_as_float(v.w);
-                }
-            }
-        int rows = w.row_end - w.m0;
-        if (rows <= 0) continue;
-        rows = rows > kLinTileM ? kLinTileM : rows;
-        if (I8) {
-            const float rs = r < rows ? __ldg(p.row_scale + w.m0 + r) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int c = w.n0 + c0 + half * 16 + j;
-                f[j] = (float)n[j] * rs * (c < p.out_cols ? __ldg(p.col_scale + (long long)w.g * p.out_cols + c) : 0.f);
-            }
+        for (int d = 16; d > 0; d >>= 1) {
+            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+            sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
+            sum.z += __shfl_xor_sync(0xffffffffu, sum.z, d);
+            sum.w += __shfl_xor_sync(0xffffffffu, sum.w, d);
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[r][half * 16 + j] = f[j];
+        if (lane == 0) s[threadIdx.x >> 5] = sum;
         __syncthreads();
-        char* out = reinterpret_cast<char*>(p.out) + (p.m_tiles ? (long long)w.g * p.out_rows * p.out_cols * 2 : 0);
-        const int c = tid & 31;
-        if (c < cols)
-            for (int rr = tid >> 5; rr < rows; rr += 8) {
-                const uint32_t v = pack2(s[rr][c], 0.f, p.out_bf16);
-                *reinterpret_cast<uint16_t*>(out + ((long long)(w.m0 + rr) * p.out_cols + w.n0 + c0 + c) * 2) = (uint16_t)v;
-            }
+        if (threadIdx.x < 4) {
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v += reinterpret_cast<const float*>(&s[j])[threadIdx.x];
+            reinterpret_cast<uint16_t*>(p.out)[(long long)n * K + k + threadIdx.x] = (uint16_t)pack2(v, 0.f, p.out_bf16);
+        }
     }
 }
 
@@ -496,10 +532,15 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     const int grid = (pl.max_units < slots ? (pl.max_units > 0 ? (int)pl.max_units : 1) : slots) * (C::PAIR ? 2 : 1);
     KDW_CUDA(launch_overlapping_previous_grid(linear_kernel<C>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, st,
                                               C::PAIR ? 2 : 1, ma, mb, p));
-    if (p.partial) {
-        const long long blocks = pl.max_tiles * (C::BN / 32) * (p.tile_m / kLinTileM);
-        KDW_CUDA(launch_overlapping_previous(linear_sum_kernel<C::I8>, (unsigned)(blocks < 4 * sms ? blocks : 4 * sms), 256u,
-                                             st, p, C::BN));
+    if (p.fold > 1) {
+        const int N = pl.out_rows / p.fold, K = pl.out_cols / p.fold;
+        const int quads = N * (K / 4);
+        KDW_CUDA(launch_overlapping_previous(linear_fold_kernel, (unsigned)(quads < 8 * sms ? quads : 8 * sms), 256u, st, p, C::BN, N, K));
+    } else if (p.partial) {
+        const bool many = pl.max_units >= 8 * pl.max_tiles;
+        const long long blocks = pl.max_tiles * (C::BN / 4) * (p.tile_m / (many ? 32 : 128));
+        KDW_CUDA(launch_overlapping_previous(many ? linear_sum_kernel<C::I8, 8> : linear_sum_kernel<C::I8, 2>,
+                                             (unsigned)(blocks < 8 * sms ? blocks : 8 * sms), 256u, st, p, C::BN));
     }
     return 0;
 }
@@ -538,7 +579,7 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     char* w = (char*)ws;
     const void* pa = a.a;
     const void* pb = a.b;
-    int64_t sa = a.a_stride, sb = a.b_stride;
+    int64_t sa = a.a_stride * pl.fold, sb = a.b_stride * pl.fold;
     if (pl.pack_a) {
         pa = w + pl.off_a;
         rc = pl.esize == 2 ? pack_rows<uint16_t>(a.a, w + pl.off_a, pl.a_rows, pl.a_cols, a.a_stride, pl.a_pitch, st)
@@ -556,7 +597,8 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     LinParams p;
     memset(&p, 0, sizeof(p));
     p.ends = a.ends;
-    p.T = (int)a.T;
+    p.T = (int)(a.T / pl.fold);
+    p.fold = pl.fold;
     p.E = (int)a.E;
     p.tile_m = pl.tile_m;
     p.m_tiles = pl.m_tiles;

@@ -1,0 +1,216 @@
+// Products of many rows with one narrow weight matrix (the pointwise product behind a depthwise convolution on a volume:
+// 8 to 128 channels, millions of voxels): bound by reading and writing the rows once.
+//
+// Rows of 16 to 256 bytes are too short for the TMA unit, which moves 40-50 G box rows per second whatever their length;
+// here a warp loads them straight into the operand registers of mma.sync, 16 rows to a tile, in runs of contiguous memory.
+// The weights stay in registers as the other operand for the whole kernel.  The order of the contraction and of the output
+// columns inside a fragment is free: a lane's words of a 16-byte piece of a row are the operands of two products as they
+// come, and the columns are dealt to the fragments so that a lane's results are 16 contiguous bytes of an output row.
+#include "../../include/kdw.h"
+#include "linear_core.cuh"
+#include "linear_plan.h"
+
+namespace kdw {
+
+struct NarrowParams {
+    const char* x;
+    const uint16_t* w;
+    char* y;
+    const int* ends;          // one end, or null
+    long long x_pitch;        // bytes
+    long long T;
+    int K, N;                 // contraction and output columns, multiples of 8
+    int w_n, w_k;             // elements between the weights of neighbouring output columns / contraction steps
+};
+
+template <bool BF16>
+__device__ __forceinline__ void narrow_mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// WORDS 32-bit words of a lane's piece of a row.
+template <int WORDS>
+__device__ __forceinline__ void narrow_load(uint32_t (&v)[WORDS], const char* p, bool live) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) v[i] = 0;
+    if (!live) return;
+    if constexpr (WORDS == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "l"(p));
+    else if constexpr (WORDS == 2)
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+}
+
+// KP, NP: contraction and columns rounded up to 8, 16, 32, 64 or 128; KP * NP <= 4096, so that the weights fit the registers.
+template <bool BF16_, int KP_, int NP_>
+struct NCfg {
+    static constexpr bool BF16 = BF16_;
+    static constexpr int KP = KP_, NP = NP_;
+    static constexpr int WORDS = KP >= 32 ? 4 : KP / 8;         // words of a lane's piece: a row is PIECES x 4 lanes x WORDS
+    static constexpr int PIECES = KP >= 32 ? KP / 32 : 1;
+    static constexpr int STEPS = KP >= 16 ? KP / 16 : 1;        // products of a tile and eight columns
+    static constexpr int COLS = NP >= 32 ? 32 : NP;             // columns whose results a lane stores as one piece
+    static constexpr int GROUPS = NP / COLS, TILES = COLS / 8;  // of eight columns, per piece
+    static constexpr int AHEAD = PIECES >= 4 ? 1 : PIECES == 2 ? 2 : 4;  // row tiles whose loads are in flight
+    static constexpr int THREADS = 128;
+    static constexpr int CTAS = KP * NP >= 4096 ? 3 : 4;        // to an SM at least: what the registers have to allow
+};
+
+template <class C>
+__global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(const __grid_constant__ NarrowParams p) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    const long long warp = ((long long)blockIdx.x * C::THREADS + threadIdx.x) >> 5, warps = (long long)gridDim.x * (C::THREADS / 32);
+    grid_dependency_wait();
+    long long rows = p.T;
+    if (p.ends) {
+        const int e = __ldg(p.ends);
+        rows = e < 0 ? 0 : (e < p.T ? e : p.T);
+    }
+    // Weights.  Step s of piece q covers, for this lane, contraction indexes q * 32 + tig * 8 + (s & 1) * 4 + {0, 1} and
+    // + {2, 3} (KP >= 32); the slot `gid` of tile j of a column group is column (gid / 2) * 2 TILES + 2 j + (gid & 1).
+    uint32_t b[C::GROUPS][C::TILES][C::STEPS][2];
+#pragma unroll
+    for (int g = 0; g < C::GROUPS; ++g)
+#pragma unroll
+        for (int j = 0; j < C::TILES; ++j)
+#pragma unroll
+            for (int s = 0; s < C::STEPS; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int n = g * C::COLS + (gid >> 1) * 2 * C::TILES + 2 * j + (gid & 1);
+                    const int k = C::KP >= 32 ? (s >> 1) * 32 + tig * 8 + (s & 1) * 4 + h * 2 : tig * C::KP / 4 + h * 2;
+                    uint32_t v = 0;
+                    if (n < p.N && k < p.K && (C::KP > 8 || h == 0)) {
+                        const uint16_t* w = p.w + (long long)n * p.w_n + (long long)k * p.w_k;
+                        v = w[0] | (uint32_t)w[p.w_k] << 16;
+                    }
+                    b[g][j][s][h] = v;
+                }
+    const long long tiles = (p.T + 15) >> 4;
+    const int kbytes = p.K * 2;
+    auto load = [&](uint32_t (&a)[C::PIECES][2][C::WORDS], long long t) {
+#pragma unroll
+        for (int q = 0; q < C::PIECES; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long r = t * 16 + gid + 8 * h;
+                const int at = q * 64 + tig * C::WORDS * 4;
+                narrow_load<C::WORDS>(a[q][h], p.x + r * p.x_pitch + at, r < rows && at < kbytes);
+            }
+    };
+    uint32_t a[C::AHEAD][C::PIECES][2][C::WORDS];
+#pragma unroll
+    for (int i = 0; i < C::AHEAD; ++i) load(a[i], warp + i * warps);
+    for (long long t0 = warp; t0 < tiles; t0 += C::AHEAD * warps) {
+#pragma unroll
+        for (int i = 0; i < C::AHEAD; ++i) {
+            const long long t = t0 + i * warps;
+            if (t >= tiles) break;
+#pragma unroll
+            for (int g = 0; g < C::GROUPS; ++g) {
+                float c[C::TILES][4];
+#pragma unroll
+                for (int j = 0; j < C::TILES; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[j][e] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < C::STEPS; ++s) {
+                        constexpr int M = C::WORDS - 1;
+                        const int q = C::KP >= 32 ? s >> 1 : 0, o = C::KP >= 32 ? (s & 1) * 2 : 0;
+                        narrow_mma16<C::BF16>(c[j], a[i][q][0][o], a[i][q][1][o], C::KP > 8 ? a[i][q][0][(o + 1) & M] : 0u,
+                                              C::KP > 8 ? a[i][q][1][(o + 1) & M] : 0u, b[g][j][s][0], b[g][j][s][1]);
+                    }
+                }
+                if (g + 1 == C::GROUPS) load(a[i], t + C::AHEAD * warps);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const long long r = t * 16 + gid + 8 * h;
+                    const int col = g * C::COLS + tig * 2 * C::TILES;
+                    if (r >= p.T || col >= p.N) continue;
+                    uint32_t o[C::TILES];
+#pragma unroll
+                    for (int j = 0; j < C::TILES; ++j) o[j] = r < rows ? pack2(c[j][2 * h], c[j][2 * h + 1], C::BF16) : 0u;
+                    char* dst = p.y + (r * p.N + col) * 2;
+                    if constexpr (C::TILES == 4)
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+                    else if constexpr (C::TILES == 2)
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+                    else
+                        *reinterpret_cast<uint32_t*>(dst) = o[0];
+                }
+            }
+        }
+    }
+}
+
+template <class C>
+static int narrow_launch(const NarrowParams& p, cudaStream_t st) {
+    static KernelSetup setup;
+    int sms = 0, occ = 0;
+    int rc = setup.get((const void*)linear_narrow_kernel<C>, C::THREADS, 0, &sms, &occ);
+    if (rc) return rc;
+    const long long want = ((p.T + 15) / 16 + C::THREADS / 32 - 1) / (C::THREADS / 32);
+    const long long most = (long long)sms * occ;
+    KDW_CUDA(launch_overlapping_previous(linear_narrow_kernel<C>, (unsigned)(want < most ? want : most), (unsigned)C::THREADS, st, p));
+    return 0;
+}
+template <bool BF16, int KP>
+static int narrow_cols(const NarrowParams& p, cudaStream_t st) {
+    if (p.N <= 8) return narrow_launch<NCfg<BF16, KP, 8>>(p, st);
+    if (p.N <= 16) return narrow_launch<NCfg<BF16, KP, 16>>(p, st);
+    if (p.N <= 32) return narrow_launch<NCfg<BF16, KP, 32>>(p, st);
+    if constexpr (KP <= 64) {
+        if (p.N <= 64) return narrow_launch<NCfg<BF16, KP, 64>>(p, st);
+    }
+    if constexpr (KP <= 32) {
+        if (p.N <= 128) return narrow_launch<NCfg<BF16, KP, 128>>(p, st);
+    }
+    set_error("linear: %d x %d weights are not narrow", p.K, p.N);
+    return KDW_ERR_ARG;
+}
+template <bool BF16>
+static int narrow_rows(const NarrowParams& p, cudaStream_t st) {
+    if (p.K <= 8) return narrow_cols<BF16, 8>(p, st);
+    if (p.K <= 16) return narrow_cols<BF16, 16>(p, st);
+    if (p.K <= 32) return narrow_cols<BF16, 32>(p, st);
+    if (p.K <= 64) return narrow_cols<BF16, 64>(p, st);
+    return narrow_cols<BF16, 128>(p, st);
+}
+
+static int64_t narrow_pad(int64_t v) { return v <= 8 ? 8 : v <= 16 ? 16 : v <= 32 ? 32 : v <= 64 ? 64 : 128; }
+
+bool is_narrow(const LinArgs& a) {
+    if (a.op == LIN_WGRAD || a.esize != 2 || a.E != 1 || a.K > 128 || a.N > 128) return false;
+    if (narrow_pad(a.K) * narrow_pad(a.N) > 4096) return false;
+    // (the weights are read by elements; a base that TMA cannot address would need a workspace on the other path)
+    return a.K % 8 == 0 && a.N % 8 == 0 && ((uintptr_t)a.a & 15) == 0 && ((uintptr_t)a.b & 15) == 0 && a.a_stride % 8 == 0;
+}
+
+int linear_narrow(const LinArgs& a, cudaStream_t st) {
+    NarrowParams p;
+    const bool fwd = a.op == LIN_FWD;
+    p.x = (const char*)a.a;
+    p.w = (const uint16_t*)a.b;
+    p.y = (char*)a.out;
+    p.ends = a.ends;
+    p.x_pitch = a.a_stride * 2;
+    p.T = a.T;
+    p.K = (int)(fwd ? a.K : a.N);
+    p.N = (int)(fwd ? a.N : a.K);
+    p.w_n = fwd ? (int)a.K : 1;
+    p.w_k = fwd ? 1 : (int)a.K;
+    return a.in_bf16 ? narrow_rows<true>(p, st) : narrow_rows<false>(p, st);
+}
+
+}  // namespace kdw

@@ -23,6 +23,7 @@ struct LinArgs {
 struct LinPlan {
     int esize, bn, tile_m;  // tile_m 256: a pair of CTAs to a tile
     int m_tiles, n_tiles, out_rows, out_cols, k_blocks, splits, chunk;
+    int fold;                // weight gradient: rows that are taken as one (see linear_plan)
     bool pack_a, pack_b;
     int64_t a_rows, a_cols, a_pitch, b_rows, b_cols, b_pitch;  // pitches of the packed copies, in elements
     int64_t off_a, off_b, off_table, off_partial;              // off_partial < 0: no tile has several shares
@@ -37,6 +38,10 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st);
 constexpr int kFewRows = 32;
 constexpr int kFewQuantRows = 8, kFewQuantPitch = 128 * 96 + 64;  // rows and bytes of a row that a CTA quantises itself
 int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
+
+// Products of many rows with one narrow weight matrix, without a workspace (linear_narrow.cu).
+bool is_narrow(const LinArgs& a);
+int linear_narrow(const LinArgs& a, cudaStream_t st);
 
 // Quantises rows of 16-bit values (see quant_rows.cu); q_padded: what lies between `cols` and q_stride may be written.
 int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride, int bf16,

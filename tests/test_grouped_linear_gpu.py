@@ -75,6 +75,36 @@ def test_larger(T, K, N, ends):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('K', [8, 16, 24, 32, 64, 104, 128])
+def test_narrow_weights_and_many_rows(K, dtype):
+    """Few channels: row products that stream the rows, and weight gradients that fold rows together."""
+    for i, N in enumerate((8, 16, 40, 64, 128)):
+        _check((8192, 9000, 8200, 8194, 8193)[(i + K // 8) % 5], K, N, None, dtype)
+        _check(777, K, N, [771], dtype)
+
+
+def test_folded_rows_do_not_mix():
+    """A NaN in one voxel stays with its own products: the blocks that pair neighbouring voxels are not summed."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    T, K, N = 16384, 8, 16
+    x, g = ref.integers((T, K), torch.float16, 1), ref.integers((T, N), torch.float16, 2)
+    w = ref.integers((N, K), torch.float16, 3)
+    y, dx = ref.fwd(x, w[None], [T]).half(), ref.dgrad(g, w[None], [T]).half()
+    x[1001, 3] = float('nan')
+    g[1000] = float('inf')  # the neighbouring voxel
+    got = GroupedLinearWGRAD(x, g)
+    assert torch.isnan(got[:, 3]).all()
+    keep = [0, 1, 2, 4, 5, 6, 7]
+    want = ref.wgrad(x[:, keep], g, [T])[0]
+    assert torch.equal(got[:, keep].nan_to_num(7.0), want.half().nan_to_num(7.0))
+    gy, gdx = GroupedLinear(x, w), GroupedLinearDGRAD(g, w)
+    rows = torch.arange(T, device='cuda')
+    assert torch.equal(gy[rows != 1001], y[rows != 1001]) and torch.isnan(gy[1001]).all()
+    assert torch.equal(gdx[rows != 1000], dx[rows != 1000])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 def test_normal_values_within_the_rounding(dtype):
     from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
 
