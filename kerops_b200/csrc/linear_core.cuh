@@ -4,9 +4,13 @@
 //   row products     out[t, :] = a[t, :] * B_g          for the rows t of group g   (forward, input gradient, int8)
 //   weight gradient  out[g]    = sum_t a[t, :]^T b[t, :] over the rows t of group g
 //
-// A UNIT is one output tile of 128 x BN (a CTA) or 256 x BN (a pair of CTAs) and one share of its contraction.  Row groups end where the device array
-// `ends` says; every CTA scans it once into a table in shared memory (first row and first unit of each group), and a
-// unit index is found in it by bisection, so the host never waits for the row counts.
+// Row products are computed as their transpose: the output channels take the M side of the tensor cores, in tiles of 128
+// (a CTA) or 256 (a pair of CTAs), the rows the N side, whose width may change from tile to tile in steps of 32.  A group
+// of any size then wastes at most 31 rows of products; with rows on the M side it would be 127 or 255.
+//
+// A UNIT is one output tile and one share of its contraction.  Row groups end where the device array `ends` says; every CTA
+// scans it once into a table in shared memory (first row and first unit of each group), and a unit index is found in it by
+// bisection, so the host never waits for the row counts.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -16,7 +20,7 @@
 namespace kdw {
 
 constexpr int kLinMaxGroups = 1024;   // groups of one call: the table of a CTA holds them all
-constexpr int kLinTileM = 128;        // output rows of a CTA's tile = lanes of the accumulator
+constexpr int kLinTileM = 128;        // M of a CTA's tile = lanes of the accumulator
 constexpr int kLinSpan = 128;         // bytes of a shared-memory row = the swizzle span
 
 enum LinOp : int { LIN_FWD = 0, LIN_DGRAD = 1, LIN_WGRAD = 2 };
@@ -24,22 +28,23 @@ enum LinOp : int { LIN_FWD = 0, LIN_DGRAD = 1, LIN_WGRAD = 2 };
 struct LinParams {
     const int* ends;        // [E] cumulative row ends, or null: one group of all rows
     int T, E;               // rows, groups
-    int tile_m;             // output rows of a tile: 128, or 256 for a pair of CTAs
-    int m_tiles;            // weight gradient: tiles along the output rows; row products: 0 (follows from the group)
-    int n_tiles;            // tiles along the output columns
+    int wgrad;
+    int tile_m, bn, bn_log; // tile: M (128, or 256 for a pair of CTAs) x N (row products: at most that many rows)
+    int m_tiles;            // tiles along M: output channels of row products, output rows of the weight gradient
+    int n_tiles;            // weight gradient: tiles along the output columns; row products: 0 (follows from the group)
     int out_rows, out_cols; // weight gradient: rows of one output matrix; columns of the output
     int k_blocks;           // row products: blocks of the contraction
     int splits;             // row products: shares of the contraction
     int chunk;              // weight gradient: rows of one share (a multiple of 64)
     void* out;
-    float* partial;         // [unit][tile_m / 128][BN / 4][128] float4 sums of the shares, or null: every tile has one share
+    float* partial;         // [unit][tile_m / 128][bn / 4][128] float4 sums of the shares, or null: every tile has one share
     int fold;               // weight gradient: > 1, all tiles go to `partial`
     int* table;             // copy of the table for the kernel that adds the shares, or null
     const float* row_scale; // 8-bit operands: [T] and [E][out_cols]
     const float* col_scale;
     int out_bf16;
     int out_vec;            // 1: rows of the output start on 16-byte boundaries
-    uint32_t idesc;
+    uint32_t idesc;         // without N
     int* status;
     unsigned long long limit_ns;
     int stop_after;
@@ -52,29 +57,46 @@ struct LinTable {
 };
 
 struct LinUnit {
-    int g, m0, n0;     // group; first output row (row products: an absolute row of the output) and column
-    int row_end;       // row products: end of the group; weight gradient: rows of the output matrix
+    int g;             // group
+    int c0;            // M side: first output channel (row products), first output row (weight gradient)
+    int t0, width;     // N side: first row of `out` and how many columns of the accumulator the tile has, a multiple of 32
+    int rows;          // row products: rows of the tile
     int kb, ke;        // blocks of the contraction; weight gradient: blocks of 64 rows counted from k_row
-    int k_row;         // weight gradient: first row of the share
-    int k_rows;        // weight gradient: rows of the share (the last block may be partly beyond them)
+    int k_row, k_rows; // weight gradient: first row and rows of the share (the last block may be partly beyond them)
     bool whole;        // this unit is the only share of its tile
 };
 
 __host__ __device__ __forceinline__ int lin_ceil(int a, int b) { return (a + b - 1) / b; }
 
+// n / d for 0 <= n < 2^31, 0 < d: a quotient from the reciprocal in fp32, off by n 2^-22 / d at most, corrected twice.  A
+// tenth of the latency of the integer division, of which finding a unit needs several.
+__host__ __device__ __forceinline__ int lin_div(int n, int d) {
+#ifdef __CUDA_ARCH__
+    const float r = __frcp_rn((float)d);
+    int q = __float2int_rz((float)n * r);
+    int rest = n - q * d;  // may wrap where q is off by much: only its low bits count, the true rest fits
+    const int fix = __float2int_rd((float)rest * r);
+    q += fix;
+    rest -= fix * d;
+    return q + (rest >= d) - (rest < 0);
+#else
+    return n / d;
+#endif
+}
+
 __host__ __device__ __forceinline__ int lin_shares(const LinParams& p, int rows) {
-    if (p.m_tiles == 0) return p.splits;
-    return rows > p.chunk ? lin_ceil(rows, p.chunk) : 1;
+    if (!p.wgrad) return p.splits;
+    return rows > p.chunk ? lin_div(rows - 1, p.chunk) + 1 : 1;
 }
 __host__ __device__ __forceinline__ int lin_group_tiles(const LinParams& p, int rows) {
-    return (p.m_tiles ? p.m_tiles : lin_ceil(rows, p.tile_m)) * p.n_tiles;
+    return p.m_tiles * (p.wgrad ? p.n_tiles : (rows + p.bn - 1) >> p.bn_log);
 }
 
-// Tiles of a group in bands of 16 tile rows, a band's rows fastest: the CTAs that run at the same time then share
-// both operands' tiles in L2 (148 CTAs = 16 tile rows x 9 tile columns).
+// Tiles of a group in bands of 16 along N, a band's N fastest: the CTAs that run at the same time then share both
+// operands' tiles in L2 (148 CTAs = 16 x 9 tiles).
 constexpr int kLinBand = 16;
 
-__host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const int* row, const int* unit, int u, int BN) {
+__host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const int* row, const int* unit, int u) {
     int lo = 0, hi = p.E;  // unit[lo] <= u < unit[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -86,38 +108,47 @@ __host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const i
     LinUnit r;
     r.g = lo;
     const int rows = row[lo + 1] - row[lo];
-    const int mt = p.m_tiles ? p.m_tiles : lin_ceil(rows, p.tile_m);
+    const int nt = p.wgrad ? p.n_tiles : (rows + p.bn - 1) >> p.bn_log;
     const int shares = lin_shares(p, rows);
-    int share = 0, nt = 0, m = u - unit[lo];
+    int share = 0, n = u - unit[lo], m = 0;
     if (shares > 1) {
-        const int tiles = mt * p.n_tiles;
-        share = m / tiles;
-        m -= share * tiles;
+        const int tiles = p.m_tiles * nt;
+        share = lin_div(n, tiles);
+        n -= share * tiles;
     }
-    if (p.n_tiles > 1) {
-        const int band = m / (kLinBand * p.n_tiles);
-        const int inside = m - band * kLinBand * p.n_tiles;
-        const int high = mt - band * kLinBand < kLinBand ? mt - band * kLinBand : kLinBand;
-        nt = inside / high;
-        m = band * kLinBand + inside - nt * high;
+    if (p.m_tiles > 1) {
+        const int band = nt > kLinBand ? lin_div(n, kLinBand * p.m_tiles) : 0;
+        const int inside = n - band * kLinBand * p.m_tiles;
+        const int wide = nt - band * kLinBand < kLinBand ? nt - band * kLinBand : kLinBand;
+        m = lin_div(inside, wide);
+        n = band * kLinBand + inside - m * wide;
     }
-    r.n0 = nt * BN;
+    r.c0 = m * p.tile_m;
     r.k_row = 0;
     r.k_rows = 0;
     r.whole = shares == 1;
-    if (p.m_tiles == 0) {
-        r.m0 = row[lo] + m * p.tile_m;
-        r.row_end = row[lo + 1];
-        r.kb = (int)((long long)p.k_blocks * share / shares);
-        r.ke = (int)((long long)p.k_blocks * (share + 1) / shares);
+    if (!p.wgrad) {
+        // the group's rows in tiles of about equal width, so that tiles cost about the same
+        const int width = nt > 1 ? (lin_div(rows - 1, nt) + 32) & ~31 : p.bn;
+        const int left = rows - n * width;
+        r.t0 = row[lo] + n * width;
+        r.rows = left < width ? (left > 0 ? left : 0) : width;
+        r.width = (r.rows + 31) & ~31;
+        r.kb = 0;
+        r.ke = r.rows ? p.k_blocks : 0;
+        if (shares > 1 && r.rows) {  // at most 64 shares
+            r.kb = lin_div(p.k_blocks * share, shares);
+            r.ke = lin_div(p.k_blocks * (share + 1), shares);
+        }
     } else {
-        r.m0 = m * p.tile_m;
-        r.row_end = p.out_rows;
+        r.t0 = n * p.bn;
+        r.width = p.bn;
+        r.rows = 0;
         r.k_row = row[lo] + share * p.chunk;
         const int left = row[lo + 1] - r.k_row;
         r.k_rows = left < p.chunk ? left : p.chunk;
         r.kb = 0;
-        r.ke = lin_ceil(r.k_rows, 64);
+        r.ke = (r.k_rows + 63) >> 6;
     }
     return r;
 }
@@ -162,14 +193,11 @@ __device__ __forceinline__ void lin_build_table(const LinParams& p, int* row, in
     }
 }
 
-// Loads of a box; PAIR: the barrier may be the other CTA's (a shared::cluster address), as the two CTAs of a pair
+// Loads of a box.  Stages start on 1024-byte boundaries and innermost coordinates are multiples of a box row (128 bytes)
+// by construction.  PAIR: the barrier may be the other CTA's (a shared::cluster address), as the two CTAs of a pair
 // report to one of them.
 template <bool PAIR>
-__device__ __forceinline__ void tma_load_2d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
-    if ((dst & 1023u) != 0) {
-        atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
-        return;
-    }
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1) {
     if constexpr (PAIR)
         asm volatile(
             "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -182,12 +210,7 @@ __device__ __forceinline__ void tma_load_2d(int* status, uint32_t dst, const CUt
             : "memory");
 }
 template <bool PAIR>
-__device__ __forceinline__ void tma_load_3d(int* status, uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1,
-                                            int c2) {
-    if ((dst & 1023u) != 0) {
-        atomicExch(status, (int)KDW_STATUS_TMA_ARGS);
-        return;
-    }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1, int c2) {
     if constexpr (PAIR)
         asm volatile(
             "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
@@ -313,7 +336,8 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 }
 #undef KDW_TC_MMA
 
-// 32 accumulator columns of the calling warp's 32 lanes.
+// 32 accumulator columns of the calling warp's 32 lanes: a lane's columns in its registers.  The values are there after
+// tmem_wait.
 __device__ __forceinline__ void tmem_load_32(uint32_t addr, uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -325,7 +349,32 @@ __device__ __forceinline__ void tmem_load_32(uint32_t addr, uint32_t (&v)[32]) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr)
         : "memory");
+}
+// The same values in the fragment layout of an 8 x 8 matrix store: register 16 h + 4 j + 2 i + e of lane l is accumulator
+// lane 16 h + 8 i + l / 4, column 8 j + 2 (l % 4) + e.
+__device__ __forceinline__ void tmem_load_frag(uint32_t addr, uint32_t (&v)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(v[16 * h]), "=r"(v[16 * h + 1]), "=r"(v[16 * h + 2]), "=r"(v[16 * h + 3]), "=r"(v[16 * h + 4]),
+              "=r"(v[16 * h + 5]), "=r"(v[16 * h + 6]), "=r"(v[16 * h + 7]), "=r"(v[16 * h + 8]), "=r"(v[16 * h + 9]),
+              "=r"(v[16 * h + 10]), "=r"(v[16 * h + 11]), "=r"(v[16 * h + 12]), "=r"(v[16 * h + 13]), "=r"(v[16 * h + 14]),
+              "=r"(v[16 * h + 15])
+            : "r"(addr + ((uint32_t)(16 * h) << 16))
+            : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void tmem_wait(T& v) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i]));  // no use of the values moves above the wait
+}
+// Stores four 8 x 8 matrices of 16-bit values transposed; lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void store_matrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
 }
 
 // Shared-memory matrix descriptors, 128-byte swizzle.

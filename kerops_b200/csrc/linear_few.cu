@@ -9,7 +9,6 @@
 //
 // 8-bit products of 16-bit rows: with at most eight rows every CTA quantises the rows it needs itself (they come from L2),
 // which is cheaper than a kernel in front.
-#include <stdlib.h>
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
@@ -133,6 +132,7 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const int n0 = blockIdx.x * 16;
     grid_dependency_wait();
+    grid_launch_dependents();
     int g = 0, begin = 0, end = p.T, last = p.T;
     if (p.ends) {
         if (warp == 0) {
@@ -276,15 +276,10 @@ static int few_warps(const FewParams& p, dim3 grid, cudaStream_t st) {
 template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
 static int few_launch(const FewParams& p, cudaStream_t st) {
     const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)(p.ends ? (p.E < p.T ? p.E : p.T) : 1));
-    constexpr int U0 = NT == 1 ? 8 : NT == 2 ? 4 : 2;
-    const char* f = getenv("KDW_FEW");
-    switch (f ? atoi(f) : 0) {
-        case 1: return few_warps<I8, BF16, QUANT, NT, VEC, 4, U0>(p, grid, st);
-        case 2: return few_warps<I8, BF16, QUANT, NT, VEC, 8, U0>(p, grid, st);
-        case 3: return few_warps<I8, BF16, QUANT, NT, VEC, 4, U0 / 2>(p, grid, st);
-        case 4: return few_warps<I8, BF16, QUANT, NT, VEC, 16, U0 / 2>(p, grid, st);
-        default: return few_warps<I8, BF16, QUANT, NT, VEC, 8, U0 / 2>(p, grid, st);
-    }
+    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four; rows
+    // that start anywhere need five loads and twenty operations to a piece: 27.6 us with four, 51 us with eight.
+    constexpr int U = (NT == 1 ? 8 : NT == 2 ? 4 : 2) / (VEC ? 1 : 2);
+    return few_warps<I8, BF16, QUANT, NT, VEC, 8, U>(p, grid, st);
 }
 template <bool I8, bool BF16, bool VEC>
 static int few_rows(const FewParams& p, cudaStream_t st) {

@@ -52,41 +52,47 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
 
     const int64_t k_elems = 128 / a.esize;
     pl->k_blocks = wgrad ? 0 : (int)ceil_div(con, k_elems);
-    pl->splits = 1;
     pl->chunk = 0;
-    // Tile and shares.  LINEAR_TILE (a build for measurements) fixes the tile.
+    // Tile and shares: the smallest estimate of the cycles on the busiest SM.  A stage of 64 (128 bytes of) contraction
+    // steps costs a CTA the larger of the products, 2 cycles a column, and shared memory, which writes and reads the stage
+    // at 128 bytes a cycle: 256 cycles for the M side and 2 a column of the N side it loads (a pair: half of them).  A
+    // tile costs some 1500 cycles more that the next one does not hide, adding shares 6000 of another kernel.
     const int64_t groups = std::min(a.E, a.T);
+    const double rows = (double)a.T / groups;  // of a group, about
     double best = 1e300;
-    for (int tile_m : {256, 128})
-        for (int bn : {256, 128, 64}) {
-            if (tile_m == 256 && bn == 64) continue;
-            const int slots = tile_m == 256 ? sms / 2 : sms;
-            // Groups are rounded up to whole tiles: at most one tile row more per group than the rows fill, half of
-            // one on average.
-            const double m_tiles = wgrad ? (double)ceil_div(a.N, tile_m) * a.E
-                                         : std::max<double>((double)ceil_div(a.T, tile_m), (double)a.T / tile_m + 0.5 * groups);
-            const double tiles = m_tiles * ceil_div(pl->out_cols, bn);
-            // time of a CTA in columns: its tiles times what a tile costs
-            const double per_tile = tile_m == 256 ? bn + 32 : bn + (bn == 256 ? 96 : 64);
-            const double cost = std::ceil(tiles / slots) * per_tile;
+    pl->splits = 1;
+    static const struct { int tile_m, bn; } tiles_of[] = {{256, 256}, {128, 256}, {128, 128}, {128, 64}};
+    for (auto& c : tiles_of) {
+        const char* force = getenv("KDW_LINEAR_TILE");
+        if (force && atoi(force) != c.tile_m * 1000 + c.bn) continue;
+        const bool pair = c.tile_m == 256;
+        const int slots = pair ? sms / 2 : sms;
+        const double m_tiles = (double)ceil_div(wgrad ? a.N : pl->out_cols, c.tile_m);
+        const double n_tiles = wgrad ? (double)ceil_div(pl->out_cols, c.bn) : std::ceil(rows / c.bn);
+        const double width = wgrad ? c.bn : std::min<double>(c.bn, std::ceil(rows / n_tiles / 32) * 32);
+        const double tiles = m_tiles * n_tiles * (wgrad ? a.E : groups);
+        const double block = std::max(2 * width, 256 + (pair ? 1 : 2) * (double)c.bn);
+        const double blocks = wgrad ? std::ceil(rows / 64) : pl->k_blocks;
+        for (int splits = 1; splits <= 64; splits *= 2) {
+            if (splits > 1 && (blocks / splits < 4 || tiles * splits > 2 * slots)) break;
+            const double units = tiles * splits;
+            const double cost = std::ceil(units / slots) * (blocks / splits * block + 1500) + (splits > 1 ? 6000 : 0);
             if (cost < best) {
                 best = cost;
-                pl->bn = bn;
-                pl->tile_m = tile_m;
+                pl->bn = c.bn;
+                pl->tile_m = c.tile_m;
+                pl->splits = splits;
             }
         }
-    if (const char* force = getenv("KDW_LINEAR_TILE")) {
-        pl->tile_m = atoi(force) / 1000;
-        pl->bn = atoi(force) % 1000;
     }
     const int slots = pl->tile_m == 256 ? sms / 2 : sms;
-    const int64_t m_tiles = wgrad ? ceil_div(a.N, pl->tile_m) : ceil_div(a.T, pl->tile_m) + groups - 1;
-    pl->n_tiles = (int)ceil_div(pl->out_cols, pl->bn);
-    pl->m_tiles = wgrad ? (int)m_tiles : 0;
-    const int64_t tiles = m_tiles * pl->n_tiles * (wgrad ? a.E : 1);
+    pl->m_tiles = (int)ceil_div(wgrad ? a.N : pl->out_cols, pl->tile_m);
+    pl->n_tiles = wgrad ? (int)ceil_div(pl->out_cols, pl->bn) : 0;
+    // the most there can be, however the rows are distributed
+    const int64_t tiles = pl->m_tiles * (wgrad ? pl->n_tiles * a.E : ceil_div(a.T, pl->bn) + groups - 1);
     pl->max_tiles = tiles;
-    pl->max_units = tiles;
-    bool split = false;
+    pl->max_units = tiles * pl->splits;
+    bool split = pl->splits > 1;
     if (wgrad) {
         // shares of the rows so that every SM has work
         int64_t chunk = round_up(std::max<int64_t>(a.T, 1), 64);
@@ -94,13 +100,11 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
             const int64_t per_tile = std::max<int64_t>(1, 2 * slots / tiles);
             chunk = std::max<int64_t>(256, round_up(ceil_div(a.T, per_tile), 64));
         }
+        pl->splits = 1;
         pl->chunk = (int)std::min<int64_t>(chunk, 1 << 30);
         split = pl->chunk < a.T || pl->fold > 1;  // the folded product's blocks are summed from the shares
+        pl->max_units = tiles;
         if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
-    } else if (tiles * 2 <= slots && pl->k_blocks >= 8) {
-        pl->splits = (int)std::min<int64_t>(slots / tiles, pl->k_blocks / 4);
-        split = pl->splits > 1;
-        pl->max_units = tiles * pl->splits;
     }
     int64_t off = 0;
     pl->off_a = pl->off_b = pl->off_table = 0;

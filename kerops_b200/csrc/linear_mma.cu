@@ -10,26 +10,27 @@ namespace kdw {
 
 // ------------------------------------------------------------------------------------------------------------------
 // The product kernel.  One persistent CTA per SM: warp 0 loads operand tiles with TMA into a ring of stages, warp 1
-// issues the tensor-core products into accumulators in tensor memory, warps 4-7 and 8-11 take finished accumulators in
-// turn and bring them to memory while the next tiles are being multiplied, warps 2-3 clear the output rows behind the
-// last group.
-//   A_ROWS / B_ROWS: the operand is stored with its output index contiguous (the contraction runs along memory rows)
-//   PAIR: two CTAs of a cluster share a 256 x BN tile.  Each loads its 128 rows of A and half of B's columns; the tensor
-//         cores of both read both halves of B, so a byte that enters shared memory is used for twice the products.  CTA 0
-//         waits for the loads of both and issues the products.
+// issues the tensor-core products into accumulators in tensor memory, warps 4-11 and 12-19 take finished accumulators in
+// turn and bring them to memory while the next tiles are being multiplied (eight warps to an accumulator: a warp reads 32
+// of its lanes and every other 32 of its columns), warps 2-3 clear the output rows behind the last group.
+//   M side: weights (row products; stored with the contraction contiguous for the forward pass, across it for the input
+//           gradient) or the gradient's rows, transposed (weight gradient).  N side: rows, or their transpose.
+//   PAIR: two CTAs of a cluster share a 256 x BN tile.  Each loads its 128 of M and half of N; the tensor cores of both
+//         read both halves of N, so a byte that enters shared memory is used for twice the products (a 128 x 256 tile of
+//         one CTA is bound by shared memory: 768 cycles to a stage where the products take 512).  CTA 0 waits for the
+//         loads of both and issues the products.
 // ------------------------------------------------------------------------------------------------------------------
-template <bool I8_, bool A_ROWS_, bool B_ROWS_, int BN_, bool PAIR_>
+template <int OP_, bool I8_, int BN_, bool PAIR_>
 struct LCfg {
-    static constexpr bool I8 = I8_, A_ROWS = A_ROWS_, B_ROWS = B_ROWS_, WGRAD = A_ROWS_, PAIR = PAIR_;
+    static constexpr bool I8 = I8_, WGRAD = OP_ == LIN_WGRAD, PAIR = PAIR_;
+    static constexpr bool A_ACROSS = OP_ != LIN_FWD, B_ACROSS = WGRAD;  // memory rows run across the contraction
     static constexpr int BN = BN_;
-    static constexpr int LOAD_N = PAIR ? BN / 2 : BN;  // columns of B that a CTA loads
-    static constexpr int THREADS = 384;
+    static constexpr int LOAD_N = PAIR ? BN / 2 : BN;  // of the N side, what a CTA loads
+    static constexpr int THREADS = 640;
     static constexpr int A_BYTES = kLinTileM * kLinSpan;
     static constexpr int B_BYTES = LOAD_N * kLinSpan;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int SCOLS = BN == 256 ? 32 : 64;  // output columns staged at a time
-    static constexpr int PITCH = SCOLS * 2 + 16;       // bytes of a staged row: free of bank conflicts
-    static constexpr int STAGING = 8 * 32 * PITCH;
+    static constexpr int STAGING = 16 * (1024 + (I8 ? 128 : 0));  // 16 rows of 64 bytes for each warp, and its rows' scales
     static constexpr int STAGES = (232448 - 1024 - STAGING - (int)sizeof(LinTable) - 512) / STAGE;
     static constexpr int ACCS = BN == 256 ? 2 : 4;
     static constexpr int TMEM_COLS = ACCS * BN;
@@ -40,26 +41,24 @@ struct LCfg {
     static_assert(SMEM <= 232448 && BARS * 8 + 16 <= 512, "");
 };
 
-// Writes `rows` x `cols` (<= SCOLS) staged 16-bit values of one warp to memory.
-template <int SCOLS, int PITCH>
+// 16 staged rows of 64 bytes; the 16-byte pieces of a row change places so that neither columns nor rows of pieces meet in
+// a bank.
+__device__ __forceinline__ int staged(int row, int piece) { return row * 64 + ((piece ^ (row >> 1)) & 3) * 16; }
+
+// Writes the first `rows` of 16 staged rows of `cols` (<= 32) values of one warp to memory.
 __device__ __forceinline__ void store_staged(const char* stage, char* dst, long long dst_pitch, int rows, int cols, bool vec,
                                              int lane) {
-    if (vec) {  // 16-byte pieces, SCOLS / 8 lanes to a row
-        constexpr int LPR = SCOLS / 8;
-        const int c = lane % LPR;
-        if (c * 8 < cols) {
-#pragma unroll
-            for (int r = lane / LPR; r < 32; r += 32 / LPR) {
-                if (r < rows)
-                    *reinterpret_cast<uint4*>(dst + r * dst_pitch + c * 16) =
-                        *reinterpret_cast<const uint4*>(stage + r * PITCH + c * 16);
-            }
-        }
-    } else {
-        for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < cols; c += 32)
-                *reinterpret_cast<uint16_t*>(dst + r * dst_pitch + c * 2) =
-                    *reinterpret_cast<const uint16_t*>(stage + r * PITCH + c * 2);
+    if (vec) {  // 16-byte pieces, four lanes to a row
+        const int c = lane & 3, r = lane >> 2;
+        const uint4 v0 = *reinterpret_cast<const uint4*>(stage + staged(r, c));
+        const uint4 v1 = *reinterpret_cast<const uint4*>(stage + staged(r + 8, c));
+        dst += r * dst_pitch + c * 16;
+        if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(dst) = v0;
+        if (r + 8 < rows && c * 8 < cols) *reinterpret_cast<uint4*>(dst + 8 * dst_pitch) = v1;
+    } else if (lane < cols) {
+        for (int r = 0; r < (rows < 16 ? rows : 16); ++r)
+            *reinterpret_cast<uint16_t*>(dst + r * dst_pitch + lane * 2) =
+                *reinterpret_cast<const uint16_t*>(stage + staged(r, lane >> 3) + (lane & 7) * 2);
     }
 }
 
@@ -84,6 +83,48 @@ __device__ __forceinline__ int boxes_inside(int left, int width) {
     const int n = (left + 63) >> 6;
     return n < 0 ? 0 : n > width / 64 ? width / 64 : n;
 }
+
+// What a CTA loads for a unit.  Boxes wholly beyond the output are not loaded: what is left in their place reaches only
+// rows and columns of the accumulator that are not stored.
+template <class C>
+struct LinLoad {
+    int g, c0, t0, kb, ke, k_row, k_rows, a_boxes, b_boxes;
+    uint32_t bytes;
+    __device__ __forceinline__ LinLoad(const LinParams& p, const LinTable* tab, int u, uint32_t rank) {
+        const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
+        g = w.g;
+        kb = w.kb;
+        ke = w.ke;
+        k_row = w.k_row;
+        k_rows = w.k_rows;
+        c0 = w.c0 + (int)rank * kLinTileM;
+        t0 = w.t0 + (int)rank * (C::WGRAD ? C::LOAD_N : w.width >> 1);
+        a_boxes = C::A_ACROSS ? boxes_inside((C::WGRAD ? p.out_rows : p.out_cols) - c0, kLinTileM) : 1;
+        b_boxes = C::WGRAD ? boxes_inside(p.out_cols - t0, C::LOAD_N) : 1;
+        bytes = (C::A_ACROSS ? a_boxes * 8192 : C::A_BYTES) + (C::WGRAD ? b_boxes * 8192 : C::B_BYTES);
+    }
+    __device__ __forceinline__ void load(const CUtensorMap* ma, const CUtensorMap* mb, int k, uint32_t a, uint32_t b,
+                                         uint32_t bar) const {
+        if constexpr (C::WGRAD) {
+            const int r = k_row + k * 64;
+#pragma unroll
+            for (int j = 0; j < kLinTileM / 64; ++j)
+                if (j < a_boxes) tma_load_2d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, r);
+#pragma unroll
+            for (int j = 0; j < C::LOAD_N / 64; ++j)
+                if (j < b_boxes) tma_load_2d<C::PAIR>(b + j * 8192, mb, bar, t0 + j * 64, r);
+        } else {
+            if constexpr (C::A_ACROSS) {
+#pragma unroll
+                for (int j = 0; j < kLinTileM / 64; ++j)
+                    if (j < a_boxes) tma_load_3d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, k * 64, g);
+            } else {
+                tma_load_3d<C::PAIR>(a, ma, bar, k * C::K_ELEMS, c0, g);
+            }
+            tma_load_2d<C::PAIR>(b, mb, bar, k * C::K_ELEMS, t0);
+        }
+    }
+};
 
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_constant__ CUtensorMap map_a,
@@ -111,7 +152,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         }
         for (int i = 0; i < C::ACCS; ++i) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, C::PAIR ? 8 : 4);
+            mbar_init(acc_empty + 8 * i, C::PAIR ? 16 : 8);
         }
         mbar_init(drain, 1);
         mbar_fence_init();
@@ -120,6 +161,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     }
     // operands, scales and `ends` may be the work of the kernel before this one
     grid_dependency_wait();
+    grid_launch_dependents();
     if (warp == 2) lin_build_table(p, tab->row, tab->unit, lane);
     tc_fence_before();
     __syncthreads();
@@ -134,8 +176,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             uint32_t phase = 0;
             bool ok = true;
             for (int u = first; u < units && ok; u += step) {
-                const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
-                const int m0 = w.m0 + (int)rank * kLinTileM, n0 = w.n0 + (int)rank * C::LOAD_N;
+                const LinLoad<C> w(p, tab, u, rank);
                 for (int k = w.kb; k < w.ke; ++k) {
                     if (p.stop_after >= 0 && loads >= p.stop_after) {
                         ok = false;
@@ -147,34 +188,17 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         break;
                     }
                     const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES;
-                    // Boxes wholly beyond the output are not loaded: what is left in their place reaches only rows and
-                    // columns of the accumulator that are not stored.
-                    const int a_boxes = C::WGRAD ? boxes_inside(p.out_rows - m0, kLinTileM) : 1;
-                    const int b_boxes = C::B_ROWS ? boxes_inside(p.out_cols - n0, C::LOAD_N) : 1;
-                    const uint32_t bytes = (C::WGRAD ? a_boxes * 8192 : C::A_BYTES) + (C::B_ROWS ? b_boxes * 8192 : C::B_BYTES);
                     uint32_t bar = full + 8 * stage;
                     if (rank == 0) {
-                        mbar_expect_tx(bar, bytes);
+                        mbar_expect_tx(bar, w.bytes);
                     } else if (C::WGRAD && w.k_rows - k * 64 < 64) {
                         bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
-                        mbar_expect_tx(bar, bytes);
+                        mbar_expect_tx(bar, w.bytes);
                     } else {
                         bar = cluster_addr(bar, 0);  // CTA 0 waits for the loads of both
-                        cluster_expect_tx(bar, bytes);
+                        cluster_expect_tx(bar, w.bytes);
                     }
-                    if constexpr (C::WGRAD) {
-                        const int r = w.k_row + k * 64;
-                        for (int j = 0; j < a_boxes; ++j) tma_load_2d<C::PAIR>(p.status, a + j * 8192, &map_a, bar, m0 + j * 64, r);
-                        for (int j = 0; j < b_boxes; ++j) tma_load_2d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, r);
-                    } else {
-                        tma_load_2d<C::PAIR>(p.status, a, &map_a, bar, k * C::K_ELEMS, m0);
-                        if constexpr (C::B_ROWS) {
-                            for (int j = 0; j < b_boxes; ++j)
-                                tma_load_3d<C::PAIR>(p.status, b + j * 8192, &map_b, bar, n0 + j * 64, k * 64, w.g);
-                        } else {
-                            tma_load_3d<C::PAIR>(p.status, b, &map_b, bar, k * C::K_ELEMS, n0, w.g);
-                        }
-                    }
+                    w.load(&map_a, &map_b, k, a, b, bar);
                     ++loads;
                     if (++stage == C::STAGES) {
                         stage = 0;
@@ -202,14 +226,14 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         uint32_t phase = 0, acc_phase = 0, partly_phase = 0;
         bool ok = true;
         for (int u = first; u < units && ok; u += step) {
-            const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+            const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
             if (w.kb == w.ke) continue;
             if (rank == 0) {
                 ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
                 if (!ok) break;
                 tc_fence_after();
             }
-            const uint32_t d = tmem + acc * C::BN;
+            const uint32_t d = tmem + acc * C::BN, idesc = p.idesc | (uint32_t)(w.width >> 3) << 17;
             for (int k = w.kb; k < w.ke; ++k) {
                 char* const sa = base + stage * C::STAGE;
                 // rows beyond the share are another group's (or of no group): their products must vanish even where
@@ -236,12 +260,12 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 if (rank == 0) {
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint64_t da = smem_desc(smem_u32(sa), C::A_ROWS);
-                        const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ROWS);
+                        const uint64_t da = smem_desc(smem_u32(sa), C::A_ACROSS);
+                        const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ACROSS);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            tc_mma<C::I8, C::PAIR>(d, da + i * (C::A_ROWS ? 2048 >> 4 : 32 >> 4),
-                                                   db + i * (C::B_ROWS ? 2048 >> 4 : 32 >> 4), p.idesc, k > w.kb || i > 0);
+                            tc_mma<C::I8, C::PAIR>(d, da + i * (C::A_ACROSS ? 2048 >> 4 : 32 >> 4),
+                                                   db + i * (C::B_ACROSS ? 2048 >> 4 : 32 >> 4), idesc, k > w.kb || i > 0);
                         tc_commit<C::PAIR>(empty + 8 * stage);
                         if (k + 1 == w.ke) tc_commit<C::PAIR>(acc_full + 8 * acc);
                     }
@@ -272,12 +296,12 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 p.table[p.E + 1 + i] = tab->unit[i];
             }
     } else {
-        const int q = warp & 3, turn = (warp >> 2) - 1;
-        char* const stg = staging + (warp - 4) * 32 * C::PITCH;
+        const int q = warp & 3, turn = (warp - 4) >> 3, odd = (warp >> 2) & 1 ^ 1;
+        char* const stg = staging + (warp - 4) * 1024;
         int acc = 0, count = 0;  // accumulators used so far: the two groups of warps take them in turn
         uint32_t acc_phase = 0;
         for (int u = first; u < units; u += step) {
-            const LinUnit w = lin_unit(p, tab->row, tab->unit, u, C::BN);
+            const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
             const bool any = w.ke > w.kb;
             const bool mine = (count & 1) == turn;
             if (any) ++count;
@@ -296,68 +320,109 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 tc_fence_after();
             }
             const uint32_t d = tmem + acc * C::BN + ((uint32_t)(q * 32) << 16);
-            const int row0 = w.m0 + (int)rank * kLinTileM + q * 32;
-            int rows = w.row_end - row0;
-            rows = rows > 32 ? 32 : rows;
-            if (!p.partial || (w.whole && p.fold == 1)) {
-                char* out = reinterpret_cast<char*>(p.out);
-                const long long pitch = (long long)p.out_cols * 2;
-                if (C::WGRAD) out += (long long)w.g * p.out_rows * pitch;
-                float rs = 1.f;
-                if (C::I8) rs = lane < rows ? __ldg(p.row_scale + row0 + lane) : 0.f;
-                const float* cs = C::I8 ? p.col_scale + (long long)w.g * p.out_cols : nullptr;
-#pragma unroll 1
-                for (int c0 = 0; c0 < C::BN; c0 += C::SCOLS) {
-                    int cols = p.out_cols - w.n0 - c0;
-                    if (cols <= 0 || rows <= 0) break;
-                    cols = cols > C::SCOLS ? C::SCOLS : cols;
-#pragma unroll
-                    for (int h = 0; h < C::SCOLS / 32; ++h) {
-                        uint32_t v[32];
-                        if (any) {
-                            tmem_load_32(d + c0 + h * 32, v);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 0u;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float f[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                if constexpr (C::I8) {
-                                    // one rounding of the exact sum and of each factor; the row's scale first, so
-                                    // that two small scales do not underflow in a product of their own
-                                    const int c = w.n0 + c0 + h * 32 + i + j;
-                                    f[j] = (float)(int)v[i + j] * rs * (c < p.out_cols ? __ldg(cs + c) : 0.f);
-                                } else {
-                                    f[j] = __uint_as_float(v[i + j]);
-                                }
-                            }
-                            uint4 o;
-                            o.x = pack2(f[0], f[1], p.out_bf16);
-                            o.y = pack2(f[2], f[3], p.out_bf16);
-                            o.z = pack2(f[4], f[5], p.out_bf16);
-                            o.w = pack2(f[6], f[7], p.out_bf16);
-                            *reinterpret_cast<uint4*>(stg + lane * C::PITCH + h * 64 + i * 2) = o;
-                        }
-                    }
-                    __syncwarp();
-                    store_staged<C::SCOLS, C::PITCH>(stg, out + row0 * pitch + (long long)(w.n0 + c0) * 2, pitch, rows, cols,
-                                                     p.out_vec, lane);
-                    __syncwarp();
-                }
-            } else {
-                // a share of a tile: column quadruples of a row side by side over the rows
+            const int c0 = w.c0 + (int)rank * kLinTileM + q * 32;  // of this warp's 32 lanes
+            const long long pitch = (long long)p.out_cols * 2;
+            if (p.partial && !(w.whole && p.fold == 1)) {
+                // a share of a tile: column quadruples of a lane side by side over the lanes
                 uint4* out = reinterpret_cast<uint4*>(p.partial) +
                              ((long long)u * (C::PAIR ? 2 : 1) + rank) * (C::BN / 4) * kLinTileM + q * 32 + lane;
 #pragma unroll 1
-                for (int c0 = 0; c0 < C::BN; c0 += 32) {
+                for (int n = 32 * odd; n < w.width; n += 64) {
                     uint32_t v[32];
-                    tmem_load_32(d + c0, v);
+                    tmem_load_32(d + n, v);
+                    tmem_wait(v);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        out[(long long)((c0 + i) / 4) * kLinTileM] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        out[(long long)((n + i) / 4) * kLinTileM] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            } else if constexpr (C::WGRAD) {
+                // lanes are output rows, accumulator columns output columns
+                char* out = reinterpret_cast<char*>(p.out) + ((long long)w.g * p.out_rows + c0) * pitch;
+                const int rows = p.out_rows - c0;
+#pragma unroll 1
+                for (int n = 32 * odd; n < C::BN; n += 64) {
+                    int cols = p.out_cols - w.t0 - n;
+                    if (cols <= 0 || rows <= 0) break;
+                    cols = cols > 32 ? 32 : cols;
+                    uint32_t v[32];
+                    if (any) {
+                        tmem_load_32(d + n, v);
+                        tmem_wait(v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0u;
+                    }
+                    uint4 o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[i].x = pack2(__uint_as_float(v[8 * i]), __uint_as_float(v[8 * i + 1]), p.out_bf16);
+                        o[i].y = pack2(__uint_as_float(v[8 * i + 2]), __uint_as_float(v[8 * i + 3]), p.out_bf16);
+                        o[i].z = pack2(__uint_as_float(v[8 * i + 4]), __uint_as_float(v[8 * i + 5]), p.out_bf16);
+                        o[i].w = pack2(__uint_as_float(v[8 * i + 6]), __uint_as_float(v[8 * i + 7]), p.out_bf16);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (lane >> 4 == h) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(stg + staged(lane & 15, i)) = o[i];
+                        }
+                        __syncwarp();
+                        store_staged(stg, out + 16 * h * pitch + (long long)(w.t0 + n) * 2, pitch, rows - 16 * h, cols, p.out_vec, lane);
+                        __syncwarp();
+                    }
+                }
+            } else {
+                // lanes are output channels, accumulator columns rows of the output: blocks are transposed on their way
+                // into shared memory
+                int cols = p.out_cols - c0;
+                cols = cols > 32 ? 32 : cols;
+                float cs[4];  // of channels l / 4 + 8 i
+                float* const srs = reinterpret_cast<float*>(staging + 16 * 1024) + (warp - 4) * 32;
+                if constexpr (C::I8) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int c = (lane >> 2) + 8 * i;
+                        cs[i] = c < cols ? __ldg(p.col_scale + (long long)w.g * p.out_cols + c0 + c) : 0.f;
+                    }
+                }
+                char* out = reinterpret_cast<char*>(p.out) + (w.t0 + 32ll * odd) * pitch + c0 * 2;
+                const uint32_t mat = smem_u32(stg) + staged(lane & 7, lane >> 3);
+#pragma unroll 1
+                for (int n = 32 * odd; n < w.rows; n += 64) {
+                    if (cols <= 0) break;
+                    const int rows = w.rows - n;
+                    if constexpr (C::I8) {
+                        srs[lane] = lane < rows ? __ldg(p.row_scale + w.t0 + n + lane) : 0.f;
+                        __syncwarp();
+                    }
+                    uint32_t v[32];
+                    tmem_load_frag(d + n, v);
+                    tmem_wait(v);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int j = 2 * h + k;
+                            float2 rs = make_float2(1.f, 1.f);
+                            if constexpr (C::I8) rs = *reinterpret_cast<const float2*>(srs + 8 * j + 2 * (lane & 3));
+                            uint32_t o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t a = v[16 * (i >> 1) + 4 * j + 2 * (i & 1)], b = v[16 * (i >> 1) + 4 * j + 2 * (i & 1) + 1];
+                                if constexpr (C::I8)
+                                    // one rounding of the exact sum and of each factor; the row's scale first, so that two
+                                    // small scales do not underflow in a product of their own
+                                    o[i] = pack2((float)(int)a * rs.x * cs[i], (float)(int)b * rs.y * cs[i], p.out_bf16);
+                                else
+                                    o[i] = pack2(__uint_as_float(a), __uint_as_float(b), p.out_bf16);
+                            }
+                            store_matrix_trans(mat + k * 512, o[0], o[1], o[2], o[3]);
+                        }
+                        __syncwarp();
+                        store_staged(stg, out + 16 * h * pitch, pitch, rows - 16 * h, cols, p.out_vec, lane);
+                        __syncwarp();
+                    }
+                    out += 64 * pitch;
                 }
             }
             if (any) {
@@ -394,6 +459,7 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
     const int* row = p.table;
     const int* unit = p.table + p.E + 1;
     grid_dependency_wait();
+    grid_launch_dependents();
     for (int i = blockIdx.x;; i += gridDim.x) {
         int t = i / blocks, g = 0, shares = 0, tiles = 0;  // the tile, counted over the groups
         for (; g < p.E; ++g) {
@@ -406,12 +472,12 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
         if (g == p.E) return;
         if (shares == 1) continue;
         const int u = unit[g] + t;
-        const LinUnit w = lin_unit(p, row, unit, u, BN);
-        const int part = i % blocks, quad = part % quads, m = part / quads * R + r;  // row of the tile
-        const int c0 = w.n0 + quad * 4;
-        if (c0 >= p.out_cols) continue;
+        const LinUnit w = lin_unit(p, row, unit, u);
+        const int part = i % blocks, n = part % quads * 4, m = part / quads * R + r;  // of the tile
+        if (n >= (p.wgrad ? p.out_cols - w.t0 : w.rows)) continue;
         const long long halves = p.tile_m / kLinTileM, step = tiles * halves * quads * kLinTileM;
-        const uint4* src = reinterpret_cast<const uint4*>(p.partial) + ((u * halves + m / kLinTileM) * quads + quad) * kLinTileM + m % kLinTileM;
+        const uint4* src = reinterpret_cast<const uint4*>(p.partial) +
+                           ((u * halves + m / kLinTileM) * quads + n / 4) * kLinTileM + m % kLinTileM;
         uint4 sum = make_uint4(0, 0, 0, 0);
         auto add = [&](const uint4& v) {
             if (I8) {
@@ -431,23 +497,23 @@ __global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__
         __syncthreads();
         s[l][r] = sum;
         __syncthreads();
-        if (l != 0 || w.m0 + m >= w.row_end) continue;
+        if (l != 0 || w.c0 + m >= (p.wgrad ? p.out_rows : p.out_cols)) continue;
 #pragma unroll
         for (int k = 1; k < L; ++k) add(s[k][r]);
         const uint32_t v[4] = {sum.x, sum.y, sum.z, sum.w};
-        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) +
-                        ((p.m_tiles ? (long long)w.g * p.out_rows : 0) + w.m0 + m) * p.out_cols + c0;
-        const float rs = I8 ? __ldg(p.row_scale + w.m0 + m) : 1.f;
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.out);
+        const float cs = I8 ? __ldg(p.col_scale + (long long)w.g * p.out_cols + w.c0 + m) : 1.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c0 + j < p.out_cols) {
-                float f;
-                if (I8)
-                    f = (float)(int)v[j] * rs * __ldg(p.col_scale + (long long)w.g * p.out_cols + c0 + j);
-                else
-                    f = __uint_as_float(v[j]);
-                out[j] = (uint16_t)pack2(f, 0.f, p.out_bf16);
+        for (int j = 0; j < 4; ++j) {
+            float f = __uint_as_float(v[j]);
+            if (p.wgrad) {
+                if (w.t0 + n + j < p.out_cols)
+                    out[((long long)w.g * p.out_rows + w.c0 + m) * p.out_cols + w.t0 + n + j] = (uint16_t)pack2(f, 0.f, p.out_bf16);
+            } else if (n + j < w.rows) {
+                if (I8) f = (float)(int)v[j] * __ldg(p.row_scale + w.t0 + n + j) * cs;
+                out[(long long)(w.t0 + n + j) * p.out_cols + w.c0 + m] = (uint16_t)pack2(f, 0.f, p.out_bf16);
             }
+        }
     }
 }
 
@@ -457,6 +523,7 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const __grid_constant_
     __shared__ float4 s[8];
     const int lane = threadIdx.x & 31, quads = K / 4, tiles = p.m_tiles * p.n_tiles;
     grid_dependency_wait();
+    grid_launch_dependents();
     const int shares = p.table[p.E + 1 + p.E] / tiles;
     for (int i = blockIdx.x; i < N * quads; i += gridDim.x) {
         const int n = i / quads, k = (i - n * quads) * 4;
@@ -465,9 +532,9 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const __grid_constant_
         for (int j = threadIdx.x; j < shares * p.fold; j += 256) {
             const int share = j / p.fold, block = j - share * p.fold;
             const int m = block * N + n, c = block * K + k;
-            const int mt = m / p.tile_m, nt = c / BN, band = mt / kLinBand;
-            const int high = p.m_tiles - band * kLinBand < kLinBand ? p.m_tiles - band * kLinBand : kLinBand;
-            const long long u = (long long)share * tiles + band * kLinBand * p.n_tiles + nt * high + mt - band * kLinBand;
+            const int mt = m / p.tile_m, nt = c / BN, band = nt / kLinBand;
+            const int wide = p.n_tiles - band * kLinBand < kLinBand ? p.n_tiles - band * kLinBand : kLinBand;
+            const long long u = (long long)share * tiles + (p.m_tiles > 1 ? band * kLinBand * p.m_tiles + mt * wide + nt - band * kLinBand : nt);
             const long long half = u * (p.tile_m / kLinTileM) + (m % p.tile_m) / kLinTileM;
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial) + (half * (BN / 4) + (c % BN) / 4) * kLinTileM + m % kLinTileM);
             sum.x += v.x;
@@ -501,6 +568,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ sr
                                                         long long src_stride, int dst_stride) {
     constexpr int V = 16 / sizeof(T);
     grid_dependency_wait();
+    grid_launch_dependents();
     const int per_row = (cols + V - 1) / V;
     const long long n = rows * per_row;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
@@ -545,16 +613,14 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     return 0;
 }
 
-template <bool I8, bool AR, bool BR>
+template <int OP, bool I8>
 static int launch_width(const LinPlan& pl, const CUtensorMap& ma, const CUtensorMap& mb, const LinParams& p,
                         cudaStream_t st) {
-    if (pl.tile_m == 256)
-        return pl.bn == 128 ? launch_product<LCfg<I8, AR, BR, 128, true>>(pl, ma, mb, p, st)
-                            : launch_product<LCfg<I8, AR, BR, 256, true>>(pl, ma, mb, p, st);
+    if (pl.tile_m == 256) return launch_product<LCfg<OP, I8, 256, true>>(pl, ma, mb, p, st);
     switch (pl.bn) {
-        case 64: return launch_product<LCfg<I8, AR, BR, 64, false>>(pl, ma, mb, p, st);
-        case 128: return launch_product<LCfg<I8, AR, BR, 128, false>>(pl, ma, mb, p, st);
-        default: return launch_product<LCfg<I8, AR, BR, 256, false>>(pl, ma, mb, p, st);
+        case 64: return launch_product<LCfg<OP, I8, 64, false>>(pl, ma, mb, p, st);
+        case 128: return launch_product<LCfg<OP, I8, 128, false>>(pl, ma, mb, p, st);
+        default: return launch_product<LCfg<OP, I8, 256, false>>(pl, ma, mb, p, st);
     }
 }
 
@@ -600,7 +666,10 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     p.T = (int)(a.T / pl.fold);
     p.fold = pl.fold;
     p.E = (int)a.E;
+    p.wgrad = a.op == LIN_WGRAD;
     p.tile_m = pl.tile_m;
+    p.bn = pl.bn;
+    p.bn_log = pl.bn == 256 ? 8 : pl.bn == 128 ? 7 : 6;
     p.m_tiles = pl.m_tiles;
     p.n_tiles = pl.n_tiles;
     p.out_rows = pl.out_rows;
@@ -619,25 +688,25 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     const WaitTest wt = wait_test();
     p.limit_ns = wt.limit_ns;
     p.stop_after = wt.stop_after;
-    const bool wgrad = a.op == LIN_WGRAD, b_rows = a.op != LIN_FWD;
-    // accumulator fp32 (1) or int32 (2); operands fp16 (0) / bf16 (1) / int8 (1); which are stored by output index
+    // accumulator fp32 (1) or int32 (2); operands fp16 (0) / bf16 (1) / int8 (1); which run across the contraction; M
     const uint32_t fmt = pl.esize == 1 ? 1u : (uint32_t)a.in_bf16;
-    p.idesc = (pl.esize == 1 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)wgrad << 15 | (uint32_t)b_rows << 16 |
-              (uint32_t)(pl.bn >> 3) << 17 | (uint32_t)(pl.tile_m >> 4) << 24;
+    p.idesc = (pl.esize == 1 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)(a.op != LIN_FWD) << 15 |
+              (uint32_t)p.wgrad << 16 | (uint32_t)(pl.tile_m >> 4) << 24;
+    // the M side is the weights (row products) or the gradient, the N side the rows
     CUtensorMap ma, mb;
-    const int span = kLinSpan / pl.esize;
-    rc = encode_rows_map(&ma, pa, pl.esize, pl.a_cols, pl.a_rows, sa, 0, 0, span, wgrad ? 64 : kLinTileM);
+    const int span = kLinSpan / pl.esize, load_n = pl.tile_m == 256 ? pl.bn / 2 : pl.bn;
+    if (p.wgrad) {
+        rc = encode_rows_map(&ma, pa, pl.esize, pl.a_cols, pl.a_rows, sa, 0, 0, span, 64);
+        if (!rc) rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows, sb, 0, 0, span, 64);
+        return rc ? rc : launch_width<LIN_WGRAD, false>(pl, ma, mb, p, st);
+    }
+    const int64_t wrows = pl.b_rows / a.E;
+    rc = encode_rows_map(&ma, pb, pl.esize, pl.b_cols, wrows, sb, a.E, wrows * sb, span, a.op == LIN_FWD ? kLinTileM : 64);
+    if (!rc) rc = encode_rows_map(&mb, pa, pl.esize, pl.a_cols, pl.a_rows, sa, 0, 0, span, load_n);
     if (rc) return rc;
-    if (wgrad)
-        rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows, sb, 0, 0, 64, 64);
-    else
-        rc = encode_rows_map(&mb, pb, pl.esize, pl.b_cols, pl.b_rows / a.E, sb, a.E, pl.b_rows / a.E * sb, span,
-                             b_rows ? 64 : pl.tile_m == 256 ? pl.bn / 2 : pl.bn);
-    if (rc) return rc;
-    if (pl.esize == 1) return launch_width<true, false, false>(pl, ma, mb, p, st);
-    if (wgrad) return launch_width<false, true, true>(pl, ma, mb, p, st);
-    if (b_rows) return launch_width<false, false, true>(pl, ma, mb, p, st);
-    return launch_width<false, false, false>(pl, ma, mb, p, st);
+    if (pl.esize == 1) return launch_width<LIN_FWD, true>(pl, ma, mb, p, st);
+    if (a.op == LIN_DGRAD) return launch_width<LIN_DGRAD, false>(pl, ma, mb, p, st);
+    return launch_width<LIN_FWD, false>(pl, ma, mb, p, st);
 }
 
 }  // namespace kdw

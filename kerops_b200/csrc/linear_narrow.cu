@@ -72,6 +72,7 @@ __global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(cons
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const long long warp = ((long long)blockIdx.x * C::THREADS + threadIdx.x) >> 5, warps = (long long)gridDim.x * (C::THREADS / 32);
     grid_dependency_wait();
+    grid_launch_dependents();
     long long rows = p.T;
     if (p.ends) {
         const int e = __ldg(p.ends);

@@ -25,6 +25,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
     constexpr int RPB = 256 / TPR;
     const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
     grid_dependency_wait();
+    grid_launch_dependents();
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
         const long long r = r0 + sub;
         const bool live = r < rows;
