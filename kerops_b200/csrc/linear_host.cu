@@ -2,6 +2,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/kdw.h"
@@ -24,6 +25,39 @@ static int fold_of(const LinArgs& a) {
     int f = 1;
     while (f < 8 && narrow * f * 2 <= 64 && a.T % (f * 2) == 0) f *= 2;
     return f;
+}
+
+int device_facts(int** status, int* sms) {
+    struct Facts {
+        int* status;
+        std::atomic<int> sms;  // set last; a race only repeats the lookup
+    };
+    static Facts facts[KernelSetup::kMaxDevices];
+    int dev = 0;
+    KDW_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= KernelSetup::kMaxDevices) {
+        set_error("device index %d is outside the supported range 0..%d", dev, KernelSetup::kMaxDevices - 1);
+        return KDW_ERR_ARG;
+    }
+    // A thread that has made no runtime call yet (a worker of an autograd engine) has no current context, which encoding a
+    // tensor map needs.
+    static thread_local int bound = -1;
+    if (bound != dev) {
+        KDW_CUDA(cudaFree(nullptr));
+        bound = dev;
+    }
+    Facts& f = facts[dev];
+    if (f.sms.load(std::memory_order_acquire) == 0) {
+        int* p = nullptr;
+        int n = 0, rc = status_ptr(&p);
+        if (!rc) rc = device_sm_count(&n);
+        if (rc) return rc;
+        f.status = p;
+        f.sms.store(n, std::memory_order_release);
+    }
+    if (status) *status = f.status;
+    *sms = f.sms.load(std::memory_order_relaxed);
+    return 0;
 }
 
 int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
@@ -52,17 +86,26 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
 
     const int64_t k_elems = 128 / a.esize;
     pl->k_blocks = wgrad ? 0 : (int)ceil_div(con, k_elems);
-    pl->chunk = 0;
-    // Tile and shares: the smallest estimate of the cycles on the busiest SM.  A stage of 64 (128 bytes of) contraction
+    // Tile and parts: the smallest estimate of the cycles on the busiest SM.  A stage of 64 (128 bytes of) contraction
     // steps costs a CTA the larger of the products, 2 cycles a column, and shared memory, which writes and reads the stage
     // at 128 bytes a cycle: 256 cycles for the M side and 2 a column of the N side it loads (a pair: half of them).  A
-    // tile costs some 1500 cycles more that the next one does not hide, adding shares 6000 of another kernel.
+    // tile costs some 1500 cycles more that the next one does not hide, and 4000 to 10000 where two to eight CTAs of a
+    // cluster share it (500 x 1000 -> 1000: 2 us for four).
+    // Shares of the weight gradient that are added in memory cost another kernel and their bytes, written and read.
     const int64_t groups = std::min(a.E, a.T);
     const double rows = (double)a.T / groups;  // of a group, about
+    const int cluster_slots[] = {0, sms, 0, 0, 132 * sms / 148, 0, 0, 0, 120 * sms / 148};  // CTAs in clusters that fit at once
     double best = 1e300;
-    pl->splits = 1;
-    static const struct { int tile_m, bn; } tiles_of[] = {{256, 256}, {128, 256}, {128, 128}, {128, 64}};
-    for (auto& c : tiles_of) {
+    auto consider = [&](double cost, int tile_m, int bn, int splits, int64_t chunk) {
+        if (cost >= best) return;
+        best = cost;
+        pl->tile_m = tile_m;
+        pl->bn = bn;
+        pl->splits = splits;
+        pl->chunk = (int)chunk;
+    };
+    static const struct { int tile_m, bn; } shapes[] = {{256, 256}, {128, 256}, {128, 128}, {128, 64}};
+    for (auto& c : shapes) {
         const char* force = getenv("KDW_LINEAR_TILE");
         if (force && atoi(force) != c.tile_m * 1000 + c.bn) continue;
         const bool pair = c.tile_m == 256;
@@ -73,39 +116,29 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
         const double tiles = m_tiles * n_tiles * (wgrad ? a.E : groups);
         const double block = std::max(2 * width, 256 + (pair ? 1 : 2) * (double)c.bn);
         const double blocks = wgrad ? std::ceil(rows / 64) : pl->k_blocks;
-        for (int splits = 1; splits <= 64; splits *= 2) {
-            if (splits > 1 && (blocks / splits < 4 || tiles * splits > 2 * slots)) break;
-            const double units = tiles * splits;
-            const double cost = std::ceil(units / slots) * (blocks / splits * block + 1500) + (splits > 1 ? 6000 : 0);
-            if (cost < best) {
-                best = cost;
-                pl->bn = c.bn;
-                pl->tile_m = c.tile_m;
-                pl->splits = splits;
-            }
+        if (pl->fold == 1) {
+            consider(std::ceil(tiles / slots) * (blocks * block + 1500), c.tile_m, c.bn, 1, INT32_MAX);
+            for (int splits = 2; splits <= 8 && !pair; splits *= 2)
+                if (blocks / splits >= 2 && tiles * splits <= (splits == 2 ? sms : cluster_slots[splits]))
+                    consider(std::ceil(blocks / splits) * block + 3500 + 1000 * splits, c.tile_m, c.bn, splits, INT32_MAX);
+        }
+        if (!wgrad || (pl->fold == 1 && (tiles > slots || rows < 1024))) continue;
+        for (int waves = 1; waves <= 2; ++waves) {
+            const double shares = std::max(1.0, std::floor(waves * slots / tiles));
+            const int64_t chunk = std::max<int64_t>(256, round_up((int64_t)std::ceil(rows / shares), 64));
+            const double units = tiles * std::ceil(rows / chunk), bytes = units * c.tile_m * c.bn * 4;
+            consider(std::ceil(units / slots) * (chunk / 64 * block + 1500) + 6000 + bytes / (sms * 10.0), c.tile_m, c.bn, 1,
+                     std::min<int64_t>(chunk, 1 << 30));
         }
     }
-    const int slots = pl->tile_m == 256 ? sms / 2 : sms;
     pl->m_tiles = (int)ceil_div(wgrad ? a.N : pl->out_cols, pl->tile_m);
     pl->n_tiles = wgrad ? (int)ceil_div(pl->out_cols, pl->bn) : 0;
     // the most there can be, however the rows are distributed
-    const int64_t tiles = pl->m_tiles * (wgrad ? pl->n_tiles * a.E : ceil_div(a.T, pl->bn) + groups - 1);
-    pl->max_tiles = tiles;
-    pl->max_units = tiles * pl->splits;
-    bool split = pl->splits > 1;
-    if (wgrad) {
-        // shares of the rows so that every SM has work
-        int64_t chunk = round_up(std::max<int64_t>(a.T, 1), 64);
-        if (tiles < 2 * slots && a.T > 512) {
-            const int64_t per_tile = std::max<int64_t>(1, 2 * slots / tiles);
-            chunk = std::max<int64_t>(256, round_up(ceil_div(a.T, per_tile), 64));
-        }
-        pl->splits = 1;
-        pl->chunk = (int)std::min<int64_t>(chunk, 1 << 30);
-        split = pl->chunk < a.T || pl->fold > 1;  // the folded product's blocks are summed from the shares
-        pl->max_units = tiles;
-        if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
-    }
+    pl->max_tiles = pl->m_tiles * (wgrad ? pl->n_tiles * a.E : ceil_div(a.T, pl->bn) + groups - 1);
+    pl->max_units = pl->max_tiles;
+    // (the folded product's blocks are summed from the shares, whatever their number)
+    const bool split = wgrad && (pl->chunk < a.T || pl->fold > 1);
+    if (split) pl->max_units = (int64_t)pl->m_tiles * pl->n_tiles * (a.T / pl->chunk + a.E);
     int64_t off = 0;
     pl->off_a = pl->off_b = pl->off_table = 0;
     pl->off_partial = -1;
@@ -230,7 +263,7 @@ static bool quant_inside(const LinArgs& a, int x_type) {
 static int plan_and_run(LinArgs* a, void* workspace, int64_t workspace_bytes, void* stream) {
     LinPlan pl;
     int sms = 0;
-    int rc = device_sm_count(&sms);
+    int rc = device_facts(nullptr, &sms);
     if (!rc) rc = linear_plan(&pl, *a, sms);
     if (rc) return rc;
     if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || ((uintptr_t)workspace & 255) != 0)) {
@@ -252,7 +285,7 @@ int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int
     LinPlan pl;
     int sms = 0;
     int rc = f16_args(&args, op, a, b, T, E, K, N, a_stride, b_stride, dtype);
-    if (!rc) rc = device_sm_count(&sms);
+    if (!rc) rc = device_facts(nullptr, &sms);
     if (!rc && (is_few(args) || is_narrow(args))) return 0;
     if (!rc) rc = linear_plan(&pl, args, sms);
     return rc ? (rc < 0 ? rc : -rc) : pl.bytes;
@@ -289,7 +322,7 @@ int64_t kdw_linear_i8_workspace_bytes(const void* x, const void* w, int64_t T, i
     I8Layout l;
     int sms = 0;
     int rc = i8_args(&args, &l, x, w, T, E, K, N, x_stride, x_type, dtype);
-    if (!rc) rc = device_sm_count(&sms);
+    if (!rc) rc = device_facts(nullptr, &sms);
     if (!rc && is_few(args)) return quant_inside(args, x_type) ? 0 : l.off_rest;
     if (!rc) rc = linear_plan(&pl, args, sms);
     return rc ? (rc < 0 ? rc : -rc) : l.off_rest + pl.bytes;

@@ -1,6 +1,9 @@
 // Channel-mixing products of ragged row groups: forward, input gradient, weight gradient (16-bit operands) and the
 // 8-bit integer product with a scale per row and per output channel.
+#include <limits.h>
 #include <string.h>
+
+#include <algorithm>
 
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
@@ -9,10 +12,10 @@
 namespace kdw {
 
 // ------------------------------------------------------------------------------------------------------------------
-// The product kernel.  One persistent CTA per SM: warp 0 loads operand tiles with TMA into a ring of stages, warp 1
-// issues the tensor-core products into accumulators in tensor memory, warps 4-11 and 12-19 take finished accumulators in
+// The product kernel.  One persistent CTA per SM: warp 2 finds the CTA's units and hands their descriptions to the others
+// through a ring in shared memory, warp 0 loads operand tiles with TMA into a ring of stages, warp 1 issues the tensor-core products into accumulators in tensor memory, warps 4-11 and 12-19 take finished accumulators in
 // turn and bring them to memory while the next tiles are being multiplied (eight warps to an accumulator: a warp reads 32
-// of its lanes and every other 32 of its columns), warps 2-3 clear the output rows behind the last group.
+// of its lanes and every other 32 of its columns), warp 3 clears the output rows behind the last group.
 //   M side: weights (row products; stored with the contraction contiguous for the forward pass, across it for the input
 //           gradient) or the gradient's rows, transposed (weight gradient).  N side: rows, or their transpose.
 //   PAIR: two CTAs of a cluster share a 256 x BN tile.  Each loads its 128 of M and half of N; the tensor cores of both
@@ -31,14 +34,15 @@ struct LCfg {
     static constexpr int B_BYTES = LOAD_N * kLinSpan;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGING = 16 * (1024 + (I8 ? 128 : 0));  // 16 rows of 64 bytes for each warp, and its rows' scales
-    static constexpr int STAGES = (232448 - 1024 - STAGING - (int)sizeof(LinTable) - 512) / STAGE;
+    static constexpr int STAGES = (232448 - 1024 - STAGING - (int)sizeof(LinTable) - 768) / STAGE;
     static constexpr int ACCS = BN == 256 ? 2 : 4;
     static constexpr int TMEM_COLS = ACCS * BN;
-    static constexpr int BARS = 3 * STAGES + 2 * ACCS + 1;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + (int)sizeof(LinTable) + BARS * 8 + 16;
+    static constexpr int UNITS = 4;  // descriptions on their way
+    static constexpr int BARS = 3 * STAGES + 2 * ACCS + 1 + 2 * UNITS;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + STAGING + UNITS * (int)sizeof(LinUnit) + (int)sizeof(LinTable) + BARS * 8 + 16;
     static constexpr int K_ELEMS = I8 ? 128 : 64;  // contraction steps of a stage
     static_assert(LOAD_N >= 64 && TMEM_COLS >= 32 && TMEM_COLS <= 512, "");
-    static_assert(SMEM <= 232448 && BARS * 8 + 16 <= 512, "");
+    static_assert(SMEM <= 232448 && BARS * 8 + 16 + UNITS * (int)sizeof(LinUnit) <= 768, "");
 };
 
 // 16 staged rows of 64 bytes; the 16-byte pieces of a row change places so that neither columns nor rows of pieces meet in
@@ -90,8 +94,7 @@ template <class C>
 struct LinLoad {
     int g, c0, t0, kb, ke, k_row, k_rows, a_boxes, b_boxes;
     uint32_t bytes;
-    __device__ __forceinline__ LinLoad(const LinParams& p, const LinTable* tab, int u, uint32_t rank) {
-        const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
+    __device__ __forceinline__ LinLoad(const LinParams& p, const LinUnit& w, uint32_t rank) {
         g = w.g;
         kb = w.kb;
         ke = w.ke;
@@ -126,6 +129,82 @@ struct LinLoad {
     }
 };
 
+template <bool I8>
+__device__ __forceinline__ void add_share(uint4& sum, const uint4& v) {
+    if (I8) {
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+    } else {
+        sum.x = __float_as_uint(__uint_as_float(sum.x) + __uint_as_float(v.x));
+        sum.y = __float_as_uint(__uint_as_float(sum.y) + __uint_as_float(v.y));
+        sum.z = __float_as_uint(__uint_as_float(sum.z) + __uint_as_float(v.z));
+        sum.w = __float_as_uint(__uint_as_float(sum.w) + __uint_as_float(v.w));
+    }
+}
+
+// The CTAs of a cluster add their parts of a tile: CTA `part` takes its share of the column quadruples, in the order of the
+// parts.
+template <class C, int PARTS>
+__device__ __forceinline__ void add_parts(const LinParams& p, const LinUnit& w, int part, uint32_t tile) {
+    const int m = threadIdx.x & 127, c = w.c0 + m;
+    const int cols = C::WGRAD ? (p.out_cols - w.t0 < C::BN ? p.out_cols - w.t0 : C::BN) : w.rows;
+    const bool live = c < (C::WGRAD ? p.out_rows : p.out_cols);
+    float cs = 1.f;
+    if (C::I8 && live) cs = __ldg(p.col_scale + (long long)w.g * p.out_cols + c);
+    uint16_t* out = reinterpret_cast<uint16_t*>(p.out) +
+                    (C::WGRAD ? ((long long)w.g * p.out_rows + c) * p.out_cols + w.t0 : (long long)w.t0 * p.out_cols + c);
+    const int quads = (cols + 3) >> 2, end = quads * (part + 1) / PARTS;
+    uint32_t src[PARTS];
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) src[k] = cluster_addr(tile + m * 16, k);
+    for (int j = quads * part / PARTS + (threadIdx.x >> 7); j < end; j += C::THREADS / 128) {
+        uint4 v[PARTS];
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) v[k] = cluster_load(src[k] + j * kLinTileM * 16);
+#pragma unroll
+        for (int k = 1; k < PARTS; ++k) add_share<C::I8>(v[0], v[k]);
+        if (!live) continue;
+        const uint32_t s[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f[e] = __uint_as_float(s[e]);
+            if (C::I8) f[e] = 4 * j + e < cols ? (float)(int)s[e] * __ldg(p.row_scale + w.t0 + 4 * j + e) * cs : 0.f;
+        }
+        const uint32_t lo = pack2(f[0], f[1], p.out_bf16), hi = pack2(f[2], f[3], p.out_bf16);
+        if (C::WGRAD && p.out_vec) {
+            *reinterpret_cast<uint2*>(out + 4 * j) = make_uint2(lo, hi);  // rows are multiples of 8 values
+        } else {
+            const long long next = C::WGRAD ? 1 : p.out_cols;
+            uint16_t* o = out + 4 * j * next;
+            if (4 * j < cols) o[0] = (uint16_t)lo;
+            if (4 * j + 1 < cols) o[next] = (uint16_t)(lo >> 16);
+            if (4 * j + 2 < cols) o[2 * next] = (uint16_t)hi;
+            if (4 * j + 3 < cols) o[3 * next] = (uint16_t)(hi >> 16);
+        }
+    }
+}
+
+// The next unit's description; lanes of a warp take it together and give the place back.
+__device__ __forceinline__ bool take_unit(LinUnit& w, const LinUnit* ring, uint32_t full, uint32_t empty, int& slot, uint32_t& phase,
+                                          int slots, int lane, const LinParams& p) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + 8 * slot, phase, p.limit_ns));
+    if (!ok) {
+        if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        return false;
+    }
+    w = ring[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * slot);
+    if (++slot == slots) {
+        slot = 0;
+        phase ^= 1;
+    }
+    return w.u >= 0;
+}
+
 template <class C>
 __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                const __grid_constant__ CUtensorMap map_b,
@@ -133,14 +212,18 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     extern __shared__ char smem_raw[];
     char* const base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     char* const staging = base + C::STAGES * C::STAGE;
-    LinTable* const tab = reinterpret_cast<LinTable*>(staging + C::STAGING);
+    LinUnit* const ring = reinterpret_cast<LinUnit*>(staging + C::STAGING);
+    LinTable* const tab = reinterpret_cast<LinTable*>(ring + C::UNITS);
     uint64_t* const bars = reinterpret_cast<uint64_t*>(tab + 1);
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + C::BARS);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES,
-                   acc_empty = acc_full + 8 * C::ACCS, drain = acc_empty + 8 * C::ACCS, partly = drain + 8;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * C::STAGES, partly = empty + 8 * C::STAGES,
+                   acc_full = partly + 8 * C::STAGES, acc_empty = acc_full + 8 * C::ACCS, drain = acc_empty + 8 * C::ACCS,
+                   unit_full = drain + 8, unit_empty = unit_full + 8 * C::UNITS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = C::PAIR ? cluster_rank() : 0;
-    const int first = C::PAIR ? blockIdx.x >> 1 : blockIdx.x, step = C::PAIR ? gridDim.x >> 1 : gridDim.x;
+    // Few tiles: a cluster of CTAs takes one tile, a part of the contraction each, and adds the parts at the end.
+    const bool shared_tile = !C::PAIR && p.splits > 1;
+    const int part = shared_tile ? (int)cluster_rank() : 0;
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&map_a);
@@ -155,6 +238,10 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             mbar_init(acc_empty + 8 * i, C::PAIR ? 16 : 8);
         }
         mbar_init(drain, 1);
+        for (int i = 0; i < C::UNITS; ++i) {
+            mbar_init(unit_full + 8 * i, 1);
+            mbar_init(unit_empty + 8 * i, 18);  // warps 0, 1 and 4-19
+        }
         mbar_fence_init();
     } else if (warp == 1) {
         tmem_alloc<C::PAIR>(smem_u32(s_tmem), C::TMEM_COLS);
@@ -168,56 +255,58 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     if (C::PAIR) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
-    const int units = tab->unit[p.E];
+    int slot = 0;  // of the ring of units
+    uint32_t slot_phase = 0;
+    LinUnit w;
 
     if (warp == 0) {
-        if (elect_one()) {
-            int loads = 0, stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int u = first; u < units && ok; u += step) {
-                const LinLoad<C> w(p, tab, u, rank);
-                for (int k = w.kb; k < w.ke; ++k) {
-                    if (p.stop_after >= 0 && loads >= p.stop_after) {
-                        ok = false;
-                        break;
-                    }
-                    if (!lin_wait<C::PAIR>(empty + 8 * stage, phase ^ 1, p.limit_ns)) {
-                        atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
-                        ok = false;
-                        break;
-                    }
+        int loads = 0, stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        while (ok && take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
+            const LinLoad<C> l(p, w, rank);
+            for (int k = l.kb; k < l.ke; ++k) {
+                if (p.stop_after >= 0 && loads >= p.stop_after) {
+                    ok = false;
+                    break;
+                }
+                ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(empty + 8 * stage, phase ^ 1, p.limit_ns));
+                if (!ok) {
+                    if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+                    break;
+                }
+                if (elect_one()) {
                     const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES;
                     uint32_t bar = full + 8 * stage;
                     if (rank == 0) {
-                        mbar_expect_tx(bar, w.bytes);
-                    } else if (C::WGRAD && w.k_rows - k * 64 < 64) {
+                        mbar_expect_tx(bar, l.bytes);
+                    } else if (C::WGRAD && l.k_rows - k * 64 < 64) {
                         bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
-                        mbar_expect_tx(bar, w.bytes);
+                        mbar_expect_tx(bar, l.bytes);
                     } else {
                         bar = cluster_addr(bar, 0);  // CTA 0 waits for the loads of both
-                        cluster_expect_tx(bar, w.bytes);
+                        cluster_expect_tx(bar, l.bytes);
                     }
-                    w.load(&map_a, &map_b, k, a, b, bar);
-                    ++loads;
-                    if (++stage == C::STAGES) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
+                    l.load(&map_a, &map_b, k, a, b, bar);
+                }
+                __syncwarp();
+                ++loads;
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1;
                 }
             }
-            // a CTA (a pair) leaves only when its last copies have landed
-            if (rank == 0) {
-                const int last = loads < C::STAGES ? loads : C::STAGES;
-                for (int i = 0; i < last; ++i) {
-                    if (stage == 0) {
-                        stage = C::STAGES;
-                        phase ^= 1;
-                    }
-                    --stage;
-                    if (!lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns))
-                        atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        }
+        // a CTA (a pair) leaves only when its last copies have landed
+        if (rank == 0) {
+            const int last = loads < C::STAGES ? loads : C::STAGES;
+            for (int i = 0; i < last; ++i) {
+                if (stage == 0) {
+                    stage = C::STAGES;
+                    phase ^= 1;
                 }
+                --stage;
+                if (!lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
             }
         }
         __syncwarp();
@@ -225,8 +314,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0, partly_phase = 0;
         bool ok = true;
-        for (int u = first; u < units && ok; u += step) {
-            const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
+        while (ok && take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
             if (w.kb == w.ke) continue;
             if (rank == 0) {
                 ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
@@ -259,17 +347,15 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 }
                 if (rank == 0) {
                     tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t da = smem_desc(smem_u32(sa), C::A_ACROSS);
-                        const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ACROSS);
+                    const uint32_t el = elect_one();
+                    const uint64_t da = smem_desc(smem_u32(sa), C::A_ACROSS);
+                    const uint64_t db = smem_desc(smem_u32(sa) + C::A_BYTES, C::B_ACROSS);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc_mma<C::I8, C::PAIR>(d, da + i * (C::A_ACROSS ? 2048 >> 4 : 32 >> 4),
-                                                   db + i * (C::B_ACROSS ? 2048 >> 4 : 32 >> 4), idesc, k > w.kb || i > 0);
-                        tc_commit<C::PAIR>(empty + 8 * stage);
-                        if (k + 1 == w.ke) tc_commit<C::PAIR>(acc_full + 8 * acc);
-                    }
-                    __syncwarp();
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma<C::I8, C::PAIR>(el, d, da + i * (C::A_ACROSS ? 2048 >> 4 : 32 >> 4),
+                                               db + i * (C::B_ACROSS ? 2048 >> 4 : 32 >> 4), idesc, k > w.kb || i > 0);
+                    tc_commit<C::PAIR>(el, empty + 8 * stage);
+                    if (k + 1 == w.ke) tc_commit<C::PAIR>(el, acc_full + 8 * acc);
                 }
                 if (++stage == C::STAGES) {
                     stage = 0;
@@ -283,15 +369,38 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         }
         if (!ok && lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         // products in flight still read shared memory and write tensor memory
-        if (rank == 0 && elect_one()) {
-            tc_commit<C::PAIR>(drain);
+        if (rank == 0) {
+            tc_commit<C::PAIR>(elect_one(), drain);
             if (!lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         }
         __syncwarp();
-    } else if (warp < 4) {
-        if (!C::WGRAD) clear_rows(p, tab->row[p.E], threadIdx.x - 64, 64);
+    } else if (warp == 2) {
+        const int units = tab->unit[p.E];
+        const int first = C::PAIR ? blockIdx.x >> 1 : shared_tile ? blockIdx.x / p.splits : blockIdx.x;
+        const int step = C::PAIR ? gridDim.x >> 1 : shared_tile ? units : gridDim.x;
+        for (int u = first;; u += step) {
+            const bool more = u < units;
+            if (more) w = lin_unit(p, tab->row, tab->unit, u, part);
+            else w.u = -1;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(unit_empty + 8 * slot, slot_phase ^ 1, p.limit_ns))) {
+                if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+                break;
+            }
+            if (lane == 0) {
+                ring[slot] = w;
+                mbar_arrive(unit_full + 8 * slot);
+            }
+            __syncwarp();
+            if (++slot == C::UNITS) {
+                slot = 0;
+                slot_phase ^= 1;
+            }
+            if (!more) break;
+        }
+    } else if (warp == 3) {
+        if (!C::WGRAD) clear_rows(p, tab->row[p.E], lane, 32);
         if (p.table && blockIdx.x == 0)
-            for (int i = threadIdx.x - 64; i <= p.E; i += 64) {
+            for (int i = lane; i <= p.E; i += 32) {
                 p.table[i] = tab->row[i];
                 p.table[p.E + 1 + i] = tab->unit[i];
             }
@@ -300,8 +409,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         char* const stg = staging + (warp - 4) * 1024;
         int acc = 0, count = 0;  // accumulators used so far: the two groups of warps take them in turn
         uint32_t acc_phase = 0;
-        for (int u = first; u < units; u += step) {
-            const LinUnit w = lin_unit(p, tab->row, tab->unit, u);
+        while (take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
             const bool any = w.ke > w.kb;
             const bool mine = (count & 1) == turn;
             if (any) ++count;
@@ -322,15 +430,22 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             const uint32_t d = tmem + acc * C::BN + ((uint32_t)(q * 32) << 16);
             const int c0 = w.c0 + (int)rank * kLinTileM + q * 32;  // of this warp's 32 lanes
             const long long pitch = (long long)p.out_cols * 2;
-            if (p.partial && !(w.whole && p.fold == 1)) {
-                // a share of a tile: column quadruples of a lane side by side over the lanes
-                uint4* out = reinterpret_cast<uint4*>(p.partial) +
-                             ((long long)u * (C::PAIR ? 2 : 1) + rank) * (C::BN / 4) * kLinTileM + q * 32 + lane;
+            if ((C::WGRAD && p.partial && !(w.whole && p.fold == 1)) || shared_tile) {
+                // a share of a tile: column quadruples of a lane side by side over the lanes, in memory or, where the CTAs
+                // of a cluster add them, in the ring of stages (the tile is the CTA's only one: its loads have been used)
+                uint4* out = shared_tile ? reinterpret_cast<uint4*>(base)
+                                         : reinterpret_cast<uint4*>(p.partial) + ((long long)w.u * (C::PAIR ? 2 : 1) + rank) * (C::BN / 4) * kLinTileM;
+                out += q * 32 + lane;
 #pragma unroll 1
                 for (int n = 32 * odd; n < w.width; n += 64) {
                     uint32_t v[32];
-                    tmem_load_32(d + n, v);
-                    tmem_wait(v);
+                    if (any) {
+                        tmem_load_32(d + n, v);
+                        tmem_wait(v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0u;
+                    }
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
                         out[(long long)((n + i) / 4) * kLinTileM] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -443,77 +558,61 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     }
     tc_fence_before();
     __syncthreads();
-    if (C::PAIR) cluster_sync();
+    if (C::PAIR || shared_tile) cluster_sync();
     tc_fence_after();
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
+    if (!C::PAIR && shared_tile) {
+        w = ring[0];
+        if (w.u >= 0) {
+            if (p.splits == 2)
+                add_parts<C, 2>(p, w, part, smem_u32(base));
+            else if (p.splits == 4)
+                add_parts<C, 4>(p, w, part, smem_u32(base));
+            else
+                add_parts<C, 8>(p, w, part, smem_u32(base));
+        }
+        cluster_sync();  // the others may still read this CTA's part
+    }
 }
 
-// Adds the shares of the tiles that have several, and rounds once.  A CTA takes four columns of 256 / L rows of a tile; L
-// threads to a row add every L-th share each, and their sums are added in order: the same bits every call.
-template <bool I8, int L>
-__global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__ LinParams p, int BN) {
+// Weight gradient: adds the shares of the tiles that have several, and rounds once.  A CTA takes four columns of 256 / L
+// rows of a tile; L threads to a row add every L-th share each, and their sums are added in order: the same bits every call.
+template <int L>
+__global__ __launch_bounds__(256) void linear_sum_kernel(const __grid_constant__ LinParams p) {
     constexpr int R = 256 / L;  // rows at a time
     __shared__ uint4 s[L][R];
     const int r = threadIdx.x % R, l = threadIdx.x / R;
-    const int quads = BN / 4, blocks = p.tile_m / R * quads;  // of a tile
+    const int quads = p.bn / 4, blocks = p.tile_m / R * quads;  // of a tile
+    const int tiles = p.m_tiles * p.n_tiles;                    // of a group
     const int* row = p.table;
     const int* unit = p.table + p.E + 1;
     grid_dependency_wait();
     grid_launch_dependents();
-    for (int i = blockIdx.x;; i += gridDim.x) {
-        int t = i / blocks, g = 0, shares = 0, tiles = 0;  // the tile, counted over the groups
-        for (; g < p.E; ++g) {
-            const int rows = row[g + 1] - row[g];
-            tiles = lin_group_tiles(p, rows);
-            shares = lin_shares(p, rows);
-            if (t < tiles) break;
-            t -= tiles;
-        }
-        if (g == p.E) return;
+    for (int i = blockIdx.x; i < p.E * tiles * blocks; i += gridDim.x) {
+        const int t = i / blocks, part = i - t * blocks, g = t / tiles;
+        const int shares = lin_shares(p, row[g + 1] - row[g]);
         if (shares == 1) continue;
-        const int u = unit[g] + t;
+        const int u = unit[g] + t - g * tiles;
         const LinUnit w = lin_unit(p, row, unit, u);
-        const int part = i % blocks, n = part % quads * 4, m = part / quads * R + r;  // of the tile
-        if (n >= (p.wgrad ? p.out_cols - w.t0 : w.rows)) continue;
+        const int n = part % quads * 4, m = part / quads * R + r;  // of the tile
+        if (w.t0 + n >= p.out_cols) continue;
         const long long halves = p.tile_m / kLinTileM, step = tiles * halves * quads * kLinTileM;
         const uint4* src = reinterpret_cast<const uint4*>(p.partial) +
                            ((u * halves + m / kLinTileM) * quads + n / 4) * kLinTileM + m % kLinTileM;
         uint4 sum = make_uint4(0, 0, 0, 0);
-        auto add = [&](const uint4& v) {
-            if (I8) {
-                sum.x += v.x;
-                sum.y += v.y;
-                sum.z += v.z;
-                sum.w += v.w;
-            } else {
-                sum.x = __float_as_uint(__uint_as_float(sum.x) + __uint_as_float(v.x));
-                sum.y = __float_as_uint(__uint_as_float(sum.y) + __uint_as_float(v.y));
-                sum.z = __float_as_uint(__uint_as_float(sum.z) + __uint_as_float(v.z));
-                sum.w = __float_as_uint(__uint_as_float(sum.w) + __uint_as_float(v.w));
-            }
-        };
 #pragma unroll 8
-        for (int k = l; k < shares; k += L) add(__ldcg(src + k * step));
+        for (int k = l; k < shares; k += L) add_share<false>(sum, __ldcg(src + k * step));
         __syncthreads();
         s[l][r] = sum;
         __syncthreads();
-        if (l != 0 || w.c0 + m >= (p.wgrad ? p.out_rows : p.out_cols)) continue;
+        if (l != 0 || w.c0 + m >= p.out_rows) continue;
 #pragma unroll
-        for (int k = 1; k < L; ++k) add(s[k][r]);
+        for (int k = 1; k < L; ++k) add_share<false>(sum, s[k][r]);
         const uint32_t v[4] = {sum.x, sum.y, sum.z, sum.w};
-        uint16_t* out = reinterpret_cast<uint16_t*>(p.out);
-        const float cs = I8 ? __ldg(p.col_scale + (long long)w.g * p.out_cols + w.c0 + m) : 1.f;
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + ((long long)g * p.out_rows + w.c0 + m) * p.out_cols + w.t0 + n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f = __uint_as_float(v[j]);
-            if (p.wgrad) {
-                if (w.t0 + n + j < p.out_cols)
-                    out[((long long)w.g * p.out_rows + w.c0 + m) * p.out_cols + w.t0 + n + j] = (uint16_t)pack2(f, 0.f, p.out_bf16);
-            } else if (n + j < w.rows) {
-                if (I8) f = (float)(int)v[j] * __ldg(p.row_scale + w.t0 + n + j) * cs;
-                out[(long long)(w.t0 + n + j) * p.out_cols + w.c0 + m] = (uint16_t)pack2(f, 0.f, p.out_bf16);
-            }
-        }
+        for (int j = 0; j < 4; ++j)
+            if (w.t0 + n + j < p.out_cols) out[j] = (uint16_t)pack2(__uint_as_float(v[j]), 0.f, p.out_bf16);
     }
 }
 
@@ -562,17 +661,21 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const __grid_constant_
 }
 
 // Copies rows whose pitch or base TMA cannot address to rows of a 16-byte pitch; what lies between the columns and
-// the pitch is never read (the tensor maps end at the columns).
+// the pitch is never read (the tensor maps end at the columns).  The first `split` CTAs take the first operand.
+struct PackRows {
+    const void* src;
+    void* dst;
+    long long rows, src_stride, dst_stride;  // in elements
+    int cols;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, T* __restrict__ dst, long long rows, int cols,
-                                                        long long src_stride, int dst_stride) {
+__device__ __forceinline__ void pack_rows(const PackRows& a, long long cta, long long ctas) {
     constexpr int V = 16 / sizeof(T);
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const int per_row = (cols + V - 1) / V;
-    const long long n = rows * per_row;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long r = i / per_row;
+    const T* src = reinterpret_cast<const T*>(a.src);
+    const int per_row = (a.cols + V - 1) / V;
+    const long long n = a.rows * per_row;
+    for (long long i = cta * 256 + threadIdx.x; i < n; i += ctas * 256) {
+        const long long r = n <= INT_MAX ? (unsigned)i / (unsigned)per_row : i / per_row;
         const int c = (int)(i - r * per_row) * V;
         union {
             uint4 u;
@@ -581,9 +684,18 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ sr
         v.u = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (c + j < cols) v.t[j] = src[r * src_stride + c + j];
-        *reinterpret_cast<uint4*>(dst + r * dst_stride + c) = v.u;
+            if (c + j < a.cols) v.t[j] = src[r * a.src_stride + c + j];
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + r * a.dst_stride + c) = v.u;
     }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const __grid_constant__ PackRows a, const __grid_constant__ PackRows b, int split) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if ((int)blockIdx.x < split)
+        pack_rows<T>(a, blockIdx.x, split);
+    else
+        pack_rows<T>(b, blockIdx.x - split, gridDim.x - split);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -596,19 +708,20 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     int sms = 0, occ = 0;
     int rc = setup.get((const void*)linear_kernel<C>, C::THREADS, C::SMEM, &sms, &occ);
     if (rc) return rc;
-    const int slots = C::PAIR ? sms / 2 : sms;
-    const int grid = (pl.max_units < slots ? (pl.max_units > 0 ? (int)pl.max_units : 1) : slots) * (C::PAIR ? 2 : 1);
-    KDW_CUDA(launch_overlapping_previous_grid(linear_kernel<C>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, st,
-                                              C::PAIR ? 2 : 1, ma, mb, p));
+    const int cluster = C::PAIR ? 2 : p.splits;
+    const int64_t slots = C::PAIR ? sms / 2 : p.splits > 1 ? INT_MAX : sms;  // shared tiles: a cluster to each, in waves
+    const int64_t grid = std::max<int64_t>(1, std::min(pl.max_units, slots)) * cluster;
+    KDW_CUDA(launch_overlapping_previous_grid(linear_kernel<C>, dim3((unsigned)grid), dim3(C::THREADS), (size_t)C::SMEM, st, cluster,
+                                              ma, mb, p));
     if (p.fold > 1) {
         const int N = pl.out_rows / p.fold, K = pl.out_cols / p.fold;
         const int quads = N * (K / 4);
-        KDW_CUDA(launch_overlapping_previous(linear_fold_kernel, (unsigned)(quads < 8 * sms ? quads : 8 * sms), 256u, st, p, C::BN, N, K));
+        KDW_CUDA(launch_overlapping_previous(linear_fold_kernel, (unsigned)std::min(quads, 8 * sms), 256u, st, p, C::BN, N, K));
     } else if (p.partial) {
         const bool many = pl.max_units >= 8 * pl.max_tiles;
-        const long long blocks = pl.max_tiles * (C::BN / 4) * (p.tile_m / (many ? 32 : 128));
-        KDW_CUDA(launch_overlapping_previous(many ? linear_sum_kernel<C::I8, 8> : linear_sum_kernel<C::I8, 2>,
-                                             (unsigned)(blocks < 8 * sms ? blocks : 8 * sms), 256u, st, p, C::BN));
+        const int64_t blocks = pl.max_tiles * (C::BN / 4) * (p.tile_m / (many ? 32 : 128));
+        KDW_CUDA(launch_overlapping_previous(many ? linear_sum_kernel<8> : linear_sum_kernel<2>,
+                                             (unsigned)std::min<int64_t>(blocks, 8 * sms), 256u, st, p));
     }
     return 0;
 }
@@ -624,41 +737,32 @@ static int launch_width(const LinPlan& pl, const CUtensorMap& ma, const CUtensor
     }
 }
 
-template <typename T>
-static int pack_rows(const void* src, void* dst, int64_t rows, int64_t cols, int64_t src_stride, int64_t dst_stride,
-                     cudaStream_t st) {
-    const int64_t pieces = rows * ((cols * (int64_t)sizeof(T) + 15) / 16);
-    int sms = 0;
-    int rc = device_sm_count(&sms);
-    if (rc) return rc;
-    const int64_t want = (pieces + 255) / 256;
-    KDW_CUDA(launch_overlapping_previous(pack_rows_kernel<T>, (unsigned)(want < 8 * sms ? want : 8 * sms), 256u, st,
-                                         (const T*)src, (T*)dst, (long long)rows, (int)cols, (long long)src_stride,
-                                         (int)dst_stride));
-    return 0;
-}
-
 int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     int* status = nullptr;
-    int rc = status_ptr(&status);
+    int sms = 0, rc = device_facts(&status, &sms);
     if (rc) return rc;
     char* w = (char*)ws;
     const void* pa = a.a;
     const void* pb = a.b;
     int64_t sa = a.a_stride * pl.fold, sb = a.b_stride * pl.fold;
-    if (pl.pack_a) {
-        pa = w + pl.off_a;
-        rc = pl.esize == 2 ? pack_rows<uint16_t>(a.a, w + pl.off_a, pl.a_rows, pl.a_cols, a.a_stride, pl.a_pitch, st)
-                           : pack_rows<uint8_t>(a.a, w + pl.off_a, pl.a_rows, pl.a_cols, a.a_stride, pl.a_pitch, st);
-        if (rc) return rc;
-        sa = pl.a_pitch;
-    }
-    if (pl.pack_b) {
-        pb = w + pl.off_b;
-        rc = pl.esize == 2 ? pack_rows<uint16_t>(a.b, w + pl.off_b, pl.b_rows, pl.b_cols, a.b_stride, pl.b_pitch, st)
-                           : pack_rows<uint8_t>(a.b, w + pl.off_b, pl.b_rows, pl.b_cols, a.b_stride, pl.b_pitch, st);
-        if (rc) return rc;
-        sb = pl.b_pitch;
+    if (pl.pack_a || pl.pack_b) {
+        PackRows ra = {pa, w + pl.off_a, pl.pack_a ? pl.a_rows : 0, sa, pl.a_pitch, (int)pl.a_cols};
+        PackRows rb = {pb, w + pl.off_b, pl.pack_b ? pl.b_rows : 0, sb, pl.b_pitch, (int)pl.b_cols};
+        auto ctas = [&](const PackRows& r) {
+            const int64_t want = (r.rows * ((r.cols * (int64_t)pl.esize + 15) / 16) + 255) / 256;
+            return (int)std::min<int64_t>(want, 8 * sms);
+        };
+        const int na = ctas(ra), nb = ctas(rb);
+        KDW_CUDA(launch_overlapping_previous(pl.esize == 2 ? pack_rows_kernel<uint16_t> : pack_rows_kernel<uint8_t>,
+                                             (unsigned)(na + nb), 256u, st, ra, rb, na));
+        if (pl.pack_a) {
+            pa = w + pl.off_a;
+            sa = pl.a_pitch;
+        }
+        if (pl.pack_b) {
+            pb = w + pl.off_b;
+            sb = pl.b_pitch;
+        }
     }
     LinParams p;
     memset(&p, 0, sizeof(p));

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(cons
                     uint32_t v = 0;
                     if (n < p.N && k < p.K && (C::KP > 8 || h == 0)) {
                         const uint16_t* w = p.w + (long long)n * p.w_n + (long long)k * p.w_k;
-                        v = w[0] | (uint32_t)w[p.w_k] << 16;
+                        v = p.w_k == 1 ? *reinterpret_cast<const uint32_t*>(w) : w[0] | (uint32_t)w[p.w_k] << 16;
                     }
                     b[g][j][s][h] = v;
                 }

@@ -31,6 +31,9 @@ struct LinPlan {
     int64_t max_tiles, max_units;                              // over all row distributions
 };
 
+// The library's status word on the current device and its SMs, looked up once per device.
+int device_facts(int** status, int* sms);
+
 int linear_plan(LinPlan* pl, const LinArgs& a, int sms);
 int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st);
 

@@ -75,7 +75,7 @@ template <int TPR, int KEEP>
 static int quant_launch(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride,
                         int bf16, bool vec, bool qvec, cudaStream_t st) {
     int sms = 0;
-    int rc = device_sm_count(&sms);
+    int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
     const int64_t blocks = (rows + 256 / TPR - 1) / (256 / TPR);
     const unsigned grid = (unsigned)(blocks < 8 * sms ? blocks : 8 * sms);
@@ -92,7 +92,7 @@ int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols,
     // a last piece may run into the padding of its row, but not into the next row
     const bool qvec = ((uintptr_t)q & 7) == 0 && q_stride % 8 == 0 && (cols % 8 == 0 || q_padded);
     int sms = 0;
-    int rc = device_sm_count(&sms);
+    int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
     // A warp to a row needs no barrier; with few rows, or rows that a warp cannot keep, the CTA takes a row together.
     // 8192 x 4096 bf16: 18 us with a warp to a row, 33 us with the CTA (0.85 and 0.46 of the measured bandwidth).

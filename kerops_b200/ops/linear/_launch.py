@@ -12,18 +12,22 @@ INT8 = 2  # KDW_I8
 FWD, DGRAD, WGRAD = 0, 1, 2
 MAX_GROUPS = 1024
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index; torch.cuda.current_stream costs 2 us more
+# of a device index, and the current one: torch.cuda.current_stream and torch.cuda.device cost 3 us more, a quarter of a
+# small call
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def as_rows(t, name):
     """The [rows, channels] matrix of `t`: `t` itself, or the voxels of a channels_last_3d (N, C, H, W, D) volume."""
-    if t.ndim == 5:
-        assert t.is_contiguous(memory_format=torch.channels_last_3d), f'{name}: channels_last_3d volume expected'
-        return t.permute(0, 2, 3, 4, 1).reshape(-1, t.shape[1])
-    assert t.ndim == 2, f'{name}: [rows, channels] matrix or (N, C, H, W, D) volume expected'
-    assert t.stride(1) == 1 or t.shape[1] == 1, f'{name}: the channels of a row must be contiguous'
-    assert t.stride(0) >= t.shape[1] or t.shape[0] <= 1, f'{name}: rows must not overlap'
-    return t
+    if t.ndim == 2:
+        if not t.is_contiguous():
+            assert t.stride(1) == 1 or t.shape[1] == 1, f'{name}: the channels of a row must be contiguous'
+            assert t.stride(0) >= t.shape[1] or t.shape[0] <= 1, f'{name}: rows must not overlap'
+        return t
+    assert t.ndim == 5, f'{name}: [rows, channels] matrix or (N, C, H, W, D) volume expected'
+    assert t.is_contiguous(memory_format=torch.channels_last_3d), f'{name}: channels_last_3d volume expected'
+    return t.permute(0, 2, 3, 4, 1).reshape(-1, t.shape[1])
 
 
 def like_rows(rows, t):
@@ -38,13 +42,13 @@ def row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def check_ends(ends, groups, device):
+def check_ends(ends, groups, rows):
     if ends is None:
         assert groups == 1, 'ends is needed with more than one group'
         return
     assert ends.dtype == torch.int32 and ends.ndim == 1 and ends.is_contiguous(), 'ends: contiguous int32 vector expected'
     assert ends.shape[0] == groups, 'ends: one cumulative row count per group expected'
-    assert ends.device == device, 'ends must be on the device of the rows'
+    assert ends.get_device() == rows.get_device(), 'ends must be on the device of the rows'
 
 
 # The workspace depends on sizes and on the operands' alignment to 16 bytes alone; asking the library costs more than the
@@ -67,18 +71,19 @@ def _int8_workspace(device, x_align, w_align, T, E, K, N, sx, x_type, dtype):
 
 def product(op, a, b, out, ends, T, E, K, N):
     """Enqueues one product (FWD | DGRAD | WGRAD) of 16-bit operands on a's device / current stream."""
-    lib = _lib.load()
     device = a.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return product(op, a, b, out, ends, T, E, K, N)
     dtype = TYPES[a.dtype]
     sa, sb = row_stride(a), row_stride(b) if op == WGRAD else K
     pa, pb = a.data_ptr(), b.data_ptr()
-    with _on(device):
-        nbytes = _product_workspace(device.index, op, pa & 15, pb & 15, T, E, K, N, sa, sb, dtype)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        rc = lib.kdw_linear_f16(
-            op, pa, pb, out.data_ptr(), None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None,
-            nbytes, T, E, K, N, sa, sb, dtype, _raw_stream(device.index),
-        )
+    nbytes = _product_workspace(device.index, op, pa & 15, pb & 15, T, E, K, N, sa, sb, dtype)
+    ws = a.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = _lib.load().kdw_linear_f16(
+        op, pa, pb, out.data_ptr(), None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+        T, E, K, N, sa, sb, dtype, _raw_stream(device.index),
+    )
     if rc:
         _lib.check(rc)
     return out
@@ -86,18 +91,19 @@ def product(op, a, b, out, ends, T, E, K, N):
 
 def int8_product(x, x_scale, weight, w_scale, y, ends, T, E, K, N):
     """Enqueues y = Int8Linear(x); x is int8 with x_scale, or 16-bit (x_scale None)."""
-    lib = _lib.load()
     device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return int8_product(x, x_scale, weight, w_scale, y, ends, T, E, K, N)
     x_type, dtype, sx = TYPES.get(x.dtype, INT8), TYPES[y.dtype], row_stride(x)
     px, pw = x.data_ptr(), weight.data_ptr()
-    with _on(device):
-        nbytes = _int8_workspace(device.index, px & 15, pw & 15, T, E, K, N, sx, x_type, dtype)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        rc = lib.kdw_linear_i8(
-            px, None if x_scale is None else x_scale.data_ptr(), pw, w_scale.data_ptr(), y.data_ptr(),
-            None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx, x_type,
-            dtype, _raw_stream(device.index),
-        )
+    nbytes = _int8_workspace(device.index, px & 15, pw & 15, T, E, K, N, sx, x_type, dtype)
+    ws = y.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = _lib.load().kdw_linear_i8(
+        px, None if x_scale is None else x_scale.data_ptr(), pw, w_scale.data_ptr(), y.data_ptr(),
+        None if ends is None else ends.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx, x_type,
+        dtype, _raw_stream(device.index),
+    )
     if rc:
         _lib.check(rc)
     return y

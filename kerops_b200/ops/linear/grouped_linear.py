@@ -15,9 +15,9 @@ def _weight_dims(weight):
 
 def _check(a, b, groups, ends):
     assert a.dtype == b.dtype and a.dtype in _launch.TYPES, 'both operands fp16 or both bf16 expected'
-    assert a.is_cuda and b.device == a.device, 'the operands must be CUDA tensors on one device'
+    assert a.is_cuda and a.get_device() == b.get_device(), 'the operands must be CUDA tensors on one device'
     assert 1 <= groups <= _launch.MAX_GROUPS, f'1 to {_launch.MAX_GROUPS} groups'
-    _launch.check_ends(ends, groups, a.device)
+    _launch.check_ends(ends, groups, a)
 
 
 def GroupedLinear(x, weight, ends=None):
@@ -35,7 +35,7 @@ def GroupedLinear(x, weight, ends=None):
     _check(rows, weight, E, ends)
     T = rows.shape[0]
     assert rows.shape[1] == K and N >= 1 and K >= 1, 'x and weight disagree about the input channels'
-    y = torch.empty(T, N, dtype=x.dtype, device=x.device)
+    y = x.new_empty((T, N))
     if T:
         _launch.product(_launch.FWD, rows, weight, y, ends, T, E, K, N)
     return _launch.like_rows(y, x)
@@ -51,7 +51,7 @@ def GroupedLinearDGRAD(grad, weight, ends=None):
     _check(rows, weight, E, ends)
     T = rows.shape[0]
     assert rows.shape[1] == N and N >= 1 and K >= 1, 'grad and weight disagree about the output channels'
-    dx = torch.empty(T, K, dtype=grad.dtype, device=grad.device)
+    dx = grad.new_empty((T, K))
     if T:
         _launch.product(_launch.DGRAD, rows, weight, dx, ends, T, E, K, N)
     return _launch.like_rows(dx, grad)
@@ -72,7 +72,7 @@ def GroupedLinearWGRAD(x, grad, ends=None):
     if x.ndim == 5 or grad.ndim == 5:
         assert x.ndim == grad.ndim and x.shape[2:] == grad.shape[2:] and x.shape[0] == grad.shape[0], \
             'x and grad disagree about the volume'
-    dw = torch.empty((N, K) if ends is None else (E, N, K), dtype=x.dtype, device=x.device)
+    dw = x.new_empty((N, K) if ends is None else (E, N, K))
     if T:
         _launch.product(_launch.WGRAD, gr, xr, dw, ends, T, E, K, N)
     else:

@@ -63,8 +63,8 @@ def Int8Linear(x, weight, w_scale, ends=None, *, x_scale=None, dtype=None):
     assert x.is_cuda and weight.device == x.device and w_scale.device == x.device, 'CUDA tensors on one device expected'
     assert rows.shape[1] == K and N >= 1 and 1 <= K <= MAX_K, 'x and weight disagree about the input channels'
     assert 1 <= E <= _launch.MAX_GROUPS, f'1 to {_launch.MAX_GROUPS} groups'
-    _launch.check_ends(ends, E, x.device)
-    y = torch.empty(T, N, dtype=dtype, device=x.device)
+    _launch.check_ends(ends, E, x)
+    y = x.new_empty((T, N), dtype=dtype)
     if T:
         _launch.int8_product(rows, x_scale, weight, w_scale, y, ends, T, E, K, N)
     return _launch.like_rows(y, x)
