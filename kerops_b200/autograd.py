@@ -8,7 +8,8 @@ on all three axes, so it runs on the forward kernel unchanged.
 import torch
 
 from .ops.conv import DWConv, DWConvWGRAD
-from .ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+from .ops.linear import GroupedLinear
+from .ops.linear.grouped_linear import grouped_linear_grads
 
 
 def DWConvDGRAD(grad, weight, *, ACCTYPE='float32'):
@@ -69,12 +70,8 @@ class GroupedLinearFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         x, weight, ends = ctx.saved_tensors
         # an expanded or transposed gradient (of a sum, say) has no rows of contiguous channels
-        grad_out = grad_out.contiguous(memory_format=torch.channels_last_3d if grad_out.ndim == 5 else torch.contiguous_format)
-        grad_x = GroupedLinearDGRAD(grad_out, weight, ends) if ctx.needs_input_grad[0] else None
-        grad_w = None
-        if ctx.needs_input_grad[1]:
-            grad_w = GroupedLinearWGRAD(x, grad_out, ends).view(weight.shape)
-        return grad_x, grad_w, None
+        grad_out = grad_out.contiguous(memory_format=torch.channels_last_3d if x.ndim == 5 else torch.contiguous_format)
+        return (*grouped_linear_grads(x, weight, grad_out, ends, ctx.needs_input_grad[:2]), None)
 
 
 def grouped_linear(x, weight, ends=None):

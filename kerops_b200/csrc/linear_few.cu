@@ -28,38 +28,63 @@ struct FewParams {
     int q_pitch;              // QUANT: bytes between the quantised rows in shared memory
 };
 
-// Bytes [at, at + 16) of a row of `len` bytes, zeros beyond it.  VEC: rows start on 16-byte boundaries and len is a multiple
-// of 16; otherwise the piece is put together from aligned words (of which each holds at least one byte of the row).
-template <bool VEC, bool STREAM>
-__device__ __forceinline__ uint4 load_piece(const char* row, int at, int len) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (VEC) {
-        if (at < len) {
-            if (STREAM)
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                             : "l"(row + at));
-            else
-                v = __ldg(reinterpret_cast<const uint4*>(row + at));
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_16(const char* p) {
+    uint4 v;
+    if (STREAM)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    else
+        v = __ldg(reinterpret_cast<const uint4*>(p));
+    return v;
+}
+
+// Bytes [at, at + 16) of a row of `len` bytes, zeros beyond it: issue() starts the loads, get() waits for them.  VEC: rows
+// start on 16-byte boundaries and len is a multiple of 16.  Otherwise the piece is shifted together from the two aligned
+// pieces that hold its bytes.  No piece without a byte of the row is read (in its place one that has some), and the loads
+// stand outside branches, so that all of a lane's are in flight at once.
+template <bool VEC>
+struct Piece {
+    uint4 v;
+    template <bool STREAM>
+    __device__ __forceinline__ void issue(const char* row, int at, int len) {
+        v = make_uint4(0, 0, 0, 0);
+        if (at < len) v = load_16<STREAM>(row + at);
+    }
+    __device__ __forceinline__ uint4 get() const { return v; }
+};
+template <>
+struct Piece<false> {
+    uint4 v0, v1;
+    int lead, n;
+    template <bool STREAM>
+    __device__ __forceinline__ void issue(const char* row, int at, int len) {
+        n = len - at < 16 ? len - at : 16;
+        const uintptr_t p = (uintptr_t)(row + (n > 0 ? at : 0));
+        lead = (int)(p & 15);
+        const char* aligned = reinterpret_cast<const char*>(p - lead);
+        v0 = load_16<false>(aligned);
+        v1 = load_16<false>(lead + n > 16 ? aligned + 16 : aligned);
+    }
+    __device__ __forceinline__ uint4 get() const {
+        uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w}, o[4];
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = lead & 8 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = lead & 4 ? w[i + 1] : w[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int left = n - 4 * i;
+            const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (8 * (4 - left));
+            o[i] = __funnelshift_r(w[i], w[i + 1], (lead & 3) * 8) & keep;
         }
-        return v;
+        return make_uint4(o[0], o[1], o[2], o[3]);
     }
-    const int n = len - at < 16 ? len - at : 16;
-    if (n <= 0) return v;
-    const uintptr_t p = (uintptr_t)(row + at);
-    const int lead = (int)(p & 3);
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(p - lead);
-    const int count = (lead + n + 3) >> 2;
-    uint32_t w[5], o[4];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = i < count ? __ldg(words + i) : 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        o[i] = __funnelshift_r(w[i], w[i + 1], lead * 8);
-        const int left = n - 4 * i;
-        if (left < 4) o[i] = left <= 0 ? 0u : o[i] & (0xffffffffu >> (8 * (4 - left)));
-    }
-    return make_uint4(o[0], o[1], o[2], o[3]);
+};
+template <bool VEC>
+__device__ __forceinline__ uint4 load_piece(const char* row, int at, int len) {
+    Piece<VEC> p;
+    p.template issue<false>(row, at, len);
+    return p.get();
 }
 
 template <bool I8, bool BF16>
@@ -122,15 +147,16 @@ __device__ __forceinline__ void few_group(const FewParams& p, int slot, int lane
 }
 
 // NT: tiles of eight rows that share one pass over the weights.  QUANT: x holds 16-bit rows (NT == 1).
-template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U>
-__global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_constant__ FewParams p) {
+template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U, int CH>
+__global__ __launch_bounds__(32 * WARPS, 2) void linear_few_kernel(const __grid_constant__ FewParams p) {
     extern __shared__ __align__(16) char s_q[];
-    __shared__ uint32_t s_sum[WARPS][NT * 8][17];
+    constexpr int KW = WARPS * 16 / CH;  // warps along the contraction
+    __shared__ uint32_t s_sum[KW][NT * 8][CH + 1];
     __shared__ int s_group[4];
     __shared__ uint32_t s_max[8];
     __shared__ float s_scale[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = blockIdx.x * CH, kw = warp % KW, ch = warp / KW * 16;
     grid_dependency_wait();
     grid_launch_dependents();
     int g = 0, begin = 0, end = p.T, last = p.T;
@@ -152,29 +178,29 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
     }
     uint16_t* const y = reinterpret_cast<uint16_t*>(p.y);
     if (blockIdx.y == 0)
-        for (int i = threadIdx.x; i < (p.T - last) * 16; i += 32 * WARPS)
-            if (n0 + (i & 15) < p.N) y[(long long)(last + (i >> 4)) * p.N + n0 + (i & 15)] = 0;
+        for (int i = threadIdx.x; i < (p.T - last) * CH; i += 32 * WARPS)
+            if (n0 + i % CH < p.N) y[(long long)(last + i / CH) * p.N + n0 + i % CH] = 0;
     if (end <= begin) return;
 
     const char* wr[2];
     int wlen[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int n = n0 + gid + 8 * h;
+        const int n = n0 + ch + gid + 8 * h;
         wlen[h] = n < p.N ? p.len : 0;
         wr[h] = p.w + ((long long)g * p.N + (n < p.N ? n : 0)) * p.len;
     }
     const int pieces = (p.len + 63) >> 6;
 
     for (int t0 = begin; t0 < end; t0 += NT * 8) {
-        uint4 wv[U][2];
+        Piece<VEC> wp[U][2];
         auto load_weights = [&](int c) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) wv[u][h] = load_piece<VEC, true>(wr[h], (c + u * WARPS) * 64 + tig * 16, wlen[h]);
+                for (int h = 0; h < 2; ++h) wp[u][h].template issue<true>(wr[h], (c + u * KW) * 64 + tig * 16, wlen[h]);
         };
-        load_weights(warp);
+        load_weights(kw);
         if constexpr (QUANT) {
             // the rows of this tile, quantised into shared memory while the first weights are on their way
             const int rows = end - t0 < 8 ? end - t0 : 8;
@@ -185,7 +211,7 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
                 const char* row = p.x + (t0 + r) * p.x_pitch;
                 uint32_t m = 0;
                 for (int i = threadIdx.x; i < vecs; i += 32 * WARPS)
-                    m = max_bits(load_piece<VEC, false>(row, i * 16, 2 * p.len), m);
+                    m = max_bits(load_piece<VEC>(row, i * 16, 2 * p.len), m);
                 m = __reduce_max_sync(0xffffffffu, m);
                 if (lane == 0 && m) atomicMax(&s_max[r], m);
             }
@@ -196,7 +222,7 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
                 if (threadIdx.x == 0) s_scale[r] = q.scale;
                 for (int i = threadIdx.x; i < p.q_pitch / 8; i += 32 * WARPS) {
                     uint2 o = make_uint2(0, 0);
-                    if (i < vecs) o = quant8(load_piece<VEC, false>(row, i * 16, 2 * p.len), q, p.x_bf16);
+                    if (i < vecs) o = quant8(load_piece<VEC>(row, i * 16, 2 * p.len), q, p.x_bf16);
                     *reinterpret_cast<uint2*>(s_q + r * p.q_pitch + i * 8) = o;
                 }
             }
@@ -215,45 +241,48 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
             xlen[j] = t < end ? p.len : 0;
             xr[j] = QUANT ? s_q + gid * p.q_pitch : p.x + (t < end ? t : t0) * p.x_pitch;
         }
-        for (int c = warp; c < pieces; c += U * WARPS) {
-            if (c != warp) load_weights(c);
-            uint4 xv[U][NT];
+        for (int c = kw; c < pieces; c += U * KW) {
+            if (c != kw) load_weights(c);
+            Piece<VEC || QUANT> xp[U][NT];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const int at = (c + u * WARPS) * 64 + tig * 16;
+                    const int at = (c + u * KW) * 64 + tig * 16;
                     if constexpr (QUANT)
-                        xv[u][j] = at < xlen[j] ? *reinterpret_cast<const uint4*>(xr[j] + at) : make_uint4(0, 0, 0, 0);
+                        xp[u][j].v = at < xlen[j] ? *reinterpret_cast<const uint4*>(xr[j] + at) : make_uint4(0, 0, 0, 0);
                     else
-                        xv[u][j] = load_piece<VEC, false>(xr[j], at, xlen[j]);
+                        xp[u][j].template issue<false>(xr[j], at, xlen[j]);
                 }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const uint4 w0 = wp[u][0].get(), w1 = wp[u][1].get();
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    few_mma<I8, BF16>(acc[j], wv[u][0].x, wv[u][1].x, wv[u][0].y, wv[u][1].y, xv[u][j].x, xv[u][j].y);
-                    few_mma<I8, BF16>(acc[j], wv[u][0].z, wv[u][1].z, wv[u][0].w, wv[u][1].w, xv[u][j].z, xv[u][j].w);
+                    const uint4 x = xp[u][j].get();
+                    few_mma<I8, BF16>(acc[j], w0.x, w1.x, w0.y, w1.y, x.x, x.y);
+                    few_mma<I8, BF16>(acc[j], w0.z, w1.z, w0.w, w1.w, x.z, x.w);
                 }
+            }
         }
         if (t0 != begin) __syncthreads();
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s_sum[warp][j * 8 + tig * 2 + (i & 1)][gid + 8 * (i >> 1)] = acc[j][i];
+            for (int i = 0; i < 4; ++i) s_sum[kw][j * 8 + tig * 2 + (i & 1)][ch + gid + 8 * (i >> 1)] = acc[j][i];
         __syncthreads();
-        for (int i = threadIdx.x; i < NT * 8 * 16; i += 32 * WARPS) {
-            const int r = i >> 4, c = i & 15, t = t0 + r, n = n0 + c;
+        for (int i = threadIdx.x; i < NT * 8 * CH; i += 32 * WARPS) {
+            const int r = i / CH, c = i % CH, t = t0 + r, n = n0 + c;
             if (t >= end || n >= p.N) continue;
             float v = 0.f;
             if constexpr (I8) {
                 int s = 0;
 #pragma unroll
-                for (int k = 0; k < WARPS; ++k) s += (int)s_sum[k][r][c];
+                for (int k = 0; k < KW; ++k) s += (int)s_sum[k][r][c];
                 v = (float)s * (QUANT ? s_scale[r] : __ldg(p.x_scale + t)) * __ldg(p.w_scale + (long long)g * p.N + n);
             } else {
 #pragma unroll
-                for (int k = 0; k < WARPS; ++k) v += __uint_as_float(s_sum[k][r][c]);
+                for (int k = 0; k < KW; ++k) v += __uint_as_float(s_sum[k][r][c]);
             }
             y[(long long)t * p.N + n] = (uint16_t)pack2(v, 0.f, p.y_bf16);
         }
@@ -261,31 +290,32 @@ __global__ __launch_bounds__(32 * WARPS) void linear_few_kernel(const __grid_con
     }
 }
 
-template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U>
-static int few_warps(const FewParams& p, dim3 grid, cudaStream_t st) {
+template <bool I8, bool BF16, bool QUANT, int NT, bool VEC, int WARPS, int U, int CH>
+static int few_warps(const FewParams& p, cudaStream_t st) {
+    const dim3 grid((unsigned)((p.N + CH - 1) / CH), (unsigned)(p.ends ? (p.E < p.T ? p.E : p.T) : 1));
     if (QUANT) {
         static KernelSetup setup;
         int sms = 0, occ = 0;
-        int rc = setup.get((const void*)linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U>, 32 * WARPS, 8 * kFewQuantPitch, &sms, &occ);
+        int rc = setup.get((const void*)linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U, CH>, 32 * WARPS, 8 * kFewQuantPitch, &sms, &occ);
         if (rc) return rc;
     }
-    KDW_CUDA(launch_overlapping_previous_grid(linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U>, grid, dim3(32 * WARPS),
+    KDW_CUDA(launch_overlapping_previous_grid(linear_few_kernel<I8, BF16, QUANT, NT, VEC, WARPS, U, CH>, grid, dim3(32 * WARPS),
                                               (size_t)(QUANT ? p.q_pitch * 8 : 0), st, 1, p));
     return 0;
 }
 template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
 static int few_launch(const FewParams& p, cudaStream_t st) {
-    const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)(p.ends ? (p.E < p.T ? p.E : p.T) : 1));
-    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four; rows
-    // that start anywhere need five loads and twenty operations to a piece: 27.6 us with four, 51 us with eight.
-    constexpr int U = (NT == 1 ? 8 : NT == 2 ? 4 : 2) / (VEC ? 1 : 2);
-    return few_warps<I8, BF16, QUANT, NT, VEC, 8, U>(p, grid, st);
+    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four.
+    constexpr int U = (NT == 1 ? 8 : 4) / (VEC ? 1 : 4);
+    const long long ctas = (long long)((p.N + 15) / 16) * (p.ends ? (p.E < p.T ? p.E : p.T) : 1);
+    // 32 channels to a CTA where CTAs of 16 would not all be resident at once (two to an SM): 8 rows of 8 groups, 2048 ->
+    // 1024, 9.1 us instead of 10.3; with fewer CTAs the contraction is better split further (4096 x 4096: 8.5 and 11.2 us).
+    if (ctas > 296) return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 32>(p, st);
+    return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 16>(p, st);
 }
 template <bool I8, bool BF16, bool VEC>
 static int few_rows(const FewParams& p, cudaStream_t st) {
-    if (p.T <= 8) return few_launch<I8, BF16, false, 1, VEC>(p, st);
-    if (p.T <= 16) return few_launch<I8, BF16, false, 2, VEC>(p, st);
-    return few_launch<I8, BF16, false, 4, VEC>(p, st);
+    return p.T <= 8 ? few_launch<I8, BF16, false, 1, VEC>(p, st) : few_launch<I8, BF16, false, 2, VEC>(p, st);
 }
 
 int linear_few(const LinArgs& a, int x_type, cudaStream_t st) {

@@ -20,7 +20,7 @@ struct NarrowParams {
     long long x_pitch;        // bytes
     long long T;
     int K, N;                 // contraction and output columns, multiples of 8
-    int w_n, w_k;             // elements between the weights of neighbouring output columns / contraction steps
+    int across;               // 1: the contraction runs along the rows of the weights
 };
 
 template <bool BF16>
@@ -73,6 +73,16 @@ __global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(cons
     const long long warp = ((long long)blockIdx.x * C::THREADS + threadIdx.x) >> 5, warps = (long long)gridDim.x * (C::THREADS / 32);
     grid_dependency_wait();
     grid_launch_dependents();
+    // The weights, through shared memory: read in order, then picked by every lane.  [w_rows][w_cols] in memory; 16 bytes
+    // between the rows keep the picks out of each other's banks.
+    __shared__ __align__(16) uint16_t s_w[C::KP * C::NP + 8 * (C::KP > C::NP ? C::KP : C::NP)];
+    const bool across = p.across;
+    const int w_rows = across ? p.K : p.N, pieces = (across ? p.N : p.K) >> 3, pitch = pieces * 8 + 8;
+    for (int i = threadIdx.x; i < w_rows * pieces; i += C::THREADS) {
+        const int r = i / pieces, c = i - r * pieces;
+        *reinterpret_cast<uint4*>(s_w + r * pitch + c * 8) = __ldg(reinterpret_cast<const uint4*>(p.w) + i);
+    }
+    __syncthreads();
     long long rows = p.T;
     if (p.ends) {
         const int e = __ldg(p.ends);
@@ -93,8 +103,10 @@ __global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(cons
                     const int k = C::KP >= 32 ? (s >> 1) * 32 + tig * 8 + (s & 1) * 4 + h * 2 : tig * C::KP / 4 + h * 2;
                     uint32_t v = 0;
                     if (n < p.N && k < p.K && (C::KP > 8 || h == 0)) {
-                        const uint16_t* w = p.w + (long long)n * p.w_n + (long long)k * p.w_k;
-                        v = p.w_k == 1 ? *reinterpret_cast<const uint32_t*>(w) : w[0] | (uint32_t)w[p.w_k] << 16;
+                        if (across)
+                            v = s_w[k * pitch + n] | (uint32_t)s_w[(k + 1) * pitch + n] << 16;
+                        else
+                            v = *reinterpret_cast<const uint32_t*>(s_w + n * pitch + k);
                     }
                     b[g][j][s][h] = v;
                 }
@@ -209,8 +221,7 @@ int linear_narrow(const LinArgs& a, cudaStream_t st) {
     p.T = a.T;
     p.K = (int)(fwd ? a.K : a.N);
     p.N = (int)(fwd ? a.N : a.K);
-    p.w_n = fwd ? (int)a.K : 1;
-    p.w_k = fwd ? 1 : (int)a.K;
+    p.across = !fwd;
     return a.in_bf16 ? narrow_rows<true>(p, st) : narrow_rows<false>(p, st);
 }
 

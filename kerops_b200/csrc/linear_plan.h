@@ -38,7 +38,7 @@ int linear_plan(LinPlan* pl, const LinArgs& a, int sms);
 int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st);
 
 // Products of few rows, without a workspace (linear_few.cu).  x_type: KDW_I8, or 16-bit rows to quantise within the kernel.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 16;
 constexpr int kFewQuantRows = 8, kFewQuantPitch = 128 * 96 + 64;  // rows and bytes of a row that a CTA quantises itself
 int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
 

@@ -78,3 +78,24 @@ def GroupedLinearWGRAD(x, grad, ends=None):
     else:
         dw.zero_()
     return dw
+
+
+def grouped_linear_grads(x, weight, grad, ends, wanted):
+    """(dx, dw) of a GroupedLinear(x, weight, ends) that has been checked when it ran, or None where `wanted` says so; grad
+    is a contiguous gradient of its result, dw has weight's shape."""
+    E, N, K = _weight_dims(weight)
+    xr, gr = _launch.as_rows(x, 'x'), _launch.as_rows(grad, 'grad')
+    T = xr.shape[0]
+    dx = dw = None
+    if wanted[0]:
+        dx = gr.new_empty((T, K))
+        if T:
+            _launch.product(_launch.DGRAD, gr, weight, dx, ends, T, E, K, N)
+        dx = _launch.like_rows(dx, x)
+    if wanted[1]:
+        dw = torch.empty_like(weight)
+        if T:
+            _launch.product(_launch.WGRAD, gr, xr, dw, ends, T, E, K, N)
+        else:
+            dw.zero_()
+    return dx, dw
