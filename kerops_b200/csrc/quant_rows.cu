@@ -1,4 +1,6 @@
 // Quantises rows of 16-bit values (the arithmetic: quant_core.cuh).  Bound by memory: 2 bytes read and 1 written per value.
+#include <type_traits>
+
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
@@ -17,12 +19,12 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int c, int cols) {
 
 // TPR threads to a row (a warp or the CTA), KEEP vectors of 8 values of a thread stay in registers between the two passes
 // over the row; what is longer is read again.  VEC: rows of the input are 16-byte aligned, QVEC: rows of the output 8-byte.
-template <int TPR, int KEEP, bool VEC, bool QVEC>
-__global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restrict__ x, int8_t* __restrict__ q,
+template <int TPR, int KEEP, bool VEC, bool QVEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __restrict__ x, int8_t* __restrict__ q,
                                                          float* __restrict__ scale, long long rows, int cols,
                                                          long long x_stride, long long q_stride, int bf16) {
     __shared__ uint32_t s_max[8];
-    constexpr int RPB = 256 / TPR;
+    constexpr int RPB = THREADS / TPR;
     const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
     grid_dependency_wait();
     grid_launch_dependents();
@@ -45,7 +47,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
             __syncthreads();
             if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
             __syncthreads();
-            for (int i = 0; i < 8; ++i) m = s_max[i] > m ? s_max[i] : m;
+            for (int i = 0; i < THREADS / 32; ++i) m = s_max[i] > m ? s_max[i] : m;
         }
         if (!live) continue;
         const QuantRow qr = quant_row(m, bf16);
@@ -71,17 +73,17 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
     }
 }
 
-template <int TPR, int KEEP>
+template <int TPR, int KEEP, int THREADS>
 static int quant_launch(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride,
                         int bf16, bool vec, bool qvec, cudaStream_t st) {
     int sms = 0;
     int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
-    const int64_t blocks = (rows + 256 / TPR - 1) / (256 / TPR);
-    const unsigned grid = (unsigned)(blocks < 8 * sms ? blocks : 8 * sms);
-    auto* k = vec ? (qvec ? quant_rows_kernel<TPR, KEEP, true, true> : quant_rows_kernel<TPR, KEEP, true, false>)
-                  : (qvec ? quant_rows_kernel<TPR, KEEP, false, true> : quant_rows_kernel<TPR, KEEP, false, false>);
-    KDW_CUDA(launch_overlapping_previous(k, grid, 256u, st, (const uint16_t*)x, (int8_t*)q, scale, (long long)rows, (int)cols,
+    const int64_t blocks = (rows + THREADS / TPR - 1) / (THREADS / TPR);
+    const unsigned grid = (unsigned)(blocks < 2048 / THREADS * sms ? blocks : 2048 / THREADS * sms);
+    auto* k = vec ? (qvec ? quant_rows_kernel<TPR, KEEP, true, true, THREADS> : quant_rows_kernel<TPR, KEEP, true, false, THREADS>)
+                  : (qvec ? quant_rows_kernel<TPR, KEEP, false, true, THREADS> : quant_rows_kernel<TPR, KEEP, false, false, THREADS>);
+    KDW_CUDA(launch_overlapping_previous(k, grid, (unsigned)THREADS, st, (const uint16_t*)x, (int8_t*)q, scale, (long long)rows, (int)cols,
                                          (long long)x_stride, (long long)q_stride, bf16));
     return 0;
 }
@@ -94,13 +96,29 @@ int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols,
     int sms = 0;
     int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
-    // A warp to a row needs no barrier; with few rows, or rows that a warp cannot keep, the CTA takes a row together.
-    // 8192 x 4096 bf16: 18 us with a warp to a row, 33 us with the CTA (0.85 and 0.46 of the measured bandwidth).
-    if (rows < 8 * sms || cols > 4096)
-        return cols <= 2048 ? quant_launch<256, 1>(x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st)
-                            : quant_launch<256, 8>(x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st);
-    return cols <= 1024 ? quant_launch<32, 4>(x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st)
-                        : quant_launch<32, 16>(x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st);
+    auto go = [&](auto tpr, auto keep, auto threads) {
+        return quant_launch<decltype(tpr)::value, decltype(keep)::value, decltype(threads)::value>(
+            x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> k1;
+    const integral_constant<int, 2> k2;
+    const integral_constant<int, 4> k4;
+    const integral_constant<int, 8> k8;
+    const integral_constant<int, 16> k16;
+    const integral_constant<int, 32> warp;
+    const integral_constant<int, 128> cta;
+    const integral_constant<int, 256> wide;
+    // A warp to a row needs no barrier, and no more registers than the row fills; with few rows, or rows that a warp cannot
+    // keep, the CTA takes a row together.  bf16, us with a warp and with the CTA: 8192 x 4096 17.8 and 19.6 (0.86 and 0.79
+    // of the measured bandwidth), 8192 x 1024 5.2 and 9.9, 500 x 4096 3.0 and 2.5.
+    if (cols > 4096) return go(wide, k4, wide);
+    if (rows < 8 * sms) return cols <= 1024 ? go(cta, k1, cta) : go(cta, k4, cta);
+    if (cols <= 256) return go(warp, k1, cta);
+    if (cols <= 512) return go(warp, k2, cta);
+    if (cols <= 1024) return go(warp, k4, cta);
+    if (cols <= 2048) return go(warp, k8, cta);
+    return go(warp, k16, cta);
 }
 
 }  // namespace kdw

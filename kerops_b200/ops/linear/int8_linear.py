@@ -54,13 +54,13 @@ def Int8Linear(x, weight, w_scale, ends=None, *, x_scale=None, dtype=None):
         assert x_scale is not None and dtype is not None, 'int8 x needs x_scale and dtype'
         assert x_scale.dtype == torch.float32 and x_scale.shape == (T,) and x_scale.is_contiguous(), \
             'x_scale: contiguous fp32 scale per row expected'
-        assert x_scale.device == x.device
+        assert x_scale.get_device() == x.get_device(), 'x_scale must be on the device of x'
     else:
         assert x.dtype in _launch.TYPES, 'x: fp16, bf16 or int8 expected'
         assert x_scale is None, 'x_scale belongs to int8 x'
         dtype = x.dtype if dtype is None else dtype
     assert dtype in _launch.TYPES, 'dtype: torch.float16 or torch.bfloat16'
-    assert x.is_cuda and weight.device == x.device and w_scale.device == x.device, 'CUDA tensors on one device expected'
+    assert x.is_cuda and x.get_device() == weight.get_device() == w_scale.get_device(), 'CUDA tensors on one device expected'
     assert rows.shape[1] == K and N >= 1 and 1 <= K <= MAX_K, 'x and weight disagree about the input channels'
     assert 1 <= E <= _launch.MAX_GROUPS, f'1 to {_launch.MAX_GROUPS} groups'
     _launch.check_ends(ends, E, x)
