@@ -251,6 +251,14 @@ int kdw_fprop_bnrelu_f16(const void* x, const float* scale, const float* shift, 
 #define KDW_BF16 1
 #define KDW_I8 2
 
+/*
+ * The kernel that these sizes get on a device of `sms` SMs, dense aligned operands assumed (type KDW_F16, KDW_BF16, or KDW_I8
+ * with op KDW_LINEAR_FWD): 1 = few rows, 2 = narrow weights; otherwise parts * 1000000 + M * 1000 + N, M x N the tensor-core
+ * tile (256: a pair of CTAs) and `parts` who shares it: 1 nobody, 2 / 4 / 8 the CTAs of a cluster, 16 shares of the rows that
+ * are added in memory, 32 the same of folded rows.  No GPU needed.  Negative: an argument error.
+ */
+int kdw_linear_auto_variant(int op, int type, int64_t T, int64_t E, int64_t K, int64_t N, int sms);
+
 int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int64_t T, int64_t E, int64_t K, int64_t N,
                                        int64_t a_stride, int64_t b_stride, int dtype);
 int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_t* ends, void* workspace,

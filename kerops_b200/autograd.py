@@ -6,6 +6,7 @@ stride-1, pad-1 cross-correlation is the same cross-correlation of the upstream 
 on all three axes, so it runs on the forward kernel unchanged.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from .ops.conv import DWConv, DWConvWGRAD
 from .ops.linear import GroupedLinear
@@ -67,6 +68,7 @@ class GroupedLinearFunction(torch.autograd.Function):
         return GroupedLinear(x, weight, ends)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         x, weight, ends = ctx.saved_tensors
         # an expanded or transposed gradient (of a sum, say) has no rows of contiguous channels

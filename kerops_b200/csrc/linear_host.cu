@@ -1,6 +1,4 @@
 // C entry points of the channel-mixing products: argument checks, the plan and the workspace layout.
-#include <stdlib.h>
-
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -43,7 +41,7 @@ int device_facts(int** status, int* sms) {
     // tensor map needs.
     static thread_local int bound = -1;
     if (bound != dev) {
-        KDW_CUDA(cudaFree(nullptr));
+        KDW_CUDA(cudaSetDevice(dev));  // (allowed while a stream is being captured, unlike an allocation)
         bound = dev;
     }
     Facts& f = facts[dev];
@@ -106,8 +104,6 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
     };
     static const struct { int tile_m, bn; } shapes[] = {{256, 256}, {128, 256}, {128, 128}, {128, 64}};
     for (auto& c : shapes) {
-        const char* force = getenv("KDW_LINEAR_TILE");
-        if (force && atoi(force) != c.tile_m * 1000 + c.bn) continue;
         const bool pair = c.tile_m == 256;
         const int slots = pair ? sms / 2 : sms;
         const double m_tiles = (double)ceil_div(wgrad ? a.N : pl->out_cols, c.tile_m);
@@ -210,7 +206,7 @@ static int f16_args(LinArgs* a, int op, const void* pa, const void* pb, int64_t 
     return 0;
 }
 
-static bool is_few(const LinArgs& a) { return a.op == LIN_FWD && a.T <= kFewRows; }
+static bool is_few(const LinArgs& a) { return a.op == LIN_FWD && a.T <= kFewRows && a.K <= (1 << 28); }  // byte offsets in 32 bits
 
 // The 8-bit product: the rows are int8 with their scales, or 16-bit rows that are quantised into the workspace first.
 struct I8Layout {
@@ -277,6 +273,23 @@ static int plan_and_run(LinArgs* a, void* workspace, int64_t workspace_bytes, vo
 }  // namespace kdw
 
 extern "C" {
+
+int kdw_linear_auto_variant(int op, int type, int64_t T, int64_t E, int64_t K, int64_t N, int sms) {
+    using namespace kdw;
+    LinArgs args;
+    I8Layout l;
+    const void* aligned = (const void*)4096;
+    int rc = type == KDW_I8 ? i8_args(&args, &l, aligned, aligned, T, E, K, N, K, type, KDW_F16)
+                            : f16_args(&args, op, aligned, aligned, T, E, K, N, op == LIN_FWD ? K : N, K, type);
+    if (rc) return rc;
+    if (is_few(args)) return 1;
+    if (is_narrow(args)) return 2;
+    LinPlan pl;
+    rc = linear_plan(&pl, args, sms);
+    if (rc) return rc;
+    const int parts = pl.fold > 1 ? 32 : pl.off_partial >= 0 ? 16 : pl.splits;
+    return parts * 1000000 + pl.tile_m * 1000 + pl.bn;
+}
 
 int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int64_t T, int64_t E, int64_t K, int64_t N,
                                        int64_t a_stride, int64_t b_stride, int dtype) {

@@ -104,6 +104,28 @@ def test_folded_rows_do_not_mix():
     assert torch.equal(gdx[rows != 1000], dx[rows != 1000])
 
 
+@pytest.mark.parametrize('op,variant,T,E,K,N', [c for c in ref.VARIANTS if c[0] < 3])
+def test_every_variant(kdw_lib, op, variant, T, E, K, N):
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sms != 148 or kdw_lib.kdw_linear_auto_variant(op, 0, T, E, K, N, sms) == variant
+    x, g = ref.integers((T, K), torch.float16, 1, top=1), ref.integers((T, N), torch.float16, 2, top=1)
+    w = ref.integers((E, N, K), torch.float16, 3, top=1)
+    # the kernels that fold rows take one group of all rows
+    ends = [T] if variant // 1000000 == 32 else ref.uneven_ends(T, E)
+    e = None if variant // 1000000 == 32 else ref.tensor_ends(ends)
+    if op == 0:
+        assert torch.equal(GroupedLinear(x, w, e), ref.fwd(x, w, ends).half())
+    elif op == 1:
+        assert torch.equal(GroupedLinearDGRAD(g, w, e), ref.dgrad(g, w, ends).half())
+    else:
+        assert torch.equal(GroupedLinearWGRAD(x, g, e).view(E, N, K), ref.wgrad(x, g, ends).half())
+    from kerops_b200 import _lib
+
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_normal_values_within_the_rounding(dtype):
     from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
@@ -277,6 +299,28 @@ def test_capture_and_replay():
             assert torch.equal(dw, ref.wgrad(x, g, ends).half())
 
 
+def test_a_training_step_is_captured():
+    """Forward and backward in a graph, the first calls of this kind in the autograd thread among them."""
+    from kerops_b200.autograd import grouped_linear
+
+    T, K, N, ends = 400, 72, 40, [100, 390]
+    x, w = ref.integers((T, K), torch.float16, 1), ref.integers((2, N, K), torch.float16, 2)
+    g, e = ref.integers((T, N), torch.float16, 3), ref.tensor_ends(ends)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        xl, wl = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = grouped_linear(xl, wl, e)
+        dx, dw = torch.autograd.grad(y, (xl, wl), g)
+    for seed in (4, 5):
+        x.copy_(ref.integers((T, K), torch.float16, seed))
+        g.copy_(ref.integers((T, N), torch.float16, seed + 10))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref.fwd(x, w, ends).half())
+        assert torch.equal(dx, ref.dgrad(g, w, ends).half()) and torch.equal(dw, ref.wgrad(x, g, ends).half())
+
+
 @pytest.mark.parametrize('shape', ['matrix', 'volume'])
 def test_autograd_formula_and_differences(shape):
     from kerops_b200.autograd import ExpertLinear, grouped_linear
@@ -303,6 +347,9 @@ def test_autograd_formula_and_differences(shape):
         along_w = grouped_linear(x, w + dw, e).double() - y.double()
     assert (along_x * g.double()).sum() == (x.grad.double() * dx.double()).sum()
     assert (along_w * g.double()).sum() == (w.grad.double() * dw.double()).sum()
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        dx_, = torch.autograd.grad(grouped_linear(x, w, e), x, g.requires_grad_(True), create_graph=True)
+        dx_.sum().backward()
     # a gradient that is one value expanded, only one of the gradients wanted, and the module
     m = ExpertLinear(3, K, N, device='cuda')
     m(x.detach(), e).sum().backward()

@@ -106,6 +106,20 @@ def test_product_to_the_bit(T, K, N, ends, dtype):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize('op,variant,T,E,K,N', [c for c in ref.VARIANTS if c[0] == 3])
+def test_every_variant(kdw_lib, op, variant, T, E, K, N):
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import Int8Linear
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sms != 148 or kdw_lib.kdw_linear_auto_variant(0, 2, T, E, K, N, sms) == variant
+    x, xs, w, ws = _int8(T, K, N, E, T)
+    ends = ref.uneven_ends(T, E)
+    y = Int8Linear(x, w, ws, ref.tensor_ends(ends), x_scale=xs, dtype=torch.bfloat16)
+    assert torch.equal(y, _product(x, xs, w, ws, ends, torch.bfloat16))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('T,K,N,ends', [
     (1, 1, 1, None), (1, 4096, 512, None), (1, 1001, 333, None), (5, 2056, 72, None), (8, 64, 64, None), (33, 256, 100, None),

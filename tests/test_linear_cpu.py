@@ -98,3 +98,17 @@ def test_c_entry_points_refuse_bad_arguments(kdw_lib):
 def test_spans_are_clamped():
     assert ref.spans([2, 1, 9, 4], 5) == [(0, 2), (2, 2), (2, 5), (5, 5)]
     assert ref.spans([-3, 2], 5) == [(0, 0), (0, 2)]
+
+
+def test_the_listed_sizes_get_every_variant(kdw_lib):
+    """The sizes that the GPU tests run get the variants they are listed for, and no sizes get a variant that is not listed."""
+    auto = kdw_lib.kdw_linear_auto_variant
+    for op, variant, T, E, K, N in ref.VARIANTS:
+        assert auto(op % 3, 2 if op == 3 else 0, T, E, K, N, 148) == variant, (op, variant)
+    listed = {(op, v) for op, v, *_ in ref.VARIANTS}
+    g = torch.Generator().manual_seed(0)
+    for _ in range(4000):
+        T, K, N = (int(2 ** (float(torch.rand((), generator=g)) * b)) for b in (20, 13, 13))
+        E, op = int(torch.randint(1, 40, (), generator=g)), int(torch.randint(0, 4, (), generator=g))
+        assert (op, auto(op % 3, 2 if op == 3 else 0, T, E, K, N, 148)) in listed
+    assert auto(3, 0, 8, 1, 8, 8, 148) == auto(0, 3, 8, 1, 8, 8, 148) == auto(0, 0, 0, 1, 8, 8, 148) == -1
