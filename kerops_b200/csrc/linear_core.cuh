@@ -316,16 +316,16 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // The tensor-core instructions below are executed by a converged warp and issued by the lane whose `el` (elect_one) is
 // set: under a branch that only one lane takes, an issue costs some 45 cycles.
-// Arrives on `bar` (PAIR: on that barrier of both CTAs) when the tensor-core work issued so far by this thread has
-// finished.
+// Arrives on `bar` (PAIR: on that barrier of both CTAs, bits `both` of the cluster) when the tensor-core work issued so far
+// by this thread has finished.
 template <bool PAIR>
-__device__ __forceinline__ void tc_commit(uint32_t el, uint32_t bar) {
+__device__ __forceinline__ void tc_commit(uint32_t el, uint32_t bar, uint32_t both) {
     if constexpr (PAIR)
         asm volatile(
             "{\n\t.reg .pred e;\n\t"
             "setp.ne.b32 e, %2, 0;\n\t"
             "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
-            "h"((uint16_t)3), "r"(el)
+            "h"((uint16_t)both), "r"(el)
             : "memory");
     else
         asm volatile(

@@ -87,13 +87,14 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
     // Tile and parts: the smallest estimate of the cycles on the busiest SM.  A stage of 64 (128 bytes of) contraction
     // steps costs a CTA the larger of the products, 2 cycles a column, and shared memory, which writes and reads the stage
     // at 128 bytes a cycle: 256 cycles for the M side and 2 a column of the N side it loads (a pair: half of them).  A
-    // tile costs some 1500 cycles more that the next one does not hide, and 4000 to 10000 where two to eight CTAs of a
-    // cluster share it (500 x 1000 -> 1000: 2 us for four).
+    // tile costs some 1500 cycles more that the next one does not hide, a pair's 1200 on top, and 4000 to 10000 where two
+    // to eight parts of a cluster share it (measured at 64 x 4096 -> 4096 on 128 x 64 tiles: 15.8 us for 64 blocks on one
+    // CTA, 12.0 on two, 10.8 on four).
     // Shares of the weight gradient that are added in memory cost another kernel and their bytes, written and read.
     const int64_t groups = std::min(a.E, a.T);
     const double rows = (double)a.T / groups;  // of a group, about
-    const int cluster_slots[] = {0, sms, 0, 0, 132 * sms / 148, 0, 0, 0, 120 * sms / 148};  // CTAs in clusters that fit at once
-    double best = 1e300;
+    const int cluster_slots[] = {0, sms, sms, 0, 132 * sms / 148, 0, 0, 0, 120 * sms / 148};  // CTAs in clusters that fit at once
+    double best = 1e300;  // (a tile of one CTA without parts is always considered, or shares of folded rows)
     auto consider = [&](double cost, int tile_m, int bn, int splits, int64_t chunk) {
         if (cost >= best) return;
         best = cost;
@@ -113,10 +114,11 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
         const double block = std::max(2 * width, 256 + (pair ? 1 : 2) * (double)c.bn);
         const double blocks = wgrad ? std::ceil(rows / 64) : pl->k_blocks;
         if (pl->fold == 1) {
-            consider(std::ceil(tiles / slots) * (blocks * block + 1500), c.tile_m, c.bn, 1, INT32_MAX);
-            for (int splits = 2; splits <= 8 && !pair; splits *= 2)
-                if (blocks / splits >= 2 && tiles * splits <= (splits == 2 ? sms : cluster_slots[splits]))
-                    consider(std::ceil(blocks / splits) * block + 3500 + 1000 * splits, c.tile_m, c.bn, splits, INT32_MAX);
+            const double extra = pair ? 1200 : 0;
+            consider(std::ceil(tiles / slots) * (blocks * block + 1500) + extra, c.tile_m, c.bn, 1, INT32_MAX);
+            for (int splits = 2; splits <= (pair ? 4 : 8); splits *= 2)
+                if (blocks / splits >= 2 && tiles * splits * (pair ? 2 : 1) <= cluster_slots[splits * (pair ? 2 : 1)])
+                    consider(std::ceil(blocks / splits) * block + 3500 + 1000 * splits + extra, c.tile_m, c.bn, splits, INT32_MAX);
         }
         if (!wgrad || (pl->fold == 1 && (tiles > slots || rows < 1024))) continue;
         for (int waves = 1; waves <= 2; ++waves) {

@@ -144,11 +144,11 @@ __device__ __forceinline__ void add_share(uint4& sum, const uint4& v) {
     }
 }
 
-// The CTAs of a cluster add their parts of a tile: CTA `part` takes its share of the column quadruples, in the order of the
-// parts.
+// The CTAs of a cluster add their parts of a tile (of their 128 of its M): CTA `part` takes its share of the column
+// quadruples, in the order of the parts.
 template <class C, int PARTS>
-__device__ __forceinline__ void add_parts(const LinParams& p, const LinUnit& w, int part, uint32_t tile) {
-    const int m = threadIdx.x & 127, c = w.c0 + m;
+__device__ __forceinline__ void add_parts(const LinParams& p, const LinUnit& w, int part, uint32_t rank, uint32_t tile) {
+    const int m = threadIdx.x & 127, c = w.c0 + (int)rank * kLinTileM + m;
     const int cols = C::WGRAD ? (p.out_cols - w.t0 < C::BN ? p.out_cols - w.t0 : C::BN) : w.rows;
     const bool live = c < (C::WGRAD ? p.out_rows : p.out_cols);
     float cs = 1.f;
@@ -158,7 +158,7 @@ __device__ __forceinline__ void add_parts(const LinParams& p, const LinUnit& w, 
     const int quads = (cols + 3) >> 2, end = quads * (part + 1) / PARTS;
     uint32_t src[PARTS];
 #pragma unroll
-    for (int k = 0; k < PARTS; ++k) src[k] = cluster_addr(tile + m * 16, k);
+    for (int k = 0; k < PARTS; ++k) src[k] = cluster_addr(tile + m * 16, C::PAIR ? 2 * k + rank : k);
     for (int j = quads * part / PARTS + (threadIdx.x >> 7); j < end; j += C::THREADS / 128) {
         uint4 v[PARTS];
 #pragma unroll
@@ -220,10 +220,12 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                    acc_full = partly + 8 * C::STAGES, acc_empty = acc_full + 8 * C::ACCS, drain = acc_empty + 8 * C::ACCS,
                    unit_full = drain + 8, unit_empty = unit_full + 8 * C::UNITS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = C::PAIR ? cluster_rank() : 0;
-    // Few tiles: a cluster of CTAs takes one tile, a part of the contraction each, and adds the parts at the end.
-    const bool shared_tile = !C::PAIR && p.splits > 1;
-    const int part = shared_tile ? (int)cluster_rank() : 0;
+    // Few tiles: a cluster takes one tile, its CTAs (pairs) a part of the contraction each, and adds the parts at the end.
+    const bool shared_tile = p.splits > 1;
+    const uint32_t in_cluster = C::PAIR || shared_tile ? cluster_rank() : 0;
+    const uint32_t rank = C::PAIR ? in_cluster & 1 : 0, leader = in_cluster & ~1u, both = 3u << leader;  // of the pair
+    const int part = !shared_tile ? 0 : C::PAIR ? (int)(in_cluster >> 1) : (int)in_cluster;
+    const int ctas = (C::PAIR ? 2 : 1) * p.splits;  // that share a tile
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&map_a);
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
                         mbar_expect_tx(bar, l.bytes);
                     } else {
-                        bar = cluster_addr(bar, 0);  // CTA 0 waits for the loads of both
+                        bar = cluster_addr(bar, leader);  // CTA 0 waits for the loads of both
                         cluster_expect_tx(bar, l.bytes);
                     }
                     l.load(&map_a, &map_b, k, a, b, bar);
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                     __syncwarp();
                     if (rank != 0) {
                         partly_phase ^= 1u << stage;  // one parity bit per stage
-                        if (lane == 0) cluster_release_arrive(cluster_addr(full + 8 * stage, 0));
+                        if (lane == 0) cluster_release_arrive(cluster_addr(full + 8 * stage, leader));
                     }
                 }
                 if (rank == 0) {
@@ -354,8 +356,8 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                     for (int i = 0; i < 4; ++i)
                         tc_mma<C::I8, C::PAIR>(el, d, da + i * (C::A_ACROSS ? 2048 >> 4 : 32 >> 4),
                                                db + i * (C::B_ACROSS ? 2048 >> 4 : 32 >> 4), idesc, k > w.kb || i > 0);
-                    tc_commit<C::PAIR>(el, empty + 8 * stage);
-                    if (k + 1 == w.ke) tc_commit<C::PAIR>(el, acc_full + 8 * acc);
+                    tc_commit<C::PAIR>(el, empty + 8 * stage, both);
+                    if (k + 1 == w.ke) tc_commit<C::PAIR>(el, acc_full + 8 * acc, both);
                 }
                 if (++stage == C::STAGES) {
                     stage = 0;
@@ -370,14 +372,14 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         if (!ok && lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         // products in flight still read shared memory and write tensor memory
         if (rank == 0) {
-            tc_commit<C::PAIR>(elect_one(), drain);
+            tc_commit<C::PAIR>(elect_one(), drain, both);
             if (!lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         }
         __syncwarp();
     } else if (warp == 2) {
         const int units = tab->unit[p.E];
-        const int first = C::PAIR ? blockIdx.x >> 1 : shared_tile ? blockIdx.x / p.splits : blockIdx.x;
-        const int step = C::PAIR ? gridDim.x >> 1 : shared_tile ? units : gridDim.x;
+        const int first = blockIdx.x / ctas;
+        const int step = shared_tile ? units : gridDim.x / ctas;  // a shared tile is the cluster's only one
         for (int u = first;; u += step) {
             const bool more = u < units;
             if (more) w = lin_unit(p, tab->row, tab->unit, u, part);
@@ -545,7 +547,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 __syncwarp();
                 if (lane == 0) {
                     if (C::PAIR)
-                        cluster_arrive(cluster_addr(acc_empty + 8 * acc, 0));
+                        cluster_arrive(cluster_addr(acc_empty + 8 * acc, leader));
                     else
                         mbar_arrive(acc_empty + 8 * acc);
                 }
@@ -561,15 +563,15 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     if (C::PAIR || shared_tile) cluster_sync();
     tc_fence_after();
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
-    if (!C::PAIR && shared_tile) {
+    if (shared_tile) {
         w = ring[0];
         if (w.u >= 0) {
             if (p.splits == 2)
-                add_parts<C, 2>(p, w, part, smem_u32(base));
+                add_parts<C, 2>(p, w, part, rank, smem_u32(base));
             else if (p.splits == 4)
-                add_parts<C, 4>(p, w, part, smem_u32(base));
-            else
-                add_parts<C, 8>(p, w, part, smem_u32(base));
+                add_parts<C, 4>(p, w, part, rank, smem_u32(base));
+            else if constexpr (!C::PAIR)
+                add_parts<C, 8>(p, w, part, rank, smem_u32(base));
         }
         cluster_sync();  // the others may still read this CTA's part
     }
@@ -708,8 +710,8 @@ static int launch_product(const LinPlan& pl, const CUtensorMap& ma, const CUtens
     int sms = 0, occ = 0;
     int rc = setup.get((const void*)linear_kernel<C>, C::THREADS, C::SMEM, &sms, &occ);
     if (rc) return rc;
-    const int cluster = C::PAIR ? 2 : p.splits;
-    const int64_t slots = C::PAIR ? sms / 2 : p.splits > 1 ? INT_MAX : sms;  // shared tiles: a cluster to each, in waves
+    const int cluster = (C::PAIR ? 2 : 1) * p.splits;
+    const int64_t slots = p.splits > 1 ? INT_MAX : C::PAIR ? sms / 2 : sms;  // shared tiles: a cluster to each, in waves
     const int64_t grid = std::max<int64_t>(1, std::min(pl.max_units, slots)) * cluster;
     KDW_CUDA(launch_overlapping_previous_grid(linear_kernel<C>, dim3((unsigned)grid), dim3(C::THREADS), (size_t)C::SMEM, st, cluster,
                                               ma, mb, p));

@@ -51,42 +51,48 @@ VARIANTS = [
     (3, 1, 9, 3, 80, 40),
     (0, 2, 17, 1, 24, 24),
     (0, 1128064, 17, 2, 24, 24),
-    (0, 1128128, 33708, 32, 24, 24),
+    (0, 1128128, 8193, 32, 24, 24),
     (0, 1128256, 16961, 32, 24, 24),
-    (0, 1256256, 8193, 32, 24, 24),
+    (0, 1256256, 1061, 8, 24, 9880),
     (0, 2128064, 17, 3, 1368, 24),
     (0, 2128128, 4970, 1, 2128, 24),
     (0, 2128256, 9614, 3, 2040, 24),
+    (0, 2256256, 4325, 32, 1416, 168),
     (0, 4128064, 17, 1, 1528, 24),
     (0, 4128128, 2076, 2, 1968, 24),
     (0, 4128256, 4839, 1, 2032, 24),
+    (0, 4256256, 2485, 1, 2064, 144),
     (0, 8128064, 17, 2, 5536, 24),
     (0, 8128128, 561, 8, 8184, 24),
     (0, 8128256, 2140, 3, 8696, 24),
     (1, 2, 17, 1, 24, 24),
     (1, 1128064, 17, 3, 24, 24),
-    (1, 1128128, 18596, 3, 24, 24),
+    (1, 1128128, 8265, 32, 24, 24),
     (1, 1128256, 16490, 32, 24, 24),
-    (1, 1256256, 8265, 32, 24, 24),
+    (1, 1256256, 76197, 8, 136, 24),
     (1, 2128064, 18, 1, 24, 1408),
     (1, 2128128, 4812, 2, 24, 2144),
     (1, 2128256, 8546, 32, 24, 2048),
+    (1, 2256256, 4771, 2, 136, 1416),
     (1, 4128064, 17, 1, 24, 1416),
     (1, 4128128, 2378, 2, 24, 2016),
     (1, 4128256, 4265, 32, 24, 2296),
+    (1, 4256256, 2676, 3, 136, 1944),
     (1, 8128064, 17, 1, 24, 5928),
     (1, 8128128, 513, 8, 24, 8960),
     (1, 8128256, 2203, 1, 24, 9040),
     (2, 1128064, 17, 8, 24, 24),
-    (2, 1128128, 19, 32, 1152, 24),
+    (2, 1128128, 23, 32, 264, 24),
     (2, 1128256, 18, 32, 576, 24),
-    (2, 1256256, 23, 32, 264, 24),
+    (2, 1256256, 22, 32, 2360, 136),
     (2, 2128064, 10873, 8, 24, 24),
     (2, 2128128, 2119, 1, 5456, 24),
     (2, 2128256, 2042, 1, 9744, 24),
+    (2, 2256256, 1364, 1, 5232, 136),
     (2, 4128064, 11311, 8, 24, 24),
     (2, 4128128, 1957, 1, 2136, 24),
     (2, 4128256, 73470, 32, 136, 24),
+    (2, 4256256, 4020, 2, 1160, 144),
     (2, 8128128, 8138, 1, 1544, 24),
     (2, 8128256, 7955, 1, 3008, 24),
     (2, 16128064, 1223, 1, 24, 24),
@@ -97,15 +103,17 @@ VARIANTS = [
     (2, 32128128, 237740, 1, 40, 24),
     (2, 32128256, 9732, 1, 3552, 24),
     (3, 1128064, 17, 3, 24, 24),
-    (3, 1128128, 32810, 32, 24, 24),
+    (3, 1128128, 8484, 32, 24, 24),
     (3, 1128256, 16623, 32, 24, 24),
-    (3, 1256256, 8484, 32, 24, 24),
+    (3, 1256256, 2096, 8, 24, 4848),
     (3, 2128064, 18, 3, 2776, 24),
     (3, 2128128, 4926, 1, 4232, 24),
     (3, 2128256, 8309, 32, 4240, 24),
+    (3, 2256256, 4800, 8, 2760, 160),
     (3, 4128064, 17, 2, 2992, 24),
     (3, 4128128, 2149, 32, 3872, 24),
     (3, 4128256, 4105, 32, 4000, 24),
+    (3, 4256256, 2454, 2, 3936, 136),
     (3, 8128064, 18, 1, 10864, 24),
 ]
 
