@@ -69,8 +69,6 @@ struct alignas(16) LinUnit {
     int unused;
 };
 
-__host__ __device__ __forceinline__ int lin_ceil(int a, int b) { return (a + b - 1) / b; }
-
 // n / d for 0 <= n < 2^31, 0 < d: a quotient from the reciprocal in fp32, off by n 2^-21 / d at most, corrected twice.  A
 // tenth of the latency of the integer division, of which finding a unit needs several.
 __host__ __device__ __forceinline__ int lin_div(int n, int d) {
@@ -162,7 +160,7 @@ __host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const i
 #ifdef __CUDACC__
 
 // Scans `ends` into the table (one warp).  Ends that step back or pass the last row are clamped, so any content
-// gives row ranges inside the tensors.  Returns nothing; the table is complete after the CTA's next barrier.
+// gives row ranges inside the tensors.  The table is complete after the CTA's next barrier.
 __device__ __forceinline__ void lin_build_table(const LinParams& p, int* row, int* unit, int lane) {
     int rows_before = 0, units_before = 0;
     if (lane == 0) {

@@ -284,6 +284,10 @@ int kdw_linear_auto_variant(int op, int type, int64_t T, int64_t E, int64_t K, i
     int rc = type == KDW_I8 ? i8_args(&args, &l, aligned, aligned, T, E, K, N, K, type, KDW_F16)
                             : f16_args(&args, op, aligned, aligned, T, E, K, N, op == LIN_FWD ? K : N, K, type);
     if (rc) return rc;
+    if (sms < 1) {
+        set_error("linear_auto_variant: sms=%d", sms);
+        return KDW_ERR_ARG;
+    }
     if (is_few(args)) return 1;
     if (is_narrow(args)) return 2;
     LinPlan pl;
@@ -303,7 +307,14 @@ int64_t kdw_linear_f16_workspace_bytes(int op, const void* a, const void* b, int
     if (!rc) rc = device_facts(nullptr, &sms);
     if (!rc && (is_few(args) || is_narrow(args))) return 0;
     if (!rc) rc = linear_plan(&pl, args, sms);
-    return rc ? (rc < 0 ? rc : -rc) : pl.bytes;
+    int64_t bytes = rc ? 0 : pl.bytes;
+    if (!rc && pl.fold > 1) {  // the call may bring its one group's end, and then folds no rows
+        const int32_t any = 0;
+        args.ends = &any;
+        rc = linear_plan(&pl, args, sms);
+        bytes = std::max(bytes, pl.bytes);
+    }
+    return rc ? (rc < 0 ? rc : -rc) : bytes;
 }
 
 int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_t* ends, void* workspace,

@@ -12,10 +12,13 @@
 namespace kdw {
 
 // ------------------------------------------------------------------------------------------------------------------
-// The product kernel.  One persistent CTA per SM: warp 2 finds the CTA's units and hands their descriptions to the others
-// through a ring in shared memory, warp 0 loads operand tiles with TMA into a ring of stages, warp 1 issues the tensor-core products into accumulators in tensor memory, warps 4-11 and 12-19 take finished accumulators in
-// turn and bring them to memory while the next tiles are being multiplied (eight warps to an accumulator: a warp reads 32
-// of its lanes and every other 32 of its columns), warp 3 clears the output rows behind the last group.
+// The product kernel.  One persistent CTA per SM:
+//   warp 2       finds the CTA's units and hands their descriptions to the others through a ring in shared memory
+//   warp 0       loads operand tiles with TMA into a ring of stages
+//   warp 1       issues the tensor-core products into accumulators in tensor memory
+//   warps 4-11 and 12-19  take finished accumulators in turn and bring them to memory while the next tiles are being
+//                multiplied (eight warps to an accumulator: a warp reads 32 of its lanes and every other 32 of its columns)
+//   warp 3       clears the output rows behind the last group
 //   M side: weights (row products; stored with the contraction contiguous for the forward pass, across it for the input
 //           gradient) or the gradient's rows, transposed (weight gradient).  N side: rows, or their transpose.
 //   PAIR: two CTAs of a cluster share a 256 x BN tile.  Each loads its 128 of M and half of N; the tensor cores of both
@@ -382,8 +385,10 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         const int step = shared_tile ? units : gridDim.x / ctas;  // a shared tile is the cluster's only one
         for (int u = first;; u += step) {
             const bool more = u < units;
-            if (more) w = lin_unit(p, tab->row, tab->unit, u, part);
-            else w.u = -1;
+            if (more)
+                w = lin_unit(p, tab->row, tab->unit, u, part);
+            else
+                w.u = -1;
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(unit_empty + 8 * slot, slot_phase ^ 1, p.limit_ns))) {
                 if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                 break;

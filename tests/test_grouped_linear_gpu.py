@@ -83,6 +83,12 @@ def test_narrow_weights_and_many_rows(K, dtype):
         _check(777, K, N, [771], dtype)
 
 
+@pytest.mark.parametrize('K,N', [(8, 8), (8, 128), (32, 24), (128, 16), (64, 64)])
+@pytest.mark.parametrize('T', [8192, 100000])
+def test_one_narrow_group_that_ends_before_the_last_row(T, K, N):
+    _check(T, K, N, [T - 70], torch.bfloat16)
+
+
 def test_folded_rows_do_not_mix():
     """A NaN in one voxel stays with its own products: the blocks that pair neighbouring voxels are not summed."""
     from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD

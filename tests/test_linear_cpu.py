@@ -111,4 +111,4 @@ def test_the_listed_sizes_get_every_variant(kdw_lib):
         T, K, N = (int(2 ** (float(torch.rand((), generator=g)) * b)) for b in (20, 13, 13))
         E, op = int(torch.randint(1, 40, (), generator=g)), int(torch.randint(0, 4, (), generator=g))
         assert (op, auto(op % 3, 2 if op == 3 else 0, T, E, K, N, 148)) in listed
-    assert auto(3, 0, 8, 1, 8, 8, 148) == auto(0, 3, 8, 1, 8, 8, 148) == auto(0, 0, 0, 1, 8, 8, 148) == -1
+    assert auto(3, 0, 8, 1, 8, 8, 148) == auto(0, 3, 8, 1, 8, 8, 148) == auto(0, 0, 0, 1, 8, 8, 148) == auto(0, 0, 8, 1, 8, 8, 0) == -1
