@@ -1,5 +1,6 @@
 /*
- * kdw.h - C ABI of the B200 (sm_100a) depthwise 3x3x3 channels-last fp16 convolution library.
+ * kdw.h - C ABI of the B200 (sm_100a) depthwise 3x3x3 channels-last fp16 convolution library, and of the channel-mixing
+ * products that follow such a convolution (kdw_linear_*, kdw_quant_rows; no reference counterpart).
  *
  * The library replaces the device side of two kerops operators:
  *   kerops.ops.conv.DWConv       (kerops/ops/conv/dwconv.py:25-63,  kernel kerops/kernels/dw_conv.py:5-142)

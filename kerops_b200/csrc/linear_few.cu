@@ -7,6 +7,9 @@
 // the tensor pipe is idle almost always.  A CTA takes 16 output channels of one group and splits the contraction over its
 // four or eight warps in pieces of 64 bytes, so that the CTA reads runs of 256 or 512 bytes; the warps' sums are added in shared memory.
 //
+// One row of 4096 x 4096 takes 8.5 us in bf16 and 4.4 us in 8 bits (0.60 and 0.59 of the measured bandwidth: some 3 us are
+// the launch, the first load's latency and the last sums), 8192 x 16384 in bf16 51 us (0.80).
+//
 // 8-bit products of 16-bit rows: with at most eight rows every CTA quantises the rows it needs itself (they come from L2),
 // which is cheaper than a kernel in front.
 #include "../../include/kdw.h"

@@ -6,6 +6,9 @@
 // The weights stay in registers as the other operand for the whole kernel.  The order of the contraction and of the output
 // columns inside a fragment is free: a lane's words of a 16-byte piece of a row are the operands of two products as they
 // come, and the columns are dealt to the fragments so that a lane's results are 16 contiguous bytes of an output row.
+//
+// 4.48 M rows, fp16: 32 -> 32 channels 95 us, 128 -> 8 186 us (0.93 and 1.00 of the measured copy bandwidth), 64 -> 64, whose
+// weights fill the registers, 204 us (0.86); the tensor-core kernel of linear_mma.cu took 295 us for 64 -> 32 (now 139 us).
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
