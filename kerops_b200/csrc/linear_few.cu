@@ -7,7 +7,7 @@
 // the tensor pipe is idle almost always.  A CTA takes 16 output channels of one group and splits the contraction over its
 // four or eight warps in pieces of 64 bytes, so that the CTA reads runs of 256 or 512 bytes; the warps' sums are added in shared memory.
 //
-// One row of 4096 x 4096 takes 8.5 us in bf16 and 4.4 us in 8 bits (0.60 and 0.59 of the measured bandwidth: some 3 us are
+// One row of 4096 x 4096 takes 7.6 us in bf16 and 4.4 us in 8 bits (0.68 and 0.59 of the measured bandwidth: some 2 us are
 // the launch, the first load's latency and the last sums), 8192 x 16384 in bf16 51 us (0.80).
 //
 // 8-bit products of 16-bit rows: with at most eight rows every CTA quantises the rows it needs itself (they come from L2),
@@ -197,13 +197,12 @@ __global__ __launch_bounds__(32 * WARPS, 2) void linear_few_kernel(const __grid_
 
     for (int t0 = begin; t0 < end; t0 += NT * 8) {
         Piece<VEC> wp[U][2];
-        auto load_weights = [&](int c) {
+        auto load_weights = [&](int u, int c) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) wp[u][h].template issue<true>(wr[h], (c + u * KW) * 64 + tig * 16, wlen[h]);
+            for (int h = 0; h < 2; ++h) wp[u][h].template issue<true>(wr[h], c * 64 + tig * 16, wlen[h]);
         };
-        load_weights(kw);
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_weights(u, kw + u * KW);
         if constexpr (QUANT) {
             // the rows of this tile, quantised into shared memory while the first weights are on their way
             const int rows = end - t0 < 8 ? end - t0 : 8;
@@ -244,27 +243,35 @@ __global__ __launch_bounds__(32 * WARPS, 2) void linear_few_kernel(const __grid_
             xlen[j] = t < end ? p.len : 0;
             xr[j] = QUANT ? s_q + gid * p.q_pitch : p.x + (t < end ? t : t0) * p.x_pitch;
         }
+        Piece<VEC || QUANT> xp[U][NT];
+        auto load_rows = [&](int u, int c) {
+            const int at = c * 64 + tig * 16;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if constexpr (QUANT)
+                    xp[u][j].v = at < xlen[j] ? *reinterpret_cast<const uint4*>(xr[j] + at) : make_uint4(0, 0, 0, 0);
+                else
+                    xp[u][j].template issue<false>(xr[j], at, xlen[j]);
+        };
+        if (!QUANT) {  // quantised rows wait in shared memory
+#pragma unroll
+            for (int u = 0; u < U; ++u) load_rows(u, kw + u * KW);
+        }
         for (int c = kw; c < pieces; c += U * KW) {
-            if (c != kw) load_weights(c);
-            Piece<VEC || QUANT> xp[U][NT];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int at = (c + u * KW) * 64 + tig * 16;
-                    if constexpr (QUANT)
-                        xp[u][j].v = at < xlen[j] ? *reinterpret_cast<const uint4*>(xr[j] + at) : make_uint4(0, 0, 0, 0);
-                    else
-                        xp[u][j].template issue<false>(xr[j], at, xlen[j]);
-                }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                if (QUANT) load_rows(u, c + u * KW);
                 const uint4 w0 = wp[u][0].get(), w1 = wp[u][1].get();
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const uint4 x = xp[u][j].get();
                     few_mma<I8, BF16>(acc[j], w0.x, w1.x, w0.y, w1.y, x.x, x.y);
                     few_mma<I8, BF16>(acc[j], w0.z, w1.z, w0.w, w1.w, x.z, x.w);
+                }
+                // the piece that takes this one's place is on its way while the others are used
+                if (c + U * KW < pieces) {
+                    load_weights(u, c + (u + U) * KW);
+                    if (!QUANT) load_rows(u, c + (u + U) * KW);
                 }
             }
         }
@@ -308,11 +315,13 @@ static int few_warps(const FewParams& p, cudaStream_t st) {
 }
 template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
 static int few_launch(const FewParams& p, cudaStream_t st) {
-    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four.
+    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four (7.6 us
+    // since a piece's successor is loaded as soon as it has been used).
     constexpr int U = (NT == 1 ? 8 : 4) / (VEC ? 1 : 4);
     const long long ctas = (long long)((p.N + 15) / 16) * (p.ends ? (p.E < p.T ? p.E : p.T) : 1);
     // 32 channels to a CTA where CTAs of 16 would not all be resident at once (two to an SM): 8 rows of 8 groups, 2048 ->
-    // 1024, 9.1 us instead of 10.3; with fewer CTAs the contraction is better split further (4096 x 4096: 8.5 and 11.2 us).
+    // 1024, 9.1 us instead of 10.3 (8.3 now that pieces run ahead); with fewer CTAs the contraction is better split further
+    // (4096 x 4096: 8.5 and 11.2 us, measured before that too).
     if (ctas > 296) return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 32>(p, st);
     return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 16>(p, st);
 }

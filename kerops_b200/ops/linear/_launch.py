@@ -39,15 +39,16 @@ def like_rows(rows, t):
 
 
 def row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else cols
 
 
 def check_ends(ends, groups, rows):
     if ends is None:
         assert groups == 1, 'ends is needed with more than one group'
         return
-    assert ends.dtype == torch.int32 and ends.ndim == 1 and ends.is_contiguous(), 'ends: contiguous int32 vector expected'
-    assert ends.shape[0] == groups, 'ends: one cumulative row count per group expected'
+    assert ends.dtype is torch.int32 and ends.ndim == 1 and ends.is_contiguous(), 'ends: contiguous int32 vector expected'
+    assert len(ends) == groups, 'ends: one cumulative row count per group expected'
     assert ends.get_device() == rows.get_device(), 'ends must be on the device of the rows'
 
 
