@@ -6,10 +6,9 @@ stride-1, pad-1 cross-correlation is the same cross-correlation of the upstream 
 on all three axes, so it runs on the forward kernel unchanged.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from .ops.conv import DWConv, DWConvWGRAD
-from .ops.linear import GroupedLinear
+from .ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
 from .ops.linear.grouped_linear import grouped_linear_grads
 
 
@@ -59,8 +58,20 @@ class DepthwiseConv3d(torch.nn.Module):
         return depthwise_conv3d(x, self.weight)
 
 
+def _rows_contiguous(t):
+    """An expanded or transposed gradient (of a sum, say) has no rows of contiguous channels."""
+    if t.ndim == 5:
+        return t.contiguous(memory_format=torch.channels_last_3d)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+# The product is linear in each of its arguments, so the gradients of the three operators are the three operators again:
+#   y  = F(x, w):   dx = D(dy, w)   dw = W(x, dy)
+#   dx = D(g, w):   dg = F(v, w)    dw = W(v, g)        v, V: the gradients of dx, dw
+#   dw = W(x, g):   dx = D(g, V)    dg = F(x, V)
+# A backward pass that is itself to be differentiated goes through the functions below, any other calls the operators.
 class GroupedLinearFunction(torch.autograd.Function):
-    """y = GroupedLinear(x, weight, ends) with gradients for x and weight."""
+    """y = GroupedLinear(x, weight, ends) with gradients for x and weight, differentiable any number of times."""
 
     @staticmethod
     def forward(ctx, x, weight, ends):
@@ -68,12 +79,48 @@ class GroupedLinearFunction(torch.autograd.Function):
         return GroupedLinear(x, weight, ends)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
         x, weight, ends = ctx.saved_tensors
-        # an expanded or transposed gradient (of a sum, say) has no rows of contiguous channels
-        grad_out = grad_out.contiguous(memory_format=torch.channels_last_3d if x.ndim == 5 else torch.contiguous_format)
-        return (*grouped_linear_grads(x, weight, grad_out, ends, ctx.needs_input_grad[:2]), None)
+        grad_out = _rows_contiguous(grad_out)
+        need_x, need_w, _ = ctx.needs_input_grad
+        if torch.is_grad_enabled():
+            return (GroupedLinearDGRADFunction.apply(grad_out, weight, ends) if need_x else None,
+                    GroupedLinearWGRADFunction.apply(x, grad_out, weight, ends) if need_w else None, None)
+        dx, dw = grouped_linear_grads(x, weight, grad_out, ends, need_x, need_w)
+        return dx, dw, None
+
+
+class GroupedLinearDGRADFunction(torch.autograd.Function):
+    """dx = GroupedLinearDGRAD(grad, weight, ends) with gradients for grad and weight."""
+
+    @staticmethod
+    def forward(ctx, grad, weight, ends):
+        ctx.save_for_backward(grad, weight, ends)
+        return GroupedLinearDGRAD(grad, weight, ends)
+
+    @staticmethod
+    def backward(ctx, v):
+        grad, weight, ends = ctx.saved_tensors
+        v = _rows_contiguous(v)
+        need_g, need_w, _ = ctx.needs_input_grad
+        return (GroupedLinearFunction.apply(v, weight, ends) if need_g else None,
+                GroupedLinearWGRADFunction.apply(v, grad, weight, ends) if need_w else None, None)
+
+
+class GroupedLinearWGRADFunction(torch.autograd.Function):
+    """dw = GroupedLinearWGRAD(x, grad, ends) in the form of `like`, with gradients for x and grad."""
+
+    @staticmethod
+    def forward(ctx, x, grad, like, ends):
+        ctx.save_for_backward(x, grad, ends)
+        return GroupedLinearWGRAD(x, grad, ends).view(like.shape)
+
+    @staticmethod
+    def backward(ctx, v):
+        x, grad, ends = ctx.saved_tensors
+        v = v.contiguous()
+        return (GroupedLinearDGRADFunction.apply(grad, v, ends) if ctx.needs_input_grad[0] else None,
+                GroupedLinearFunction.apply(x, v, ends) if ctx.needs_input_grad[1] else None, None, None)
 
 
 def grouped_linear(x, weight, ends=None):

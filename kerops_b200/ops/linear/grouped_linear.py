@@ -80,19 +80,19 @@ def GroupedLinearWGRAD(x, grad, ends=None):
     return dw
 
 
-def grouped_linear_grads(x, weight, grad, ends, wanted):
-    """(dx, dw) of a GroupedLinear(x, weight, ends) that has been checked when it ran, or None where `wanted` says so; grad
-    is a contiguous gradient of its result, dw has weight's shape."""
-    E, N, K = _weight_dims(weight)
+def grouped_linear_grads(x, weight, grad, ends, need_x, need_w):
+    """(dx, dw) of a GroupedLinear(x, weight, ends) that has been checked when it ran, None for one that is not needed; grad is
+    a contiguous gradient of its result, dw has weight's shape."""
+    E, N, K = weight.shape if weight.ndim == 3 else (1, *weight.shape)
     xr, gr = _launch.as_rows(x, 'x'), _launch.as_rows(grad, 'grad')
     T = xr.shape[0]
     dx = dw = None
-    if wanted[0]:
+    if need_x:
         dx = gr.new_empty((T, K))
         if T:
             _launch.product(_launch.DGRAD, gr, weight, dx, ends, T, E, K, N)
         dx = _launch.like_rows(dx, x)
-    if wanted[1]:
+    if need_w:
         dw = torch.empty_like(weight)
         if T:
             _launch.product(_launch.WGRAD, gr, xr, dw, ends, T, E, K, N)

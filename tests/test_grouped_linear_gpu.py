@@ -353,9 +353,6 @@ def test_autograd_formula_and_differences(shape):
         along_w = grouped_linear(x, w + dw, e).double() - y.double()
     assert (along_x * g.double()).sum() == (x.grad.double() * dx.double()).sum()
     assert (along_w * g.double()).sum() == (w.grad.double() * dw.double()).sum()
-    with pytest.raises(RuntimeError, match='once_differentiable'):
-        dx_, = torch.autograd.grad(grouped_linear(x, w, e), x, g.requires_grad_(True), create_graph=True)
-        dx_.sum().backward()
     # a gradient that is one value expanded, only one of the gradients wanted, and the module
     m = ExpertLinear(3, K, N, device='cuda')
     m(x.detach(), e).sum().backward()
@@ -365,6 +362,33 @@ def test_autograd_formula_and_differences(shape):
     m(x, e).sum().backward()
     err = (rows(x.grad).double() - ref.dgrad(torch.ones(T, N, device='cuda'), m.weight, ends)).abs()
     assert (err <= 2.0 ** -11 * rows(x.grad).abs() + N * 2.0 ** -23 * N / 4).all()  # |w| <= 1/4
+
+
+@pytest.mark.parametrize('shape', ['matrix', 'volume'])
+@pytest.mark.parametrize('groups', [1, 3])
+def test_gradients_of_gradients(shape, groups):
+    """s = <u, dx> + <V, dw> of a backward pass, differentiated again: ds/dg = u w + x V, ds/dx = g V, ds/dw = g^T u."""
+    from kerops_b200.autograd import grouped_linear
+
+    T, K, N = 210, 16, 24
+    ends = [T] if groups == 1 else [50, 50, 200]
+    e = None if groups == 1 else ref.tensor_ends(ends)
+
+    def form(t):
+        return t if shape == 'matrix' else t.view(2, 3, 5, 7, -1).permute(0, 4, 1, 2, 3)
+
+    def rows(t):
+        return t if shape == 'matrix' else t.permute(0, 2, 3, 4, 1).reshape(T, -1)
+
+    x, g, u = (form(ref.integers((T, c), torch.float16, i, top=1)).requires_grad_(True) for i, c in enumerate((K, N, K)))
+    w, V = (ref.integers((groups, N, K) if groups > 1 else (N, K), torch.float16, i, top=1).requires_grad_(True) for i in (3, 4))
+    dx, dw = torch.autograd.grad(grouped_linear(x, w, e), (x, w), g, create_graph=True)
+    s = (dx.float() * u.float()).sum() + (dw.float() * V.float()).sum()
+    gg, gx, gw = torch.autograd.grad(s, (g, x, w))
+    xr, gr, ur, w3, V3 = rows(x.detach()), rows(g.detach()), rows(u.detach()), w.detach().view(groups, N, K), V.detach().view(groups, N, K)
+    assert torch.equal(rows(gg), (ref.fwd(ur, w3, ends) + ref.fwd(xr, V3, ends)).half())
+    assert torch.equal(rows(gx), ref.dgrad(gr, V3, ends).half())
+    assert torch.equal(gw.view(groups, N, K), ref.wgrad(ur, gr, ends).half())
 
 
 def test_depthwise_then_pointwise_step():
