@@ -8,7 +8,7 @@
 // come, and the columns are dealt to the fragments so that a lane's results are 16 contiguous bytes of an output row.
 //
 // 4.48 M rows, fp16: 32 -> 32 channels 95 us, 128 -> 8 186 us (0.93 and 1.00 of the measured copy bandwidth), 64 -> 64, whose
-// weights fill the registers, 204 us (0.86); the tensor-core kernel of linear_mma.cu took 295 us for 64 -> 32 (now 139 us).
+// weights fill the registers, 200 us (0.87); the tensor-core kernel of linear_mma.cu took 295 us for 64 -> 32 (now 139 us).
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
@@ -66,6 +66,10 @@ struct NCfg {
     static constexpr int COLS = NP >= 32 ? 32 : NP;             // columns whose results a lane stores as one piece
     static constexpr int GROUPS = NP / COLS, TILES = COLS / 8;  // of eight columns, per piece
     static constexpr int AHEAD = PIECES >= 4 ? 1 : PIECES == 2 ? 2 : 4;  // row tiles whose loads are in flight
+    // The tiles of a warp in flight are neighbours, or spread over the warps' tiles where rows of 256 bytes are written.
+    // 4.48 M rows, us, neighbours and spread: 64 -> 64 200 and 207, 32 -> 64 158 and 163, 8 -> 128 212 and 220, but 16 -> 128
+    // 270 and 241, 32 -> 128 291 and 247.
+    static constexpr bool SPREAD = NP == 128 && KP >= 16;
     static constexpr int THREADS = 128;
     static constexpr int CTAS = KP * NP >= 4096 ? 3 : 4;        // to an SM at least: what the registers have to allow
 };
@@ -127,11 +131,11 @@ __global__ __launch_bounds__(C::THREADS, C::CTAS) void linear_narrow_kernel(cons
     };
     uint32_t a[C::AHEAD][C::PIECES][2][C::WORDS];
 #pragma unroll
-    for (int i = 0; i < C::AHEAD; ++i) load(a[i], warp + i * warps);
-    for (long long t0 = warp; t0 < tiles; t0 += C::AHEAD * warps) {
+    for (int i = 0; i < C::AHEAD; ++i) load(a[i], C::SPREAD ? warp + i * warps : warp * C::AHEAD + i);
+    for (long long t0 = C::SPREAD ? warp : warp * C::AHEAD; t0 < tiles; t0 += C::AHEAD * warps) {
 #pragma unroll
         for (int i = 0; i < C::AHEAD; ++i) {
-            const long long t = t0 + i * warps;
+            const long long t = t0 + (C::SPREAD ? i * warps : i);
             if (t >= tiles) break;
 #pragma unroll
             for (int g = 0; g < C::GROUPS; ++g) {

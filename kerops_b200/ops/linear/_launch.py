@@ -14,8 +14,8 @@ MAX_GROUPS = 1024
 
 # of a device index, and the current one: torch.cuda.current_stream and torch.cuda.device cost 3 us more, a quarter of a
 # small call
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # (absent from builds of torch without CUDA)
+_current_device = getattr(torch._C, '_cuda_getDevice', None)
 
 
 def as_rows(t, name):
