@@ -108,7 +108,9 @@ int linear_plan(LinPlan* pl, const LinArgs& given, int sms) {
         const bool pair = c.tile_m == 256;
         const int slots = pair ? sms / 2 : sms;
         const double m_tiles = (double)ceil_div(wgrad ? a.N : pl->out_cols, c.tile_m);
-        const double n_tiles = wgrad ? (double)ceil_div(pl->out_cols, c.bn) : std::ceil(rows / c.bn);
+        // (groups of unlike sizes have half a tile more than their rows fill, one group as many as it needs)
+        const double n_tiles = wgrad ? (double)ceil_div(pl->out_cols, c.bn)
+                                     : groups == 1 ? std::ceil(rows / c.bn) : std::max(1.0, rows / c.bn + 0.5);
         const double width = wgrad ? c.bn : std::min<double>(c.bn, std::ceil(rows / n_tiles / 32) * 32);
         const double tiles = m_tiles * n_tiles * (wgrad ? a.E : groups);
         const double block = std::max(2 * width, 256 + (pair ? 1 : 2) * (double)c.bn);

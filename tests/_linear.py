@@ -51,36 +51,36 @@ VARIANTS = [
     (3, 1, 9, 3, 80, 40),
     (0, 2, 17, 1, 24, 24),
     (0, 1128064, 17, 2, 24, 24),
-    (0, 1128128, 8193, 32, 24, 24),
+    (0, 1128128, 8548, 32, 24, 24),
     (0, 1128256, 16961, 32, 24, 24),
-    (0, 1256256, 1061, 8, 24, 9880),
+    (0, 1256256, 2556, 32, 24, 2592),
     (0, 2128064, 17, 3, 1368, 24),
     (0, 2128128, 4970, 1, 2128, 24),
     (0, 2128256, 9614, 3, 2040, 24),
     (0, 2256256, 4325, 32, 1416, 168),
     (0, 4128064, 17, 1, 1528, 24),
-    (0, 4128128, 2076, 2, 1968, 24),
+    (0, 4128128, 1100, 32, 2504, 24),
     (0, 4128256, 4839, 1, 2032, 24),
     (0, 4256256, 2485, 1, 2064, 144),
     (0, 8128064, 17, 2, 5536, 24),
-    (0, 8128128, 561, 8, 8184, 24),
-    (0, 8128256, 2140, 3, 8696, 24),
+    (0, 8128128, 768, 8, 8016, 24),
+    (0, 8128256, 2105, 3, 8728, 24),
     (1, 2, 17, 1, 24, 24),
     (1, 1128064, 17, 3, 24, 24),
-    (1, 1128128, 8265, 32, 24, 24),
-    (1, 1128256, 16490, 32, 24, 24),
-    (1, 1256256, 76197, 8, 136, 24),
+    (1, 1128128, 8585, 32, 24, 24),
+    (1, 1128256, 17155, 32, 24, 24),
+    (1, 1256256, 777, 8, 9536, 24),
     (1, 2128064, 18, 1, 24, 1408),
-    (1, 2128128, 4812, 2, 24, 2144),
+    (1, 2128128, 4520, 8, 24, 2152),
     (1, 2128256, 8546, 32, 24, 2048),
     (1, 2256256, 4771, 2, 136, 1416),
     (1, 4128064, 17, 1, 24, 1416),
-    (1, 4128128, 2378, 2, 24, 2016),
-    (1, 4128256, 4265, 32, 24, 2296),
-    (1, 4256256, 2676, 3, 136, 1944),
+    (1, 4128128, 1114, 32, 24, 2048),
+    (1, 4128256, 3761, 32, 24, 2384),
+    (1, 4256256, 2173, 8, 152, 1960),
     (1, 8128064, 17, 1, 24, 5928),
-    (1, 8128128, 513, 8, 24, 8960),
-    (1, 8128256, 2203, 1, 24, 9040),
+    (1, 8128128, 838, 8, 24, 7944),
+    (1, 8128256, 1935, 8, 24, 8912),
     (2, 1128064, 17, 8, 24, 24),
     (2, 1128128, 23, 32, 264, 24),
     (2, 1128256, 18, 32, 576, 24),
@@ -104,14 +104,14 @@ VARIANTS = [
     (2, 32128256, 9732, 1, 3552, 24),
     (3, 1128064, 17, 3, 24, 24),
     (3, 1128128, 8484, 32, 24, 24),
-    (3, 1128256, 16623, 32, 24, 24),
-    (3, 1256256, 2096, 8, 24, 4848),
+    (3, 1128256, 16926, 32, 24, 24),
+    (3, 1256256, 638, 8, 24, 11160),
     (3, 2128064, 18, 3, 2776, 24),
     (3, 2128128, 4926, 1, 4232, 24),
-    (3, 2128256, 8309, 32, 4240, 24),
+    (3, 2128256, 9872, 2, 4024, 24),
     (3, 2256256, 4800, 8, 2760, 160),
     (3, 4128064, 17, 2, 2992, 24),
-    (3, 4128128, 2149, 32, 3872, 24),
+    (3, 4128128, 1147, 32, 3960, 24),
     (3, 4128256, 4105, 32, 4000, 24),
     (3, 4256256, 2454, 2, 3936, 136),
     (3, 8128064, 18, 1, 10864, 24),
