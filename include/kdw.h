@@ -267,6 +267,17 @@ int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_
                    int64_t b_stride, int dtype, void* stream);
 
 /*
+ * Both gradients of the forward product y = KDW_LINEAR_FWD(x, w) from the gradient of y: dx = KDW_LINEAR_DGRAD(grad, w) and
+ * dw = KDW_LINEAR_WGRAD(grad, x), with one workspace and one copy of an operand that needs it.  has_ends: whether the call
+ * will bring `ends`.
+ */
+int64_t kdw_linear_grads_f16_workspace_bytes(const void* x, const void* w, const void* grad, int has_ends, int64_t T, int64_t E,
+                                             int64_t K, int64_t N, int64_t x_stride, int64_t grad_stride, int dtype);
+int kdw_linear_grads_f16(const void* x, const void* w, const void* grad, void* dx, void* dw, const int32_t* ends, void* workspace,
+                         int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t x_stride,
+                         int64_t grad_stride, int dtype, void* stream);
+
+/*
  * Rows of 16-bit values as 8-bit integers:  scale[r] = max|x[r,:]| / 127,  q[r,c] = x[r,c] * 127 / max|x[r,:]| rounded to
  * the nearest integer, halves to even (the exact quotient's rounding).  A row of zeros gives q = 0 and scale 0, a row
  * with a NaN or an infinity q = 0 and scale NaN.  x: KDW_F16 / KDW_BF16 [rows] x x_stride; q dense [rows][cols].

@@ -45,6 +45,8 @@ SIGNATURES = {
     'kdw_linear_auto_variant': (_int, [_int, _int] + [_i64] * 4 + [_int]),
     'kdw_linear_f16_workspace_bytes': (_i64, [_int, _ptr, _ptr] + [_i64] * 6 + [_int]),
     'kdw_linear_f16': (_int, [_int] + [_ptr] * 5 + [_i64] + [_i64] * 6 + [_int, _ptr]),
+    'kdw_linear_grads_f16_workspace_bytes': (_i64, [_ptr] * 3 + [_int] + [_i64] * 6 + [_int]),
+    'kdw_linear_grads_f16': (_int, [_ptr] * 7 + [_i64] + [_i64] * 6 + [_int, _ptr]),
     'kdw_quant_rows': (_int, [_ptr] * 3 + [_i64] * 3 + [_int, _ptr]),
     'kdw_linear_i8_workspace_bytes': (_i64, [_ptr, _ptr] + [_i64] * 5 + [_int, _int]),
     'kdw_linear_i8': (_int, [_ptr] * 7 + [_i64] + [_i64] * 5 + [_int, _int, _ptr]),

@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 
 #include "kdw_common.cuh"
+#include "linear_plan.h"
 
 namespace kdw {
 
@@ -404,6 +405,29 @@ __device__ __forceinline__ void store_matrix_trans(uint32_t addr, uint32_t a, ui
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool row_contiguous) {
     const uint64_t lead = row_contiguous ? 8192 >> 4 : 1, stride = 1024 >> 4;
     return (uint64_t)((addr & 0x3ffff) >> 4) | lead << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// CTA `cta` of `ctas` (of 256 threads or fewer, `threads`) copies its part of rows to a 16-byte pitch; what lies between the
+// columns and the pitch is written too, but never read (the tensor maps end at the columns).
+template <typename T>
+__device__ __forceinline__ void pack_rows_part(const PackRows& a, long long cta, long long ctas, int threads = 256) {
+    constexpr int V = 16 / sizeof(T);
+    const T* src = reinterpret_cast<const T*>(a.src);
+    const int per_row = (a.cols + V - 1) / V;
+    const long long n = a.rows * per_row;
+    for (long long i = cta * threads + threadIdx.x; i < n; i += ctas * threads) {
+        const long long r = n <= 0x7fffffff ? (unsigned)i / (unsigned)per_row : i / per_row;
+        const int c = (int)(i - r * per_row) * V;
+        union {
+            uint4 u;
+            T t[V];
+        } v;
+        v.u = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (c + j < a.cols) v.t[j] = src[r * a.src_stride + c + j];
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + r * a.dst_stride + c) = v.u;
+    }
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {

@@ -214,7 +214,8 @@ static bool is_few(const LinArgs& a) { return a.op == LIN_FWD && a.T <= kFewRows
 
 // The 8-bit product: the rows are int8 with their scales, or 16-bit rows that are quantised into the workspace first.
 struct I8Layout {
-    int64_t q_pitch, off_scale, off_rest;  // bytes; quantised rows at 0
+    int64_t q_pitch, off_scale, off_w, off_rest;  // bytes; quantised rows at 0
+    bool pack_w;                                  // the kernel that quantises copies the weights to a pitch of 16 bytes too
 };
 static int i8_args(LinArgs* a, I8Layout* l, const void* x, const void* w, int64_t T, int64_t E, int64_t K, int64_t N,
                    int64_t x_stride, int x_type, int dtype) {
@@ -233,25 +234,68 @@ static int i8_args(LinArgs* a, I8Layout* l, const void* x, const void* w, int64_
         return KDW_ERR_ARG;
     }
     *a = LinArgs();
-    l->q_pitch = l->off_scale = l->off_rest = 0;
+    l->q_pitch = l->off_scale = l->off_w = l->off_rest = 0;
+    l->pack_w = false;
     a->op = LIN_FWD;
     a->a = x;
     a->a_stride = x_stride;
+    a->b = w;
+    a->b_stride = K;
     if (x_type != KDW_I8) {
         l->q_pitch = round_up(K, 16);
         l->off_scale = round_up(T * l->q_pitch, 256);
-        l->off_rest = round_up(l->off_scale + 4 * T, 256);
+        l->off_w = l->off_rest = round_up(l->off_scale + 4 * T, 256);
         a->a = nullptr;  // its copy in the workspace is aligned
         a->a_stride = l->q_pitch;
+        l->pack_w = T > kFewRows && (((uintptr_t)w & 15) != 0 || K % 16 != 0);
+        if (l->pack_w) {
+            l->off_rest = round_up(l->off_w + E * N * l->q_pitch, 256);
+            a->b = nullptr;
+            a->b_stride = l->q_pitch;
+        }
     }
-    a->b = w;
-    a->b_stride = K;
     a->T = T;
     a->E = E;
     a->K = K;
     a->N = N;
     a->esize = 1;
     a->out_bf16 = dtype == KDW_BF16;
+    return 0;
+}
+
+// Both gradients of one product: operands that TMA cannot address are copied once for the two.
+struct GradsLayout {
+    bool pack_g, pack_x, pack_w;
+    int64_t g_pitch, k_pitch;               // elements
+    int64_t off_g, off_x, off_w, off_rest;  // bytes
+};
+static int grads_args(LinArgs* d, LinArgs* g, GradsLayout* l, const void* x, const void* w, const void* grad, int64_t T, int64_t E,
+                      int64_t K, int64_t N, int64_t x_stride, int64_t grad_stride, int dtype) {
+    int rc = f16_args(d, LIN_DGRAD, grad, w, T, E, K, N, grad_stride, 0, dtype);
+    if (!rc) rc = f16_args(g, LIN_WGRAD, grad, x, T, E, K, N, grad_stride, x_stride, dtype);
+    if (rc) return rc;
+    auto odd = [](const void* p, int64_t stride) { return ((uintptr_t)p & 15) != 0 || stride % 8 != 0; };
+    l->pack_g = odd(grad, grad_stride);
+    l->pack_x = odd(x, x_stride);
+    l->pack_w = odd(w, K);
+    l->g_pitch = round_up(N, 8);
+    l->k_pitch = round_up(K, 8);
+    l->off_g = 0;
+    l->off_x = round_up(l->pack_g ? T * l->g_pitch * 2 : 0, 256);
+    l->off_w = round_up(l->off_x + (l->pack_x ? T * l->k_pitch * 2 : 0), 256);
+    l->off_rest = round_up(l->off_w + (l->pack_w ? E * N * l->k_pitch * 2 : 0), 256);
+    if (l->pack_g) {
+        d->a = g->a = nullptr;  // the copies in the workspace are aligned
+        d->a_stride = g->a_stride = l->g_pitch;
+    }
+    if (l->pack_x) {
+        g->b = nullptr;
+        g->b_stride = l->k_pitch;
+    }
+    if (l->pack_w) {
+        d->b = nullptr;
+        d->b_stride = l->k_pitch;
+    }
     return 0;
 }
 
@@ -342,6 +386,68 @@ int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_
     return plan_and_run(&args, workspace, workspace_bytes, stream);
 }
 
+int64_t kdw_linear_grads_f16_workspace_bytes(const void* x, const void* w, const void* grad, int has_ends, int64_t T, int64_t E,
+                                             int64_t K, int64_t N, int64_t x_stride, int64_t grad_stride, int dtype) {
+    using namespace kdw;
+    LinArgs d, g;
+    GradsLayout l;
+    LinPlan pl;
+    int sms = 0;
+    int rc = grads_args(&d, &g, &l, x, w, grad, T, E, K, N, x_stride, grad_stride, dtype);
+    if (!rc) rc = device_facts(nullptr, &sms);
+    const int32_t any = 0;
+    d.ends = g.ends = has_ends ? &any : nullptr;
+    int64_t bytes = 0;
+    for (const LinArgs* a : {&d, &g})
+        if (!rc && !is_narrow(*a)) {
+            rc = linear_plan(&pl, *a, sms);
+            bytes = std::max(bytes, rc ? 0 : pl.bytes);
+        }
+    return rc ? (rc < 0 ? rc : -rc) : l.off_rest + bytes;
+}
+
+int kdw_linear_grads_f16(const void* x, const void* w, const void* grad, void* dx, void* dw, const int32_t* ends, void* workspace,
+                         int64_t workspace_bytes, int64_t T, int64_t E, int64_t K, int64_t N, int64_t x_stride,
+                         int64_t grad_stride, int dtype, void* stream) {
+    using namespace kdw;
+    if (!x || !w || !grad || !dx || !dw || (!ends && E != 1)) {
+        set_error("linear_grads_f16: null pointer (ends may be null only with one group)");
+        return KDW_ERR_ARG;
+    }
+    LinArgs d, g;
+    GradsLayout l;
+    int rc = grads_args(&d, &g, &l, x, w, grad, T, E, K, N, x_stride, grad_stride, dtype);
+    if (rc) return rc;
+    if (((uintptr_t)x & 1) || ((uintptr_t)w & 1) || ((uintptr_t)grad & 1) || ((uintptr_t)dx & 1) || ((uintptr_t)dw & 1) ||
+        ((uintptr_t)ends & 3)) {
+        set_error("linear_grads_f16: a pointer is not aligned to its elements");
+        return KDW_ERR_ALIGN;
+    }
+    if (l.off_rest > 0 && (!workspace || workspace_bytes < l.off_rest || ((uintptr_t)workspace & 255) != 0)) {
+        set_error("linear_grads_f16: workspace of at least %lld bytes (256-byte aligned) needed", (long long)l.off_rest);
+        return KDW_ERR_WORKSPACE;
+    }
+    char* ws = (char*)workspace;
+    if (l.off_rest > 0) {
+        const PackRows r[3] = {{grad, ws + l.off_g, l.pack_g ? T : 0, grad_stride, l.g_pitch, (int)N},
+                               {x, ws + l.off_x, l.pack_x ? T : 0, x_stride, l.k_pitch, (int)K},
+                               {w, ws + l.off_w, l.pack_w ? E * N : 0, K, l.k_pitch, (int)K}};
+        rc = pack_rows(r, 3, 2, (cudaStream_t)stream);
+        if (rc) return rc;
+        if (l.pack_g) d.a = g.a = ws + l.off_g;
+        if (l.pack_x) g.b = ws + l.off_x;
+        if (l.pack_w) d.b = ws + l.off_w;
+    }
+    d.out = dx;
+    g.out = dw;
+    d.ends = g.ends = ends;
+    // the second product's kernels touch the workspace only when the first one's have completed
+    ws = ws ? ws + l.off_rest : ws;
+    rc = is_narrow(d) && ((uintptr_t)dx & 15) == 0 ? linear_narrow(d, (cudaStream_t)stream)
+                                                   : plan_and_run(&d, ws, workspace_bytes - l.off_rest, stream);
+    return rc ? rc : plan_and_run(&g, ws, workspace_bytes - l.off_rest, stream);
+}
+
 int64_t kdw_linear_i8_workspace_bytes(const void* x, const void* w, int64_t T, int64_t E, int64_t K, int64_t N,
                                       int64_t x_stride, int x_type, int dtype) {
     using namespace kdw;
@@ -390,9 +496,11 @@ int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const fl
         }
         args.a = ws;
         args.row_scale = (const float*)(ws + l.off_scale);
+        const PackRows pack = {w, ws + l.off_w, E * N, K, l.q_pitch, (int)K};
         rc = quant_rows(x, ws, (float*)(ws + l.off_scale), T, K, x_stride, l.q_pitch, x_type == KDW_BF16, true,
-                        (cudaStream_t)stream);
+                        l.pack_w ? &pack : nullptr, (cudaStream_t)stream);
         if (rc) return rc;
+        if (l.pack_w) args.b = ws + l.off_w;
         ws += l.off_rest;
     }
     if (is_few(args)) return linear_few(args, KDW_I8, (cudaStream_t)stream);

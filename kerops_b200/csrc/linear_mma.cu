@@ -674,42 +674,18 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const __grid_constant_
     }
 }
 
-// Copies rows whose pitch or base TMA cannot address to rows of a 16-byte pitch; what lies between the columns and
-// the pitch is never read (the tensor maps end at the columns).  The first `split` CTAs take the first operand.
-struct PackRows {
-    const void* src;
-    void* dst;
-    long long rows, src_stride, dst_stride;  // in elements
-    int cols;
-};
 template <typename T>
-__device__ __forceinline__ void pack_rows(const PackRows& a, long long cta, long long ctas) {
-    constexpr int V = 16 / sizeof(T);
-    const T* src = reinterpret_cast<const T*>(a.src);
-    const int per_row = (a.cols + V - 1) / V;
-    const long long n = a.rows * per_row;
-    for (long long i = cta * 256 + threadIdx.x; i < n; i += ctas * 256) {
-        const long long r = n <= INT_MAX ? (unsigned)i / (unsigned)per_row : i / per_row;
-        const int c = (int)(i - r * per_row) * V;
-        union {
-            uint4 u;
-            T t[V];
-        } v;
-        v.u = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (c + j < a.cols) v.t[j] = src[r * a.src_stride + c + j];
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dst) + r * a.dst_stride + c) = v.u;
-    }
-}
-template <typename T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const __grid_constant__ PackRows a, const __grid_constant__ PackRows b, int split) {
+__global__ __launch_bounds__(256) void pack_rows_kernel(const __grid_constant__ PackRows a, const __grid_constant__ PackRows b,
+                                                        const __grid_constant__ PackRows c, int split_b, int split_c) {
     grid_dependency_wait();
     grid_launch_dependents();
-    if ((int)blockIdx.x < split)
-        pack_rows<T>(a, blockIdx.x, split);
+    const int cta = blockIdx.x;
+    if (cta < split_b)
+        pack_rows_part<T>(a, cta, split_b);
+    else if (cta < split_c)
+        pack_rows_part<T>(b, cta - split_b, split_c - split_b);
     else
-        pack_rows<T>(b, blockIdx.x - split, gridDim.x - split);
+        pack_rows_part<T>(c, cta - split_c, gridDim.x - split_c);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -751,24 +727,36 @@ static int launch_width(const LinPlan& pl, const CUtensorMap& ma, const CUtensor
     }
 }
 
+int pack_ctas(const PackRows& r, int esize, int sms) {
+    const int64_t want = (r.rows * ((r.cols * (int64_t)esize + 15) / 16) + 255) / 256;
+    return (int)std::min<int64_t>(want, 8 * sms);
+}
+
+int pack_rows(const PackRows* r, int count, int esize, cudaStream_t st) {
+    int sms = 0, rc = device_facts(nullptr, &sms);
+    if (rc) return rc;
+    const PackRows none = {};
+    const PackRows &a = r[0], &b = count > 1 ? r[1] : none, &c = count > 2 ? r[2] : none;
+    const int na = pack_ctas(a, esize, sms), nb = pack_ctas(b, esize, sms), nc = pack_ctas(c, esize, sms);
+    if (na + nb + nc == 0) return 0;
+    KDW_CUDA(launch_overlapping_previous(esize == 2 ? pack_rows_kernel<uint16_t> : pack_rows_kernel<uint8_t>,
+                                         (unsigned)(na + nb + nc), 256u, st, a, b, c, na, na + nb));
+    return 0;
+}
+
 int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     int* status = nullptr;
-    int sms = 0, rc = device_facts(&status, &sms);
+    int sms = 0, rc = device_facts(&status, &sms);  // (launch_product asks for the SMs itself)
     if (rc) return rc;
     char* w = (char*)ws;
     const void* pa = a.a;
     const void* pb = a.b;
     int64_t sa = a.a_stride * pl.fold, sb = a.b_stride * pl.fold;
     if (pl.pack_a || pl.pack_b) {
-        PackRows ra = {pa, w + pl.off_a, pl.pack_a ? pl.a_rows : 0, sa, pl.a_pitch, (int)pl.a_cols};
-        PackRows rb = {pb, w + pl.off_b, pl.pack_b ? pl.b_rows : 0, sb, pl.b_pitch, (int)pl.b_cols};
-        auto ctas = [&](const PackRows& r) {
-            const int64_t want = (r.rows * ((r.cols * (int64_t)pl.esize + 15) / 16) + 255) / 256;
-            return (int)std::min<int64_t>(want, 8 * sms);
-        };
-        const int na = ctas(ra), nb = ctas(rb);
-        KDW_CUDA(launch_overlapping_previous(pl.esize == 2 ? pack_rows_kernel<uint16_t> : pack_rows_kernel<uint8_t>,
-                                             (unsigned)(na + nb), 256u, st, ra, rb, na));
+        const PackRows r[2] = {{pa, w + pl.off_a, pl.pack_a ? pl.a_rows : 0, sa, pl.a_pitch, (int)pl.a_cols},
+                               {pb, w + pl.off_b, pl.pack_b ? pl.b_rows : 0, sb, pl.b_pitch, (int)pl.b_cols}};
+        rc = pack_rows(r, 2, pl.esize, st);
+        if (rc) return rc;
         if (pl.pack_a) {
             pa = w + pl.off_a;
             sa = pl.a_pitch;

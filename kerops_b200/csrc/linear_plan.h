@@ -46,9 +46,22 @@ int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
 bool is_narrow(const LinArgs& a);
 int linear_narrow(const LinArgs& a, cudaStream_t st);
 
+// Rows to copy to a pitch of 16 bytes, because TMA cannot address them where they are; strides in elements.
+struct PackRows {
+    const void* src;
+    void* dst;
+    long long rows, src_stride, dst_stride;
+    int cols;
+};
+// CTAs of 256 threads that copy them; 0: there is nothing to copy.
+int pack_ctas(const PackRows& r, int esize, int sms);
+// Copies up to three operands with one kernel.
+int pack_rows(const PackRows* r, int count, int esize, cudaStream_t st);
+
 // Quantises rows of 16-bit values (see quant_rows.cu); q_padded: what lies between `cols` and q_stride may be written.
+// `pack`, if given, are rows of 8-bit weights that the same kernel copies.
 int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride, int bf16,
-               bool q_padded, cudaStream_t st);
+               bool q_padded, const PackRows* pack, cudaStream_t st);
 
 // Rows of `cols` elements (1 or 2 bytes each) `stride` elements apart, in `groups` matrices `group_stride` elements
 // apart (0 groups: one matrix, a 2-D map); a box of `box_cols` x `box_rows`, 128-byte swizzle, zeros outside.

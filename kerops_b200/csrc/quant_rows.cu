@@ -18,17 +18,22 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int c, int cols) {
 }
 
 // TPR threads to a row (a warp or the CTA), KEEP vectors of 8 values of a thread stay in registers between the two passes
-// over the row; what is longer is read again.  VEC: rows of the input are 16-byte aligned, QVEC: rows of the output 8-byte.
+// over the row; what is longer is read again.  CTAs from `ctas` on copy weights instead.  VEC: rows of the input are 16-byte aligned, QVEC: rows of the output 8-byte.
 template <int TPR, int KEEP, bool VEC, bool QVEC, int THREADS>
 __global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __restrict__ x, int8_t* __restrict__ q,
                                                          float* __restrict__ scale, long long rows, int cols,
-                                                         long long x_stride, long long q_stride, int bf16) {
+                                                         long long x_stride, long long q_stride, int bf16,
+                                                         const __grid_constant__ PackRows pack, int ctas) {
     __shared__ uint32_t s_max[8];
     constexpr int RPB = THREADS / TPR;
     const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
     grid_dependency_wait();
     grid_launch_dependents();
-    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
+    if ((int)blockIdx.x >= ctas) {
+        pack_rows_part<uint8_t>(pack, blockIdx.x - ctas, gridDim.x - ctas, THREADS);
+        return;
+    }
+    for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)ctas * RPB) {
         const long long r = r0 + sub;
         const bool live = r < rows;
         const uint16_t* row = x + (live ? r : 0) * x_stride;
@@ -75,21 +80,22 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __r
 
 template <int TPR, int KEEP, int THREADS>
 static int quant_launch(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride,
-                        int bf16, bool vec, bool qvec, cudaStream_t st) {
+                        int bf16, bool vec, bool qvec, const PackRows* pack, cudaStream_t st) {
     int sms = 0;
     int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
     const int64_t blocks = (rows + THREADS / TPR - 1) / (THREADS / TPR);
-    const unsigned grid = (unsigned)(blocks < 2048 / THREADS * sms ? blocks : 2048 / THREADS * sms);
+    const int grid = (int)(blocks < 2048 / THREADS * sms ? blocks : 2048 / THREADS * sms);
+    const int more = pack ? pack_ctas(*pack, 1, sms) * (256 / THREADS) : 0;
     auto* k = vec ? (qvec ? quant_rows_kernel<TPR, KEEP, true, true, THREADS> : quant_rows_kernel<TPR, KEEP, true, false, THREADS>)
                   : (qvec ? quant_rows_kernel<TPR, KEEP, false, true, THREADS> : quant_rows_kernel<TPR, KEEP, false, false, THREADS>);
-    KDW_CUDA(launch_overlapping_previous(k, grid, (unsigned)THREADS, st, (const uint16_t*)x, (int8_t*)q, scale, (long long)rows, (int)cols,
-                                         (long long)x_stride, (long long)q_stride, bf16));
+    KDW_CUDA(launch_overlapping_previous(k, (unsigned)(grid + more), (unsigned)THREADS, st, (const uint16_t*)x, (int8_t*)q, scale, (long long)rows, (int)cols,
+                                         (long long)x_stride, (long long)q_stride, bf16, pack ? *pack : PackRows{}, grid));
     return 0;
 }
 
 int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride, int bf16,
-               bool q_padded, cudaStream_t st) {
+               bool q_padded, const PackRows* pack, cudaStream_t st) {
     const bool vec = ((uintptr_t)x & 15) == 0 && x_stride % 8 == 0 && cols % 8 == 0;
     // a last piece may run into the padding of its row, but not into the next row
     const bool qvec = ((uintptr_t)q & 7) == 0 && q_stride % 8 == 0 && (cols % 8 == 0 || q_padded);
@@ -98,7 +104,7 @@ int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols,
     if (rc) return rc;
     auto go = [&](auto tpr, auto keep, auto threads) {
         return quant_launch<decltype(tpr)::value, decltype(keep)::value, decltype(threads)::value>(
-            x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, st);
+            x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, pack, st);
     };
     using std::integral_constant;
     const integral_constant<int, 1> k1;
@@ -139,5 +145,5 @@ extern "C" int kdw_quant_rows(const void* x, int8_t* q, float* scale, int64_t ro
         set_error("quant_rows: a pointer is not aligned to its elements");
         return KDW_ERR_ALIGN;
     }
-    return quant_rows(x, q, scale, rows, cols, x_stride, cols, dtype == KDW_BF16, false, (cudaStream_t)stream);
+    return quant_rows(x, q, scale, rows, cols, x_stride, cols, dtype == KDW_BF16, false, nullptr, (cudaStream_t)stream);
 }

@@ -63,6 +63,14 @@ def _product_workspace(device, op, a_align, b_align, T, E, K, N, sa, sb, dtype):
 
 
 @functools.lru_cache(maxsize=4096)
+def _grads_workspace(device, x_align, w_align, g_align, has_ends, T, E, K, N, sx, sg, dtype):
+    n = _lib.load().kdw_linear_grads_f16_workspace_bytes(4096 + x_align, 4096 + w_align, 4096 + g_align, has_ends, T, E, K, N, sx, sg, dtype)
+    if n < 0:
+        _lib.check(int(n))
+    return n
+
+
+@functools.lru_cache(maxsize=4096)
 def _int8_workspace(device, x_align, w_align, T, E, K, N, sx, x_type, dtype):
     n = _lib.load().kdw_linear_i8_workspace_bytes(4096 + x_align, 4096 + w_align, T, E, K, N, sx, x_type, dtype)
     if n < 0:
@@ -88,6 +96,25 @@ def product(op, a, b, out, ends, T, E, K, N):
     if rc:
         _lib.check(rc)
     return out
+
+
+def grads(x, weight, grad, dx, dw, ends, T, E, K, N):
+    """Enqueues both gradients of a forward product on x's device / current stream."""
+    device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
+            return grads(x, weight, grad, dx, dw, ends, T, E, K, N)
+    dtype = TYPES[x.dtype]
+    sx, sg = row_stride(x), row_stride(grad)
+    px, pw, pg = x.data_ptr(), weight.data_ptr(), grad.data_ptr()
+    nbytes = _grads_workspace(device.index, px & 15, pw & 15, pg & 15, ends is not None, T, E, K, N, sx, sg, dtype)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = _lib.load().kdw_linear_grads_f16(
+        px, pw, pg, dx.data_ptr(), dw.data_ptr(), None if ends is None else ends.data_ptr(),
+        ws.data_ptr() if nbytes else None, nbytes, T, E, K, N, sx, sg, dtype, _raw_stream(device.index),
+    )
+    if rc:
+        _lib.check(rc)
 
 
 def int8_product(x, x_scale, weight, w_scale, y, ends, T, E, K, N):

@@ -86,16 +86,15 @@ def grouped_linear_grads(x, weight, grad, ends, need_x, need_w):
     E, N, K = weight.shape if weight.ndim == 3 else (1, *weight.shape)
     xr, gr = _launch.as_rows(x, 'x'), _launch.as_rows(grad, 'grad')
     T = xr.shape[0]
-    dx = dw = None
-    if need_x:
-        dx = gr.new_empty((T, K))
-        if T:
-            _launch.product(_launch.DGRAD, gr, weight, dx, ends, T, E, K, N)
-        dx = _launch.like_rows(dx, x)
-    if need_w:
-        dw = torch.empty_like(weight)
-        if T:
-            _launch.product(_launch.WGRAD, gr, xr, dw, ends, T, E, K, N)
-        else:
+    dx = gr.new_empty((T, K)) if need_x else None
+    dw = torch.empty_like(weight) if need_w else None
+    if T == 0:
+        if need_w:
             dw.zero_()
-    return dx, dw
+    elif need_x and need_w:
+        _launch.grads(xr, weight, gr, dx, dw, ends, T, E, K, N)
+    elif need_x:
+        _launch.product(_launch.DGRAD, gr, weight, dx, ends, T, E, K, N)
+    elif need_w:
+        _launch.product(_launch.WGRAD, gr, xr, dw, ends, T, E, K, N)
+    return _launch.like_rows(dx, x) if need_x else None, dw

@@ -305,6 +305,32 @@ def test_capture_and_replay():
             assert torch.equal(dw, ref.wgrad(x, g, ends).half())
 
 
+@pytest.mark.parametrize('T,K,N,ends', [
+    (1, 5, 3, None), (40, 8, 8, None), (300, 37, 64, None), (300, 64, 37, [10, 10, 290]), (9000, 24, 8, None), (9000, 24, 8, [8990]),
+    (2000, 512, 264, [700, 1500]), (20000, 72, 130, None), (60, 4096, 520, [0, 60]), (8192, 8, 128, None),
+])
+@pytest.mark.parametrize('offset,extra', [(0, 0), (8, 8), (3, 5)])
+def test_both_gradients_of_one_call(T, K, N, ends, offset, extra):
+    """One call for both gradients gives what the two operators give, from rows anywhere, and writes nothing else."""
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import _launch
+
+    spec, ends = ends, [T] if ends is None else ends
+    E, guard = len(ends), 1024
+    e = None if spec is None else ref.tensor_ends(ends)
+    x, g = (torch.as_strided(ref.integers((T * (c + extra) + offset,), torch.float16, i, top=1), (T, c), (c + extra, 1), offset)
+            for i, c in enumerate((K, N)))
+    w = ref.integers((E, N, K), torch.float16, 3, top=1)
+    for shift in (0, 1):
+        bx, bw = (torch.full((n + 2 * guard,), 7.0, dtype=torch.float16, device='cuda') for n in (T * K, E * N * K))
+        dx, dw = bx[guard + shift:guard + shift + T * K].view(T, K), bw[guard + shift:guard + shift + E * N * K].view(E, N, K)
+        _launch.grads(x, w, g, dx, dw, e, T, E, K, N)
+        assert torch.equal(dx, ref.dgrad(g, w, ends).half()) and torch.equal(dw, ref.wgrad(x, g, ends).half())
+        for b, n in ((bx, T * K), (bw, E * N * K)):
+            assert (b[:guard + shift] == 7).all() and (b[guard + shift + n:] == 7).all()
+    assert _lib.device_status() == 0
+
+
 def test_a_training_step_is_captured():
     """Forward and backward in a graph, the first calls of this kind in the autograd thread among them."""
     from kerops_b200.autograd import grouped_linear

@@ -79,6 +79,17 @@ def test_c_entry_points_refuse_bad_arguments(kdw_lib):
         assert call(**kw) == -1, kw
     for kw in (dict(a=P + 1), dict(b=P + 1), dict(out=P + 1), dict(ends=P + 2)):
         assert call(**kw) == -2, kw
+    okg = dict(x=P, w=P, g=P, dx=P, dw=P, ends=P, ws=None, nb=0, T=400, E=2, K=9, N=8, sx=9, sg=8, dt=0)
+
+    def callg(**kw):
+        return kdw_lib.kdw_linear_grads_f16(*{**okg, **kw}.values(), None)
+
+    for kw in (dict(x=None), dict(w=None), dict(g=None), dict(dx=None), dict(dw=None), dict(ends=None), dict(T=0), dict(sx=8), dict(sg=7),
+               dict(dt=2), dict(E=1025)):
+        assert callg(**kw) == -1, kw
+    for kw in (dict(x=P + 1), dict(w=P + 1), dict(g=P + 1), dict(dx=P + 1), dict(dw=P + 1), dict(ends=P + 1)):
+        assert callg(**kw) == -2, kw
+    assert callg() == -3 and b'workspace' in kdw_lib.kdw_last_error()  # rows of nine values are copied into it
     ok8 = dict(x=P, xs=P, w=P, ws=P, y=P, ends=P, wsp=None, nb=0, T=4, E=2, K=16, N=8, sx=16, xt=2, dt=0)
 
     def call8(**kw):
