@@ -398,10 +398,11 @@ int64_t kdw_linear_grads_f16_workspace_bytes(const void* x, const void* w, const
     const int32_t any = 0;
     d.ends = g.ends = has_ends ? &any : nullptr;
     int64_t bytes = 0;
-    for (const LinArgs* a : {&d, &g})
+    if (!rc && is_narrow_grads(d, g)) rc = linear_narrow_grads(d, g, nullptr, 0, &bytes, nullptr);
+    for (const LinArgs* a : {&d, &g})  // (these too: an unaligned dx takes them)
         if (!rc && !is_narrow(*a)) {
             rc = linear_plan(&pl, *a, sms);
-            bytes = std::max(bytes, rc ? 0 : pl.bytes);
+            bytes = std::max<int64_t>(bytes, rc ? 0 : pl.bytes);
         }
     return rc ? (rc < 0 ? rc : -rc) : l.off_rest + bytes;
 }
@@ -443,6 +444,10 @@ int kdw_linear_grads_f16(const void* x, const void* w, const void* grad, void* d
     d.ends = g.ends = ends;
     // the second product's kernels touch the workspace only when the first one's have completed
     ws = ws ? ws + l.off_rest : ws;
+    if (is_narrow_grads(d, g) && ((uintptr_t)dx & 15) == 0) {
+        int64_t need = 0;
+        return linear_narrow_grads(d, g, ws, ws ? workspace_bytes - l.off_rest : 0, &need, (cudaStream_t)stream);
+    }
     rc = is_narrow(d) && ((uintptr_t)dx & 15) == 0 ? linear_narrow(d, (cudaStream_t)stream)
                                                    : plan_and_run(&d, ws, workspace_bytes - l.off_rest, stream);
     return rc ? rc : plan_and_run(&g, ws, workspace_bytes - l.off_rest, stream);

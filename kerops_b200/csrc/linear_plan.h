@@ -45,6 +45,9 @@ int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
 // Products of many rows with one narrow weight matrix, without a workspace (linear_narrow.cu).
 bool is_narrow(const LinArgs& a);
 int linear_narrow(const LinArgs& a, cudaStream_t st);
+// Both gradients in one pass; `need`: the workspace.  Without g.out (the weight gradient) it only says what it needs.
+bool is_narrow_grads(const LinArgs& d, const LinArgs& g);
+int linear_narrow_grads(const LinArgs& d, const LinArgs& g, void* ws, int64_t ws_bytes, int64_t* need, cudaStream_t st);
 
 // Rows to copy to a pitch of 16 bytes, because TMA cannot address them where they are; strides in elements.
 struct PackRows {

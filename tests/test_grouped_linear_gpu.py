@@ -89,6 +89,36 @@ def test_one_narrow_group_that_ends_before_the_last_row(T, K, N):
     _check(T, K, N, [T - 70], torch.bfloat16)
 
 
+def test_one_pass_gradients_keep_rows_apart_and_repeat():
+    """NaN and infinities in rows of no group reach nothing, in a row of the group its own dx and dw; same bits every call."""
+    from kerops_b200.ops.linear import _launch
+
+    T, K, N = 40000, 32, 64
+    x, g, w = ref.integers((T, K), torch.bfloat16, 1), ref.integers((T, N), torch.bfloat16, 2), ref.integers((1, N, K), torch.bfloat16, 3)
+    e = ref.tensor_ends([T - 100])
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    want = ref.dgrad(g, w, [T - 100]).bfloat16(), ref.wgrad(x, g, [T - 100]).bfloat16()
+    x[T - 100:], g[T - 100:] = float('nan'), float('inf')
+    _launch.grads(x, w, g, dx, dw, e, T, 1, K, N)
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    g[777, 5] = float('nan')
+    _launch.grads(x, w, g, dx, dw, e, T, 1, K, N)
+    rows, outs = torch.arange(T, device='cuda') != 777, torch.arange(N, device='cuda') != 5
+    assert torch.equal(dx[rows], want[0][rows]) and torch.isnan(dx[777]).all()
+    assert torch.equal(dw[:, outs], want[1][:, outs]) and torch.isnan(dw[:, 5]).all()
+    x, g = torch.randn(T, K, device='cuda').bfloat16(), torch.randn(T, N, device='cuda').bfloat16()
+    first = None
+    for _ in range(3):
+        _launch.grads(x, w, g, dx, dw, e, T, 1, K, N)
+        first = first or (dx.clone(), dw.clone())
+        assert torch.equal(dx, first[0]) and torch.equal(dw, first[1])
+    # half a step of bf16: values in [2^e, 2^(e+1)) lie 2^(e-7) apart (8 significant bits), so a rounding is off by at most
+    # 2^(e-8) <= 2^-8 of the value; and a step of fp32 of the magnitudes for each of the n additions
+    for got, f, args, n in ((dx, ref.dgrad, (g, w), N), (dw, ref.wgrad, (x, g), T)):
+        full, size = f(*args, [T - 100]), f(*(a.abs() for a in args), [T - 100])
+        assert ((got.double() - full).abs() <= 2.0 ** -8 * full.abs() + n * 2.0 ** -23 * size).all()
+
+
 def test_folded_rows_do_not_mix():
     """A NaN in one voxel stays with its own products: the blocks that pair neighbouring voxels are not summed."""
     from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
@@ -308,6 +338,10 @@ def test_capture_and_replay():
 @pytest.mark.parametrize('T,K,N,ends', [
     (1, 5, 3, None), (40, 8, 8, None), (300, 37, 64, None), (300, 64, 37, [10, 10, 290]), (9000, 24, 8, None), (9000, 24, 8, [8990]),
     (2000, 512, 264, [700, 1500]), (20000, 72, 130, None), (60, 4096, 520, [0, 60]), (8192, 8, 128, None),
+    # one pass over rows and gradients: every width of both
+    *[(32768 + 37 * i, K, N, None) for i, (K, N) in enumerate((K, N) for K in (8, 16, 24, 64, 104) for N in (8, 16, 32, 40, 128)
+                                                             if K * N <= 2048)],
+    (40000, 32, 64, [39987]), (40000, 64, 32, [0]),
 ])
 @pytest.mark.parametrize('offset,extra', [(0, 0), (8, 8), (3, 5)])
 def test_both_gradients_of_one_call(T, K, N, ends, offset, extra):
