@@ -50,6 +50,7 @@ struct LinParams {
     int* status;
     unsigned long long limit_ns;
     int stop_after;
+    int early;              // row products: the kernel before this one wrote the rows and their scales only (see linear_kernel)
 };
 
 // First row and first unit of every group (one entry more than there are groups).

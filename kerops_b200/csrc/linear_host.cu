@@ -506,6 +506,7 @@ int kdw_linear_i8(const void* x, const float* x_scale, const int8_t* w, const fl
                         l.pack_w ? &pack : nullptr, (cudaStream_t)stream);
         if (rc) return rc;
         if (l.pack_w) args.b = ws + l.off_w;
+        args.rows_fresh = !l.pack_w;
         ws += l.off_rest;
     }
     if (is_few(args)) return linear_few(args, KDW_I8, (cudaStream_t)stream);

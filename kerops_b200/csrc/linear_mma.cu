@@ -116,24 +116,25 @@ struct LinLoad {
         b_boxes = C::WGRAD ? boxes_inside(p.out_cols - t0, C::LOAD_N) : 1;
         bytes = (C::A_ACROSS ? a_boxes * 8192 : C::A_BYTES) + (C::WGRAD ? b_boxes * 8192 : C::B_BYTES);
     }
-    __device__ __forceinline__ void load(const CUtensorMap* ma, const CUtensorMap* mb, int k, uint32_t a, uint32_t b,
-                                         uint32_t bar) const {
+    __device__ __forceinline__ void load_a(const CUtensorMap* ma, int k, uint32_t a, uint32_t bar) const {
         if constexpr (C::WGRAD) {
-            const int r = k_row + k * 64;
 #pragma unroll
             for (int j = 0; j < kLinTileM / 64; ++j)
-                if (j < a_boxes) tma_load_2d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, r);
+                if (j < a_boxes) tma_load_2d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, k_row + k * 64);
+        } else if constexpr (C::A_ACROSS) {
+#pragma unroll
+            for (int j = 0; j < kLinTileM / 64; ++j)
+                if (j < a_boxes) tma_load_3d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, k * 64, g);
+        } else {
+            tma_load_3d<C::PAIR>(a, ma, bar, k * C::K_ELEMS, c0, g);
+        }
+    }
+    __device__ __forceinline__ void load_b(const CUtensorMap* mb, int k, uint32_t b, uint32_t bar) const {
+        if constexpr (C::WGRAD) {
 #pragma unroll
             for (int j = 0; j < C::LOAD_N / 64; ++j)
-                if (j < b_boxes) tma_load_2d<C::PAIR>(b + j * 8192, mb, bar, t0 + j * 64, r);
+                if (j < b_boxes) tma_load_2d<C::PAIR>(b + j * 8192, mb, bar, t0 + j * 64, k_row + k * 64);
         } else {
-            if constexpr (C::A_ACROSS) {
-#pragma unroll
-                for (int j = 0; j < kLinTileM / 64; ++j)
-                    if (j < a_boxes) tma_load_3d<C::PAIR>(a + j * 8192, ma, bar, c0 + j * 64, k * 64, g);
-            } else {
-                tma_load_3d<C::PAIR>(a, ma, bar, k * C::K_ELEMS, c0, g);
-            }
             tma_load_2d<C::PAIR>(b, mb, bar, k * C::K_ELEMS, t0);
         }
     }
@@ -258,9 +259,15 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     } else if (warp == 1) {
         tmem_alloc<C::PAIR>(smem_u32(s_tmem), C::TMEM_COLS);
     }
-    // operands, scales and `ends` may be the work of the kernel before this one
-    grid_dependency_wait();
-    grid_launch_dependents();
+    // Operands, scales and `ends` may be the work of the kernel before this one.  EARLY: that kernel is this call's own (it
+    // quantises the rows), and it let this one start only after its own wait, so whatever came before it has completed: only
+    // the rows and their scales have to be waited for, and the first weights are loaded while they are being made (64 rows,
+    // 4096 -> 8192: 12.0 us instead of 12.9, 4096 rows of 32 groups, 1024 -> 2048: 24.4 instead of 25.1).
+    const bool early = !C::WGRAD && p.early;
+    if (!early) {
+        grid_dependency_wait();
+        grid_launch_dependents();
+    }
     if (warp == 2) lin_build_table(p, tab->row, tab->unit, lane);
     tc_fence_before();
     __syncthreads();
@@ -275,9 +282,36 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         int loads = 0, stage = 0;
         uint32_t phase = 0;
         bool ok = true;
+        if (early && p.stop_after >= 0) grid_dependency_wait();
         while (ok && take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
             const LinLoad<C> l(p, w, rank);
-            for (int k = l.kb; k < l.ke; ++k) {
+            int ahead = 0;
+            if (early && loads == 0 && p.stop_after < 0) {
+                // the ring is empty: weights for all of it, then the wait, then the rows beside them
+                const int n = l.ke - l.kb < C::STAGES ? l.ke - l.kb : C::STAGES;
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1) grid_dependency_wait();
+                    if (elect_one())
+                        for (int i = 0; i < n; ++i) {
+                            const uint32_t a = smem_u32(base) + i * C::STAGE;
+                            const uint32_t bar = rank == 0 ? full + 8 * i : cluster_addr(full + 8 * i, leader);
+                            if (h == 1) {
+                                l.load_b(&map_b, l.kb + i, a + C::A_BYTES, bar);
+                                continue;
+                            }
+                            if (rank == 0)
+                                mbar_expect_tx(bar, l.bytes);
+                            else
+                                cluster_expect_tx(bar, l.bytes);
+                            l.load_a(&map_a, l.kb + i, a, bar);
+                        }
+                    __syncwarp();
+                }
+                loads = ahead = n;
+                stage = n == C::STAGES ? 0 : n;
+                phase = n == C::STAGES ? 1 : 0;
+            }
+            for (int k = l.kb + ahead; k < l.ke; ++k) {
                 if (p.stop_after >= 0 && loads >= p.stop_after) {
                     ok = false;
                     break;
@@ -299,7 +333,8 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         bar = cluster_addr(bar, leader);  // CTA 0 waits for the loads of both
                         cluster_expect_tx(bar, l.bytes);
                     }
-                    l.load(&map_a, &map_b, k, a, b, bar);
+                    l.load_a(&map_a, k, a, bar);
+                    l.load_b(&map_b, k, b, bar);
                 }
                 __syncwarp();
                 ++loads;
@@ -412,6 +447,10 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             if (!more) break;
         }
     } else if (warp == 3) {
+        if (early) {
+            grid_dependency_wait();
+            grid_launch_dependents();
+        }
         if (!C::WGRAD) clear_rows(p, tab->row[p.E], lane, 32);
         if (p.table && blockIdx.x == 0)
             for (int i = lane; i <= p.E; i += 32) {
@@ -421,6 +460,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     } else {
         const int q = warp & 3, turn = (warp - 4) >> 3, odd = (warp >> 2) & 1 ^ 1;
         char* const stg = staging + (warp - 4) * 1024;
+        if (early) grid_dependency_wait();
         int acc = 0, count = 0;  // accumulators used so far: the two groups of warps take them in turn
         uint32_t acc_phase = 0;
         while (take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
@@ -576,6 +616,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     tc_fence_after();
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
     if (shared_tile) {
+        if (early) grid_dependency_wait();  // (of the warps that have not waited)
         w = ring[0];
         if (w.u >= 0) {
             if (p.splits == 2)
@@ -794,6 +835,7 @@ int linear_run(const LinPlan& pl, const LinArgs& a, void* ws, cudaStream_t st) {
     const WaitTest wt = wait_test();
     p.limit_ns = wt.limit_ns;
     p.stop_after = wt.stop_after;
+    p.early = a.rows_fresh;
     // accumulator fp32 (1) or int32 (2); operands fp16 (0) / bf16 (1) / int8 (1); which run across the contraction; M
     const uint32_t fmt = pl.esize == 1 ? 1u : (uint32_t)a.in_bf16;
     p.idesc = (pl.esize == 1 ? 2u : 1u) << 4 | fmt << 7 | fmt << 10 | (uint32_t)(a.op != LIN_FWD) << 15 |

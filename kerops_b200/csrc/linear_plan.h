@@ -18,6 +18,7 @@ struct LinArgs {
     int esize;            // bytes of an operand element (2 or 1)
     int in_bf16, out_bf16;
     const float *row_scale, *col_scale;
+    int rows_fresh;       // 1: the kernel enqueued just before is this call's own and wrote the rows and row_scale only
 };
 
 struct LinPlan {
