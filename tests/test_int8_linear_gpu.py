@@ -243,3 +243,49 @@ def test_trained_in_16_bits_then_answering_in_8():
         slack = x[a:b].double().abs().sum(1, keepdim=True) * dw[e_] + dx[a:b] * w[e_].double().abs().sum(1) + 128 * dx[a:b] * dw[e_]
         assert ((y[a:b].double() - want[a:b]).abs() <= slack + (2.0 ** -8 + 2.0 ** -22) * (want[a:b].abs() + slack)).all()
     assert not y[90:].any()
+
+
+@pytest.mark.parametrize('T,K,N,E', [(8, 512, 256, 3), (64, 4096, 2048, 1), (200, 1024, 512, 40), (600, 512, 768, 1),
+                                     (777, 1001, 333, 2), (3000, 256, 1024, 5), (9000, 1024, 2048, 3)])
+def test_every_operand_made_by_the_call_before(T, K, N, E):
+    """Kernels start while the one before them still runs: a chain in which each call reads what the last ones wrote
+    (rows, weights, scales and row counts) gives the same bits as with a synchronisation behind every call, and as a
+    captured graph."""
+    from kerops_b200.ops.linear import GroupedLinear, Int8Linear, QuantRows
+
+    g = torch.Generator(device='cuda').manual_seed(T)
+    x0 = torch.randn(T, K, generator=g, device='cuda').bfloat16()
+    ws = [(torch.randn(E, N, K, generator=g, device='cuda') / K ** 0.5).bfloat16() for _ in range(3)]
+    back = (torch.randn(E, K, N, generator=g, device='cuda') / N ** 0.5).bfloat16()
+    counts = [torch.sort(torch.randint(0, T + 1, (E,), generator=g, device='cuda'))[0].int() for _ in range(3)]
+    counts = [torch.cat([c[:-1], torch.full_like(c[-1:], T)]) for c in counts]
+    e = torch.empty(E, dtype=torch.int32, device='cuda')
+
+    def chain(after):
+        x, out = x0, []
+        for i in range(6):
+            e.copy_(counts[i % 3])
+            after()
+            q, s = QuantRows(ws[i % 3])
+            after()
+            y = Int8Linear(x, q, s, e)
+            after()
+            x = GroupedLinear(y, back, e)
+            after()
+            out += [y, x]
+        return out
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        got = chain(lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(3):
+        for t in got:
+            t.fill_(float('nan'))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
