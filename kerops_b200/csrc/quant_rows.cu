@@ -17,8 +17,9 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int c, int cols) {
     return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
-// TPR threads to a row (a warp or the CTA), KEEP vectors of 8 values of a thread stay in registers between the two passes
-// over the row; what is longer is read again.  CTAs from `ctas` on copy weights instead.  VEC: rows of the input are 16-byte aligned, QVEC: rows of the output 8-byte.
+// TPR threads to a row (a part of a warp, a warp or the CTA), KEEP vectors of 8 values of a thread stay in registers between
+// the two passes over the row; what is longer is read again.  CTAs from `ctas` on copy weights instead.  VEC: rows of the
+// input are 16-byte aligned, QVEC: rows of the output 8-byte.
 template <int TPR, int KEEP, bool VEC, bool QVEC, int THREADS>
 __global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __restrict__ x, int8_t* __restrict__ q,
                                                          float* __restrict__ scale, long long rows, int cols,
@@ -47,7 +48,15 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __r
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) m = max_bits(keep[i], m);
         for (int c = (KEEP * TPR + t) * 8; live && c < cols; c += TPR * 8) m = max_bits(load8<VEC>(row, c, cols), m);
-        m = __reduce_max_sync(0xffffffffu, m);
+        if constexpr (TPR >= 32) {
+            m = __reduce_max_sync(0xffffffffu, m);
+        } else {
+#pragma unroll
+            for (int d = TPR / 2; d; d /= 2) {
+                const uint32_t o = __shfl_xor_sync(0xffffffffu, m, d);
+                m = o > m ? o : m;
+            }
+        }
         if (TPR > 32) {
             __syncthreads();
             if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
@@ -78,7 +87,8 @@ __global__ __launch_bounds__(THREADS) void quant_rows_kernel(const uint16_t* __r
     }
 }
 
-template <int TPR, int KEEP, int THREADS>
+// IN: 0 rows of any alignment, 1 only aligned ones, 2 only others.
+template <int TPR, int KEEP, int THREADS, int IN>
 static int quant_launch(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride, int64_t q_stride,
                         int bf16, bool vec, bool qvec, const PackRows* pack, cudaStream_t st) {
     int sms = 0;
@@ -87,8 +97,9 @@ static int quant_launch(const void* x, void* q, float* scale, int64_t rows, int6
     const int64_t blocks = (rows + THREADS / TPR - 1) / (THREADS / TPR);
     const int grid = (int)(blocks < 2048 / THREADS * sms ? blocks : 2048 / THREADS * sms);
     const int more = pack ? pack_ctas(*pack, 1, sms) * (256 / THREADS) : 0;
-    auto* k = vec ? (qvec ? quant_rows_kernel<TPR, KEEP, true, true, THREADS> : quant_rows_kernel<TPR, KEEP, true, false, THREADS>)
-                  : (qvec ? quant_rows_kernel<TPR, KEEP, false, true, THREADS> : quant_rows_kernel<TPR, KEEP, false, false, THREADS>);
+    constexpr bool V = IN != 2, S = IN == 1;  // what the two choices below stand for, where one of them is not made
+    auto* k = vec ? (qvec ? quant_rows_kernel<TPR, KEEP, V, true, THREADS> : quant_rows_kernel<TPR, KEEP, V, false, THREADS>)
+                  : (qvec ? quant_rows_kernel<TPR, KEEP, S, true, THREADS> : quant_rows_kernel<TPR, KEEP, S, false, THREADS>);
     KDW_CUDA(launch_overlapping_previous(k, (unsigned)(grid + more), (unsigned)THREADS, st, (const uint16_t*)x, (int8_t*)q, scale, (long long)rows, (int)cols,
                                          (long long)x_stride, (long long)q_stride, bf16, pack ? *pack : PackRows{}, grid));
     return 0;
@@ -102,13 +113,14 @@ int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols,
     int sms = 0;
     int rc = device_facts(nullptr, &sms);
     if (rc) return rc;
-    auto go = [&](auto tpr, auto keep, auto threads) {
-        return quant_launch<decltype(tpr)::value, decltype(keep)::value, decltype(threads)::value>(
+    auto go = [&](auto tpr, auto keep, auto threads, auto in) {
+        return quant_launch<decltype(tpr)::value, decltype(keep)::value, decltype(threads)::value, decltype(in)::value>(
             x, q, scale, rows, cols, x_stride, q_stride, bf16, vec, qvec, pack, st);
     };
     using std::integral_constant;
-    const integral_constant<int, 1> k1;
-    const integral_constant<int, 2> k2;
+    const integral_constant<int, 0> any;
+    const integral_constant<int, 1> k1, aligned;
+    const integral_constant<int, 2> k2, unaligned;
     const integral_constant<int, 4> k4;
     const integral_constant<int, 8> k8;
     const integral_constant<int, 16> k16;
@@ -118,13 +130,31 @@ int quant_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols,
     // A warp to a row needs no barrier, and no more registers than the row fills; with few rows, or rows that a warp cannot
     // keep, the CTA takes a row together.  bf16, us with a warp and with the CTA: 8192 x 4096 17.8 and 19.6 (0.86 and 0.79
     // of the measured bandwidth), 8192 x 1024 5.2 and 9.9, 500 x 4096 3.0 and 2.5.
-    if (cols > 4096) return go(wide, k4, wide);
-    if (rows < 8 * sms) return cols <= 1024 ? go(cta, k1, cta) : go(cta, k4, cta);
-    if (cols <= 256) return go(warp, k1, cta);
-    if (cols <= 512) return go(warp, k2, cta);
-    if (cols <= 1024) return go(warp, k4, cta);
-    if (cols <= 2048) return go(warp, k8, cta);
-    return go(warp, k16, cta);
+    if (cols > 4096) return go(wide, k4, wide, any);
+    if (rows < 8 * sms) return cols <= 1024 ? go(cta, k1, cta, any) : go(cta, k4, cta, any);
+    // Short rows: several to a warp, few lanes without a piece, and the more pieces a thread has on their way the better, as
+    // long as a row is still read in whole lines.  us with a warp to a row, and with the threads below: 15.68 M x 8 3122 and
+    // 114, 15.68 M x 32 3099 and 320, 8 M x 64 1621 and 273, 4 M x 128 840 and 283 (0.84 of the measured bandwidth), 2 M x 256
+    // 441 and 249, 1 M x 512 306 and 242 (0.97); 8192 x 1024 5.5 and 6.0, so 1024 keep the warp.
+    if (vec && cols <= 8) return go(k1, k1, cta, aligned);
+    if (vec && cols <= 16) return go(k1, k2, cta, aligned);
+    if (vec && cols <= 32) return go(k2, k2, cta, aligned);
+    if (vec && cols <= 64) return go(k2, k4, cta, aligned);
+    if (vec && cols <= 128) return go(k4, k4, cta, aligned);
+    if (vec && cols <= 256) return go(k4, k8, cta, aligned);
+    if (vec && cols <= 512) return go(k8, k8, cta, aligned);
+    // Unaligned ones are read value by value, where lanes side by side count more: 4 M x 100 1054 and 597 with one piece to a
+    // thread, 1241 with four.
+    if (cols <= 8) return go(k1, k1, cta, unaligned);
+    if (cols <= 16) return go(k2, k1, cta, unaligned);
+    if (cols <= 32) return go(k4, k1, cta, unaligned);
+    if (cols <= 64) return go(k8, k1, cta, unaligned);
+    if (cols <= 128) return go(k16, k1, cta, unaligned);
+    if (cols <= 256) return go(warp, k1, cta, unaligned);
+    if (cols <= 512) return go(warp, k2, cta, unaligned);
+    if (cols <= 1024) return go(warp, k4, cta, any);
+    if (cols <= 2048) return go(warp, k8, cta, any);
+    return go(warp, k16, cta, any);
 }
 
 }  // namespace kdw

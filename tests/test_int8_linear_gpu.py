@@ -289,3 +289,33 @@ def test_every_operand_made_by_the_call_before(T, K, N, E):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('T,K', [(2501, k) for k in (1, 7, 8, 9, 16, 24, 31, 32, 40, 63, 64, 100, 128, 129, 136, 200, 256, 257, 300,
+                                                     504, 512, 520, 1000, 1024, 1500, 2048, 4096)]
+                         + [(700001, 8), (400003, 16), (300007, 33), (330001, 64), (200003, 128)])
+def test_quant_many_rows(T, K, dtype):
+    """Every split of a row over threads: rows that end inside a CTA's share, rows of zeros, of a NaN, of an infinity among
+    others, rows of a wider matrix; and the product that quantises its rows itself."""
+    from kerops_b200.ops.linear import Int8Linear, QuantRows
+
+    g = torch.Generator(device='cuda').manual_seed(K)
+    x = torch.randn(T, K, generator=g, device='cuda').to(dtype)
+    x[::97] = 0
+    odd = torch.arange(5, T, 101, device='cuda')
+    good = torch.ones(T, dtype=torch.bool, device='cuda')
+    good[odd] = False
+    xr, sr = _quant(x)
+    x[odd, odd % K] = torch.where(odd % 2 == 0, float('nan'), float('-inf')).to(dtype)
+    xr[odd] = 0
+    for pad, first in ((0, 0), (8, 0), (11, 3)):
+        wide = torch.zeros(T, K + pad, dtype=dtype, device='cuda')
+        rows = wide[:, first:first + K]
+        rows.copy_(x)
+        q, s = QuantRows(rows)
+        assert torch.equal(q, xr) and torch.equal(s[good], sr[good]) and s[odd].isnan().all()
+    w, ws = QuantRows(torch.randn(24, K, generator=g, device='cuda').to(dtype)[None])
+    y = Int8Linear(x, w, ws)
+    want = Int8Linear(q, w, ws, x_scale=s, dtype=dtype)
+    assert torch.equal(y[good], want[good]) and y[odd].isnan().all()
