@@ -281,7 +281,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
 
     if (warp == 0) {
         int loads = 0, stage = 0;
-        uint32_t phase = 0;
+        uint32_t phase = 0, partly_stages = 0, partly_phase = 0;  // stages whose last load reported to `partly`, and its parity
         bool ok = true;
         if (early && p.stop_after >= 0) grid_dependency_wait();
         while (ok && take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
@@ -322,12 +322,15 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                     if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                     break;
                 }
+                const bool own = C::PAIR && C::WGRAD && rank != 0 && l.k_rows - k * 64 < 64;
+                partly_stages = own ? partly_stages | 1u << stage : partly_stages & ~(1u << stage);
+                partly_phase ^= (uint32_t)own << stage;
                 if (elect_one()) {
                     const uint32_t a = smem_u32(base) + stage * C::STAGE, b = a + C::A_BYTES;
                     uint32_t bar = full + 8 * stage;
                     if (rank == 0) {
                         mbar_expect_tx(bar, l.bytes);
-                    } else if (C::WGRAD && l.k_rows - k * 64 < 64) {
+                    } else if (own) {
                         bar = partly + 8 * stage;  // warp 1 clears the rows beyond the share first and then tells CTA 0
                         mbar_expect_tx(bar, l.bytes);
                     } else {
@@ -345,18 +348,24 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 }
             }
         }
-        // a CTA (a pair) leaves only when its last copies have landed
-        if (rank == 0) {
-            const int last = loads < C::STAGES ? loads : C::STAGES;
-            for (int i = 0; i < last; ++i) {
-                if (stage == 0) {
-                    stage = C::STAGES;
-                    phase ^= 1;
-                }
-                --stage;
-                if (!lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        // A CTA leaves only when its last copies have landed (CTA 1's report to CTA 0, but for blocks that its warp 1 clears in
+        // part) and when the products' reports on its stages have arrived, which CTA 0 sends to both CTAs of a pair.
+        bool used = true;
+        const int last = loads < C::STAGES ? loads : C::STAGES;
+        for (int i = 0; i < last; ++i) {
+            if (stage == 0) {
+                stage = C::STAGES;
+                phase ^= 1;
             }
+            --stage;
+            bool landed = true;
+            if (rank == 0)
+                landed = lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns);
+            else if (partly_stages >> stage & 1)
+                landed = lin_wait<C::PAIR>(partly + 8 * stage, partly_phase >> stage & 1 ^ 1, p.limit_ns);
+            used = used && landed && lin_wait<C::PAIR>(empty + 8 * stage, phase, p.limit_ns);
         }
+        if (!used) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         __syncwarp();
     } else if (warp == 1) {
         int stage = 0, acc = 0;
@@ -615,6 +624,8 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     __syncthreads();
     if (C::PAIR || shared_tile) cluster_sync();
     tc_fence_after();
+    // CTA 0's last report goes to both CTAs, and it has waited for its own: CTA 1 leaves when the other has arrived too
+    if (C::PAIR && rank != 0 && warp == 1 && !lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
     if (shared_tile) {
         if (early) grid_dependency_wait();  // (of the warps that have not waited)
