@@ -259,8 +259,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrivals on another CTA's barrier.  Only the first makes this thread's writes to memory visible to the CTA that waits
-// (a fence of some 1500 cycles); the second follows tensor-memory loads, which tcgen05.fence orders, the third announces
+// Arrivals on another CTA's barrier.  Only the first makes this thread's writes to memory visible to the CTA that waits by
+// cluster_wait_bounded (a fence of some 1500 cycles); the second follows tensor-memory loads, which tcgen05.fence orders, the third announces
 // bytes and has nothing to make visible.
 __device__ __forceinline__ void cluster_release_arrive(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
@@ -272,26 +272,22 @@ __device__ __forceinline__ void cluster_expect_tx(uint32_t cluster_bar, uint32_t
     asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
                  : "memory");
 }
-// Bounded wait like mbar_wait_bounded; PAIR: also orders what the other CTA of the pair did before it arrived.
-template <bool PAIR>
-__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
-    if constexpr (true) {
-        return mbar_wait_bounded(bar, parity, limit_ns);
-    } else {
-        unsigned long long t0 = 0;
-        for (uint32_t it = 0;; ++it) {
-            uint32_t ok;
-            asm volatile(
-                "{\n\t.reg .pred p;\n\t"
-                "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-                "selp.u32 %0, 1, 0, p;\n\t}"
-                : "=r"(ok)
-                : "r"(bar), "r"(parity)
-                : "memory");
-            if (ok) return true;
-            if (it == 0) t0 = global_ns();
-            if ((it & 63u) == 63u && global_ns() - t0 > limit_ns) return false;
-        }
+// Bounded wait like mbar_wait_bounded that also makes visible what threads of other CTAs of the cluster wrote before a
+// cluster_release_arrive on this barrier.
+__device__ __forceinline__ bool cluster_wait_bounded(uint32_t bar, uint32_t parity, unsigned long long limit_ns) {
+    unsigned long long t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (it == 0) t0 = global_ns();
+        if ((it & 63u) == 63u && global_ns() - t0 > limit_ns) return false;
     }
 }
 

@@ -317,7 +317,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                     ok = false;
                     break;
                 }
-                ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(empty + 8 * stage, phase ^ 1, p.limit_ns));
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + 8 * stage, phase ^ 1, p.limit_ns));
                 if (!ok) {
                     if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                     break;
@@ -360,10 +360,10 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
             --stage;
             bool landed = true;
             if (rank == 0)
-                landed = lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns);
+                landed = mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns);
             else if (partly_stages >> stage & 1)
-                landed = lin_wait<C::PAIR>(partly + 8 * stage, partly_phase >> stage & 1 ^ 1, p.limit_ns);
-            used = used && landed && lin_wait<C::PAIR>(empty + 8 * stage, phase, p.limit_ns);
+                landed = mbar_wait_bounded(partly + 8 * stage, partly_phase >> stage & 1 ^ 1, p.limit_ns);
+            used = used && landed && mbar_wait_bounded(empty + 8 * stage, phase, p.limit_ns);
         }
         if (!used) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         __syncwarp();
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         while (ok && take_unit(w, ring, unit_full, unit_empty, slot, slot_phase, C::UNITS, lane, p)) {
             if (w.kb == w.ke) continue;
             if (rank == 0) {
-                ok = __all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(acc_empty + 8 * acc, acc_phase ^ 1, p.limit_ns));
                 if (!ok) break;
                 tc_fence_after();
             }
@@ -385,8 +385,10 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 // one of the factors is a NaN or an infinity, so both operands are cleared
                 const int valid = C::WGRAD ? w.k_rows - k * 64 : 64;
                 if (rank == 0 || valid < 64) {
-                    ok = rank == 0 ? lin_wait<C::PAIR>(full + 8 * stage, phase, p.limit_ns)
-                                   : lin_wait<C::PAIR>(partly + 8 * stage, partly_phase >> stage & 1, p.limit_ns);
+                    // (CTA 0 also waits for what CTA 1 cleared: ordinary writes that the products are to read)
+                    ok = rank != 0 ? mbar_wait_bounded(partly + 8 * stage, partly_phase >> stage & 1, p.limit_ns)
+                         : C::PAIR && valid < 64 ? cluster_wait_bounded(full + 8 * stage, phase, p.limit_ns)
+                                                 : mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
         // products in flight still read shared memory and write tensor memory
         if (rank == 0) {
             tc_commit<C::PAIR>(elect_one(), drain, both);
-            if (!lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+            if (!mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 continue;
             }
             if (any) {
-                if (!__all_sync(0xffffffffu, lin_wait<C::PAIR>(acc_full + 8 * acc, acc_phase, p.limit_ns))) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(acc_full + 8 * acc, acc_phase, p.limit_ns))) {
                     if (lane == 0) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
                     break;
                 }
@@ -625,7 +627,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     if (C::PAIR || shared_tile) cluster_sync();
     tc_fence_after();
     // CTA 0's last report goes to both CTAs, and it has waited for its own: CTA 1 leaves when the other has arrived too
-    if (C::PAIR && rank != 0 && warp == 1 && !lin_wait<C::PAIR>(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+    if (C::PAIR && rank != 0 && warp == 1 && !mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
     if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
     if (shared_tile) {
         if (early) grid_dependency_wait();  // (of the warps that have not waited)

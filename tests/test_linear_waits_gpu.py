@@ -78,3 +78,24 @@ def test_waits_that_run_out_are_reported_and_leave_the_context_usable(kdw_lib, o
         finally:
             kdw_lib.kdw_test_wait_limits(2_000_000_000, -1)
         assert torch.equal(call(), want) and _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('op,variant,T,E,K,N', [c for c in WAITS if c[0] == 2])
+def test_a_pair_keeps_other_groups_rows_out(op, variant, T, E, K, N):
+    """The last block of a group's rows reaches into the next group's: both CTAs of a pair clear those before the products
+    read them, so that a NaN or an infinity there reaches nothing.  Every second group, and the rows of no group, hold such."""
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import GroupedLinearWGRAD
+
+    ends = [T - 5] if E == 1 else [min(T - 5, (e + 1) * (T // E) + (1, 0, 2)[e % 3]) for e in range(E)]
+    x, g = ref.integers((T, K), torch.float16, 1, top=1), ref.integers((T, N), torch.float16, 2, top=1)
+    want = ref.wgrad(x, g, ends).half()
+    live = torch.zeros(T, dtype=torch.bool, device='cuda')
+    for a, b in ref.spans(ends, T)[::2]:
+        live[a:b] = True
+    x[~live], g[~live] = float('nan'), float('inf')
+    e = ref.tensor_ends(ends)
+    for _ in range(30):
+        got = GroupedLinearWGRAD(x, g, e).view(E, N, K)
+        assert torch.equal(got[::2], want[::2])
+    assert _lib.device_status() == 0
