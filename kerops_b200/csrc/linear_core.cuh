@@ -88,6 +88,11 @@ __host__ __device__ __forceinline__ int lin_div(int n, int d) {
 #endif
 }
 
+// Bytes from the start of the output to a value of it; rows and columns may each number almost 2^31.
+__host__ __device__ __forceinline__ long long lin_out_offset(long long row, int col, int cols) {
+    return (row * cols + col) * 2;
+}
+
 __host__ __device__ __forceinline__ int lin_shares(const LinParams& p, int rows) {
     return p.wgrad && rows > p.chunk ? lin_div(rows - 1, p.chunk) + 1 : 1;
 }

@@ -518,7 +518,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 }
             } else if constexpr (C::WGRAD) {
                 // lanes are output rows, accumulator columns output columns
-                char* out = reinterpret_cast<char*>(p.out) + ((long long)w.g * p.out_rows + c0) * pitch;
+                char* out = reinterpret_cast<char*>(p.out) + lin_out_offset((long long)w.g * p.out_rows + c0, 0, p.out_cols);
                 const int rows = p.out_rows - c0;
 #pragma unroll 1
                 for (int n = 32 * odd; n < C::BN; n += 64) {
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                         cs[i] = c < cols ? __ldg(p.col_scale + (long long)w.g * p.out_cols + c0 + c) : 0.f;
                     }
                 }
-                char* out = reinterpret_cast<char*>(p.out) + (w.t0 + 32ll * odd) * pitch + c0 * 2;
+                char* out = reinterpret_cast<char*>(p.out) + lin_out_offset(w.t0 + 32ll * odd, c0, p.out_cols);
                 const uint32_t mat = smem_u32(stg) + staged(lane & 7, lane >> 3);
 #pragma unroll 1
                 for (int n = 32 * odd; n < w.rows; n += 64) {

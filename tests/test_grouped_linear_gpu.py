@@ -496,3 +496,32 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable():
         lib.kdw_test_wait_limits(2_000_000_000, -1)
     assert torch.equal(GroupedLinear(x, w), want[0]) and torch.equal(GroupedLinearWGRAD(x, g), want[1])
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('op', ['forward', 'input gradient', '8-bit'])
+def test_more_than_a_billion_channels(op):
+    """An output row of more than 2^31 bytes: 54 GB with the weights (8-bit: 54 GB)."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, Int8Linear
+
+    T, few, many, last = 17, 16 if op == '8-bit' else 8, 2 ** 30 + 136, 2 ** 20
+    torch.cuda.empty_cache()
+    x = ref.integers((T, few), torch.float16, 1)
+    if op == 'forward':
+        w = torch.zeros(many, few, dtype=torch.float16, device='cuda')
+        w[-last:] = ref.integers((last, few), torch.float16, 2)
+        y, want = GroupedLinear(x, w), ref.fwd(x, w[None, -last:], [T])
+    elif op == 'input gradient':
+        w = torch.zeros(few, many, dtype=torch.float16, device='cuda')
+        w[:, -last:] = ref.integers((few, last), torch.float16, 2)
+        y, want = GroupedLinearDGRAD(x, w), ref.dgrad(x, w[None, :, -last:], [T])
+    else:
+        w = torch.zeros(many, few, dtype=torch.int8, device='cuda')
+        w[-last:] = ref.integers((last, few), torch.int8, 2)
+        one = torch.ones(T, device='cuda')
+        y = Int8Linear(x.to(torch.int8), w, torch.ones(many, device='cuda'), x_scale=one, dtype=torch.float16)
+        want = ref.fwd(x, w[None, -last:], [T])
+    assert torch.equal(y[:, -last:], want.half())
+    del w
+    assert all(not torch.count_nonzero(row[:-last]) for row in y)
+    del y
+    torch.cuda.empty_cache()
