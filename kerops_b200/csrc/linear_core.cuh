@@ -14,6 +14,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <math.h>
 
 #include "kdw_common.cuh"
 #include "linear_plan.h"
@@ -92,6 +93,21 @@ __host__ __device__ __forceinline__ int lin_div(int n, int d) {
 __host__ __device__ __forceinline__ long long lin_out_offset(long long row, int col, int cols) {
     return (row * cols + col) * 2;
 }
+
+// sum * rs * cs of an 8-bit product: one rounding of the sum and of each factor.  The row's scale first, so that two small
+// scales do not underflow in a product of their own (the sum is a whole number: its product with one scale does not either).
+// A row's scale of 2^90 and more (values of bf16 rows beyond some 1e29) could take the first product out of fp32's range
+// where the result lies inside, so it is taken as rs 2^-32, which is exact, and the result is brought back: |sum| < 2^31
+// and rs 2^-32 < 2^96 stay inside, and no product comes near fp32's smallest (2^58 2^-149).
+struct RowScale {
+    float s, back;
+    __host__ __device__ __forceinline__ explicit RowScale(float rs) {
+        const bool large = fabsf(rs) >= 1.2379400392853803e27f;  // 2^90
+        s = large ? rs * 2.3283064365386963e-10f : rs;
+        back = large ? 4294967296.f : 1.f;
+    }
+    __host__ __device__ __forceinline__ float of(int sum, float cs) const { return (float)sum * s * cs * back; }
+};
 
 __host__ __device__ __forceinline__ int lin_shares(const LinParams& p, int rows) {
     return p.wgrad && rows > p.chunk ? lin_div(rows - 1, p.chunk) + 1 : 1;

@@ -289,7 +289,7 @@ __global__ __launch_bounds__(32 * WARPS, 2) void linear_few_kernel(const __grid_
                 int s = 0;
 #pragma unroll
                 for (int k = 0; k < KW; ++k) s += (int)s_sum[k][r][c];
-                v = (float)s * (QUANT ? s_scale[r] : __ldg(p.x_scale + t)) * __ldg(p.w_scale + (long long)g * p.N + n);
+                v = RowScale(QUANT ? s_scale[r] : __ldg(p.x_scale + t)).of(s, __ldg(p.w_scale + (long long)g * p.N + n));
             } else {
 #pragma unroll
                 for (int k = 0; k < KW; ++k) v += __uint_as_float(s_sum[k][r][c]);

@@ -183,7 +183,7 @@ __device__ __forceinline__ void add_parts(const LinParams& p, const LinUnit& w, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             f[e] = __uint_as_float(s[e]);
-            if (C::I8) f[e] = 4 * j + e < cols ? (float)(int)s[e] * __ldg(p.row_scale + w.t0 + 4 * j + e) * cs : 0.f;
+            if (C::I8) f[e] = 4 * j + e < cols ? RowScale(__ldg(p.row_scale + w.t0 + 4 * j + e)).of((int)s[e], cs) : 0.f;
         }
         const uint32_t lo = pack2(f[0], f[1], p.out_bf16), hi = pack2(f[2], f[3], p.out_bf16);
         if (C::WGRAD && p.out_vec) {
@@ -586,14 +586,13 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                             const int j = 2 * h + k;
                             float2 rs = make_float2(1.f, 1.f);
                             if constexpr (C::I8) rs = *reinterpret_cast<const float2*>(srs + 8 * j + 2 * (lane & 3));
+                            const RowScale ra(rs.x), rb(rs.y);
                             uint32_t o[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t a = v[16 * (i >> 1) + 4 * j + 2 * (i & 1)], b = v[16 * (i >> 1) + 4 * j + 2 * (i & 1) + 1];
                                 if constexpr (C::I8)
-                                    // one rounding of the exact sum and of each factor; the row's scale first, so that two
-                                    // small scales do not underflow in a product of their own
-                                    o[i] = pack2((float)(int)a * rs.x * cs[i], (float)(int)b * rs.y * cs[i], p.out_bf16);
+                                    o[i] = pack2(ra.of((int)a, cs[i]), rb.of((int)b, cs[i]), p.out_bf16);
                                 else
                                     o[i] = pack2(__uint_as_float(a), __uint_as_float(b), p.out_bf16);
                             }

@@ -319,3 +319,20 @@ def test_quant_many_rows(T, K, dtype):
     y = Int8Linear(x, w, ws)
     want = Int8Linear(q, w, ws, x_scale=s, dtype=dtype)
     assert torch.equal(y[good], want[good]) and y[odd].isnan().all()
+
+
+@pytest.mark.parametrize('T,K,N', [(3, 64, 24), (12, 64, 24), (300, 64, 24), (18, 10864, 24), (638, 24, 1116), (300, 512, 400)])
+def test_rows_of_large_values_do_not_overflow_on_their_way(T, K, N):
+    """bf16 rows reach 3e38: sum times row scale may lie outside fp32 where the result, after the channel's scale, is inside."""
+    from kerops_b200.ops.linear import Int8Linear, QuantRows
+
+    g = torch.Generator(device='cuda').manual_seed(K)
+    x = (torch.randn(T, K, generator=g, device='cuda') * 2.0 ** 120).bfloat16()
+    x[1::3] *= 2.0 ** -100
+    w, ws = QuantRows((torch.randn(1, N, K, generator=g, device='cuda') / (4 * K ** 0.5)).bfloat16())
+    q, s = QuantRows(x)
+    # exact sums; the scales (3 roundings of fp32) and the result (half a step of bf16, 2^-8) are rounded
+    want = ref.fwd(q, w, [T]) * s[:, None].double() * ws.double()
+    assert (s[0] * ref.fwd(q, w, [T])[0].abs().max().float()).isinf()  # the plain order's first product
+    for y in (Int8Linear(x, w, ws), Int8Linear(q, w, ws, x_scale=s, dtype=torch.bfloat16)):
+        assert ((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all()

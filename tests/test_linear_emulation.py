@@ -3,6 +3,7 @@ import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 from tests import conftest
@@ -21,6 +22,7 @@ def emu():
     lib = ctypes.CDLL(so)
     i64, ci = ctypes.c_int64, ctypes.c_int
     lib.emu_lin_out_offset.argtypes, lib.emu_lin_out_offset.restype = [i64, ci, ci], i64
+    lib.emu_scaled_sum.argtypes, lib.emu_scaled_sum.restype = [ci, ctypes.c_float, ctypes.c_float], ctypes.c_float
     return lib
 
 
@@ -30,3 +32,28 @@ def test_offsets_of_any_accepted_size(emu, cols):
     for row in (0, 1, 17, 2 ** 20, 2 ** 31 - 1026):
         for col in {0, cols // 2, max(0, cols - 32), cols - 1}:
             assert emu.emu_lin_out_offset(row, col, cols) == 2 * (row * cols + col)
+
+
+def test_a_sum_with_scales_of_any_size(emu):
+    """Three roundings of the exact product wherever it lies inside fp32's normal range, however large the row's scale or
+    small the channel's; and the plain sum * rs * cs to the bit wherever that does not overflow on its way."""
+    rng = np.random.default_rng(0)
+    f32 = np.float32
+    sums = [0, 1, -1, 127 * 127, -(2 ** 14) * 131071, *rng.integers(-2 ** 31 + 1, 2 ** 31, 40).tolist()]
+    row = [0.0, 1.0, 2.0 ** 90, np.nextafter(f32(2.0 ** 90), f32(0)), f32(3.4e38), f32(1e-38), f32(1e-44), -2.0 ** 100, *np.exp(rng.uniform(-85, 88, 40))]
+    col = [0.0, 1.0, f32(3.4e38), f32(1e-38), f32(1e-45), -1e-30, *np.exp(rng.uniform(-85, 88, 40))]
+    inside = 0
+    for s in sums:
+        for rs in map(f32, row):
+            for cs in map(f32, col):
+                got = f32(emu.emu_scaled_sum(s, rs, cs))
+                exact = float(s) * float(rs) * float(cs)
+                with np.errstate(all='ignore'):
+                    step = f32(s) * rs
+                    plain = step * cs
+                if np.isfinite(step):
+                    assert got == plain, (s, rs, cs)
+                if 2.0 ** -126 <= abs(exact) < 2.0 ** 127:
+                    inside += not np.isfinite(plain)
+                    assert abs(float(got) - exact) <= 3.1 * 2.0 ** -24 * abs(exact), (s, rs, cs)
+    assert inside > 100  # results that the plain order loses
