@@ -72,18 +72,27 @@ struct alignas(16) LinUnit {
     int unused;
 };
 
-// n / d for 0 <= n < 2^31, 0 < d: a quotient from the reciprocal in fp32, off by n 2^-21 / d at most, corrected twice.  A
-// tenth of the latency of the integer division, of which finding a unit needs several.
+// n / d for 0 <= n < 2^31, 0 < d < 2^31, from r = 1 / d, off by a unit of fp32's last place or less, and the rest of the
+// estimate, twice: the first estimate is off by n 2^-21 / d + 1 at most, the second by one.  A tenth of the latency of the
+// integer division, of which finding a unit needs several.
+__host__ __device__ __forceinline__ int lin_div_by(int n, int d, float r) {
+    const float f = (float)n * r;
+#ifdef __CUDA_ARCH__
+    int q = __float2int_rz(f);  // (the largest int where f is beyond it)
+#else
+    int q = f < 2147483648.f ? (int)f : 0x7fffffff;
+#endif
+    uint32_t rest = (uint32_t)n - (uint32_t)q * (uint32_t)d;  // modulo 2^32; the true rest is a signed one
+    const int fix = (int)floorf((float)(int)rest * r);
+    q += fix;
+    rest -= (uint32_t)fix * (uint32_t)d;
+    return q + ((int)rest >= d) - ((int)rest < 0);
+}
 __host__ __device__ __forceinline__ int lin_div(int n, int d) {
 #ifdef __CUDA_ARCH__
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((float)d));
-    int q = __float2int_rz((float)n * r);
-    int rest = n - q * d;  // may wrap where q is off by much: only its low bits count, the true rest fits
-    const int fix = __float2int_rd((float)rest * r);
-    q += fix;
-    rest -= fix * d;
-    return q + (rest >= d) - (rest < 0);
+    return lin_div_by(n, d, r);
 #else
     return n / d;
 #endif

@@ -23,6 +23,7 @@ def emu():
     i64, ci = ctypes.c_int64, ctypes.c_int
     lib.emu_lin_out_offset.argtypes, lib.emu_lin_out_offset.restype = [i64, ci, ci], i64
     lib.emu_scaled_sum.argtypes, lib.emu_scaled_sum.restype = [ci, ctypes.c_float, ctypes.c_float], ctypes.c_float
+    lib.emu_lin_div_misses.argtypes, lib.emu_lin_div_misses.restype = [ctypes.c_void_p, ctypes.c_void_p, i64, ci], i64
     return lib
 
 
@@ -57,3 +58,19 @@ def test_a_sum_with_scales_of_any_size(emu):
                     inside += not np.isfinite(plain)
                     assert abs(float(got) - exact) <= 3.1 * 2.0 ** -24 * abs(exact), (s, rs, cs)
     assert inside > 100  # results that the plain order loses
+
+
+@pytest.mark.parametrize('ulps', [-1, 0, 1])
+def test_division_by_a_reciprocal(emu, ulps):
+    """The quotient that finds units: exact for every pair, with the hardware's reciprocal off by up to its documented unit."""
+    rng, top = np.random.default_rng(ulps + 1), 2 ** 31 - 1
+    edges = np.unique(np.clip([v + k for e in range(32) for v in (2 ** e, 3 * 2 ** e // 2) for k in range(-2, 3)], 0, top))
+    pairs = [np.meshgrid(edges, edges[edges > 0])]
+    for hi in (100, 10 ** 4, 2 ** 20, 2 ** 24, top):
+        for dhi in (2, 17, 300, 5000, 2 ** 20, top):
+            n, d = rng.integers(0, hi, 100000), rng.integers(1, dhi, 100000)
+            pairs += [(n, d), (np.clip(n // d * d + rng.integers(-1, 2, n.shape), 0, top), d)]
+    pairs.append((np.full(100000, top), np.arange(1, 100001)))
+    for n, d in pairs:
+        n, d = (np.ascontiguousarray(np.ravel(a), np.int32) for a in (n, d))
+        assert emu.emu_lin_div_misses(n.ctypes.data, d.ctypes.data, len(n), ulps) == 0
