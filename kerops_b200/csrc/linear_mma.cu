@@ -348,24 +348,25 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
                 }
             }
         }
-        // A CTA leaves only when its last copies have landed (CTA 1's report to CTA 0, but for blocks that its warp 1 clears in
-        // part) and when the products' reports on its stages have arrived, which CTA 0 sends to both CTAs of a pair.
-        bool used = true;
+        // A CTA leaves only when its last copies have landed and the products' reports on its stages have arrived.  CTA 0 of a
+        // pair sends those to both CTAs and waits for its own last one in warp 1.  CTA 1's copies report to CTA 0, but for
+        // blocks that its warp 1 clears in part.
         const int last = loads < C::STAGES ? loads : C::STAGES;
+        bool ok_last = true;
         for (int i = 0; i < last; ++i) {
             if (stage == 0) {
                 stage = C::STAGES;
                 phase ^= 1;
             }
             --stage;
-            bool landed = true;
-            if (rank == 0)
-                landed = mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns);
-            else if (partly_stages >> stage & 1)
-                landed = mbar_wait_bounded(partly + 8 * stage, partly_phase >> stage & 1 ^ 1, p.limit_ns);
-            used = used && landed && mbar_wait_bounded(empty + 8 * stage, phase, p.limit_ns);
+            if (rank == 0) {
+                ok_last &= mbar_wait_bounded(full + 8 * stage, phase, p.limit_ns);
+            } else {
+                if (partly_stages >> stage & 1) ok_last &= mbar_wait_bounded(partly + 8 * stage, partly_phase >> stage & 1 ^ 1, p.limit_ns);
+                ok_last = ok_last && mbar_wait_bounded(empty + 8 * stage, phase, p.limit_ns);
+            }
         }
-        if (!used) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        if (!ok_last) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
         __syncwarp();
     } else if (warp == 1) {
         int stage = 0, acc = 0;
