@@ -5,7 +5,8 @@
 // contraction inside a fragment is free as long as both operands agree, so the four words of such a piece are, as they
 // come, the operands of two products.  The weights go from memory to registers to the tensor pipe, without shared memory;
 // the tensor pipe is idle almost always.  A CTA takes 16 output channels of one group and splits the contraction over its
-// four or eight warps in pieces of 64 bytes, so that the CTA reads runs of 256 or 512 bytes; the warps' sums are added in shared memory.
+// eight warps in pieces of 64 bytes, so that it reads runs of 512 bytes, or 32 channels with four warps to each half and runs
+// of 256 bytes; the warps' sums are added in shared memory.
 //
 // One row of 4096 x 4096 takes 7.6 us in bf16 and 4.4 us in 8 bits (0.68 and 0.59 of the measured bandwidth: some 2 us are
 // the launch, the first load's latency and the last sums), 8192 x 16384 in bf16 51 us (0.80).
@@ -318,11 +319,10 @@ static int few_launch(const FewParams& p, cudaStream_t st) {
     // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four (7.6 us
     // since a piece's successor is loaded as soon as it has been used).
     constexpr int U = (NT == 1 ? 8 : 4) / (VEC ? 1 : 4);
-    const long long ctas = (long long)((p.N + 15) / 16) * (p.ends ? (p.E < p.T ? p.E : p.T) : 1);
-    // 32 channels to a CTA where CTAs of 16 would not all be resident at once (two to an SM): 8 rows of 8 groups, 2048 ->
-    // 1024, 9.1 us instead of 10.3 (8.3 now that pieces run ahead); with fewer CTAs the contraction is better split further
-    // (4096 x 4096: 8.5 and 11.2 us, measured before that too).
-    if (ctas > 296) return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 32>(p, st);
+    int sms = 0;
+    int rc = device_facts(nullptr, &sms);
+    if (rc) return rc;
+    if (few_channels(p.N, p.ends ? (p.E < p.T ? p.E : p.T) : 1, sms) == 32) return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 32>(p, st);
     return few_warps<I8, BF16, QUANT, NT, VEC, 8, U, 16>(p, st);
 }
 template <bool I8, bool BF16, bool VEC>

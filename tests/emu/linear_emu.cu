@@ -18,3 +18,5 @@ extern "C" long long emu_lin_div_misses(const int* n, const int* d, long long co
     }
     return misses;
 }
+
+extern "C" int emu_few_channels(long long N, long long groups, int sms) { return few_channels(N, groups, sms); }

@@ -24,6 +24,7 @@ def emu():
     lib.emu_lin_out_offset.argtypes, lib.emu_lin_out_offset.restype = [i64, ci, ci], i64
     lib.emu_scaled_sum.argtypes, lib.emu_scaled_sum.restype = [ci, ctypes.c_float, ctypes.c_float], ctypes.c_float
     lib.emu_lin_div_misses.argtypes, lib.emu_lin_div_misses.restype = [ctypes.c_void_p, ctypes.c_void_p, i64, ci], i64
+    lib.emu_few_channels.argtypes = [i64, i64, ci]
     return lib
 
 
@@ -74,3 +75,12 @@ def test_division_by_a_reciprocal(emu, ulps):
     for n, d in pairs:
         n, d = (np.ascontiguousarray(np.ravel(a), np.int32) for a in (n, d))
         assert emu.emu_lin_div_misses(n.ctypes.data, d.ctypes.data, len(n), ulps) == 0
+
+
+@pytest.mark.parametrize('sms', [18, 74, 132, 148])
+def test_channels_of_a_few_rows_cta_follow_the_device(emu, sms):
+    """CTAs of 16 channels as long as two to an SM hold all of them, on a device (or a part of one) of any size."""
+    for groups in (1, 8, 16):
+        n = 2 * sms // groups * 16
+        assert emu.emu_few_channels(n, groups, sms) == 16 and emu.emu_few_channels(n + 1, groups, sms) == 32
+    assert emu.emu_few_channels(2 ** 31 - 1025, 1, sms) == 32
