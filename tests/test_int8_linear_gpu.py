@@ -336,3 +336,33 @@ def test_rows_of_large_values_do_not_overflow_on_their_way(T, K, N):
     assert (s[0] * ref.fwd(q, w, [T])[0].abs().max().float()).isinf()  # the plain order's first product
     for y in (Int8Linear(x, w, ws), Int8Linear(q, w, ws, x_scale=s, dtype=torch.bfloat16)):
         assert ((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -22) * want.abs()).all()
+
+
+@pytest.mark.parametrize('variant,T,E,K,N', [
+    (1128064, 17, 3, 32, 24), (1128128, 8484, 32, 32, 24), (1128256, 16926, 32, 32, 24), (1256256, 638, 8, 32, 11160),
+    (2128064, 18, 3, 2784, 24), (2128128, 4926, 1, 4240, 24), (2128256, 9872, 2, 4032, 24), (2256256, 4800, 8, 2768, 160),
+    (4128064, 17, 2, 2992, 24), (4128128, 1147, 32, 3968, 24), (4128256, 4105, 32, 4000, 24), (4256256, 2454, 2, 3936, 136),
+    (8128064, 18, 1, 10864, 24), (8128128, 700, 1, 16000, 136), (8128256, 567, 1, 19200, 504),
+])
+def test_every_variant_behind_its_own_quantiser(kdw_lib, variant, T, E, K, N):
+    """With 16-bit rows and aligned weights every tensor-core variant loads its weights while its rows are being quantised: the
+    same bits as from rows quantised before, with other operands' calls close behind."""
+    from kerops_b200 import _lib
+    from kerops_b200.ops.linear import Int8Linear, QuantRows
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sms != 148 or kdw_lib.kdw_linear_auto_variant(0, 2, T, E, K, N, sms) == variant
+    ends = ref.uneven_ends(T, E)
+    e = ref.tensor_ends(ends)
+    cases = []
+    for seed in (1, 2):
+        _, _, w, ws = _int8(1, K, N, E, seed)
+        x = torch.randn(T, K, generator=torch.Generator(device='cuda').manual_seed(seed), device='cuda').bfloat16()
+        q, s = QuantRows(x)
+        y = Int8Linear(q, w, ws, e, x_scale=s, dtype=torch.float16)
+        assert torch.equal(y, _product(q, s, w, ws, ends, torch.float16))
+        cases.append((x, w, ws, y))
+    for _ in range(5):
+        got = [Int8Linear(x, w, ws, e, dtype=torch.float16) for x, w, ws, _ in cases]
+        assert all(torch.equal(y, c[3]) for y, c in zip(got, cases))
+    assert _lib.device_status() == 0
