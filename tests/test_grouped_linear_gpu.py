@@ -525,3 +525,50 @@ def test_more_than_a_billion_channels(op):
     assert all(not torch.count_nonzero(row[:-last]) for row in y)
     del y
     torch.cuda.empty_cache()
+
+
+def _behind_zeros(shape, tail, dtype, seed):
+    """Zeros but for the last `tail` entries of the first dimension."""
+    t = torch.zeros(shape, dtype=dtype, device='cuda')
+    t[-tail:] = ref.integers((tail, *shape[1:]), dtype, seed)
+    return t
+
+
+def test_narrow_volumes_beyond_32_bits():
+    """More than 2^31 values a row operand, through the kernels of narrow weights and of both gradients in one pass."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD, _launch
+
+    T, K, N, tail = 70_000_011, 32, 32, 3000
+    x, w = _behind_zeros((T, K), tail, torch.float16, 1), ref.integers((N, K), torch.float16, 2)
+    for f, form in ((GroupedLinear, ref.fwd), (GroupedLinearDGRAD, ref.dgrad)):
+        y = f(x, w)
+        assert torch.equal(y[-tail:], form(x[-tail:], w[None], [tail]).half()) and not torch.count_nonzero(y[:-tail])
+        del y
+    want = ref.wgrad(x[-tail:], x[-tail:], [tail]).half()[0]
+    assert torch.equal(GroupedLinearWGRAD(x, x), want)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    _launch.grads(x, w, x, dx, dw, None, T, 1, K, N)
+    assert torch.equal(dw, want) and torch.equal(dx[-tail:], ref.dgrad(x[-tail:], w[None], [tail]).half())
+    assert not torch.count_nonzero(dx[:-tail])
+    del x, dx
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('T', [6, 40])
+def test_weights_beyond_32_bits(T):
+    """More than 2^31 weights, the rows in the last group: products of few rows and of tiles, and the weight gradient."""
+    from kerops_b200.ops.linear import GroupedLinear, GroupedLinearDGRAD, GroupedLinearWGRAD
+
+    E, N, K = 36, 8200, 7624
+    w = _behind_zeros((E, N, K), 1, torch.bfloat16, 1)
+    x, g = ref.integers((T, K), torch.bfloat16, 2), ref.integers((T, N), torch.bfloat16, 3)
+    ends = [0] * (E - 1) + [T - 1]
+    e = ref.tensor_ends(ends)
+    last = [T - 1]
+    assert torch.equal(GroupedLinear(x, w, e), ref.fwd(x, w[-1:], last).bfloat16())
+    assert torch.equal(GroupedLinearDGRAD(g, w, e), ref.dgrad(g, w[-1:], last).bfloat16())
+    del w
+    dw = GroupedLinearWGRAD(x, g, e)
+    assert torch.equal(dw[-1:], ref.wgrad(x, g, last).bfloat16()) and not any(torch.count_nonzero(d) for d in dw[:-1])
+    del dw
+    torch.cuda.empty_cache()

@@ -366,3 +366,32 @@ def test_every_variant_behind_its_own_quantiser(kdw_lib, variant, T, E, K, N):
         got = [Int8Linear(x, w, ws, e, dtype=torch.float16) for x, w, ws, _ in cases]
         assert all(torch.equal(y, c[3]) for y, c in zip(got, cases))
     assert _lib.device_status() == 0
+
+
+def test_rows_and_weights_beyond_32_bits():
+    """More than 2^31 values quantised, multiplied and written; more than 2^31 weights for few rows and for many."""
+    from kerops_b200.ops.linear import Int8Linear, QuantRows
+
+    T, K, N, tail = 17_000_100, 136, 136, 2000
+    x = torch.zeros(T, K, dtype=torch.float16, device='cuda')
+    x[-tail:] = torch.randn(tail, K, generator=torch.Generator(device='cuda').manual_seed(1), device='cuda').half()
+    w, ws = QuantRows(torch.randn(1, N, K, generator=torch.Generator(device='cuda').manual_seed(2), device='cuda').half())
+    qr, sr = _quant(x[-tail:])
+    want = _product(qr, sr, w, ws, [tail], torch.float16)
+    q, s = QuantRows(x)
+    assert torch.equal(q[-tail:], qr) and torch.equal(s[-tail:], sr) and not torch.count_nonzero(q[:-tail]) and not s[:-tail].any()
+    for y in (Int8Linear(q, w, ws, x_scale=s, dtype=torch.float16), Int8Linear(x, w, ws)):
+        assert torch.equal(y[-tail:], want) and not torch.count_nonzero(y[:-tail])
+    del x, q, y
+    torch.cuda.empty_cache()
+    E, N, K = 40, 8200, 7632
+    for T in (3, 12, 40):
+        x, xs, wl, ws = _int8(T, K, N, 1, T)
+        w = torch.zeros(E, N, K, dtype=torch.int8, device='cuda')
+        w[-1] = wl[0]
+        wide = torch.ones(E, N, device='cuda')
+        wide[-1] = ws[0]
+        y = Int8Linear(x, w, wide, ref.tensor_ends([0] * (E - 1) + [T]), x_scale=xs, dtype=torch.bfloat16)
+        assert torch.equal(y, _product(x, xs, wl, ws, [T], torch.bfloat16))
+        del w
+    torch.cuda.empty_cache()
