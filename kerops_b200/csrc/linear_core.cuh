@@ -69,7 +69,6 @@ struct alignas(16) LinUnit {
     int kb, ke;        // blocks of the contraction; weight gradient: blocks of 64 rows counted from k_row
     int k_row, k_rows; // weight gradient: first row and rows of the share (the last block may be partly beyond them)
     int whole;         // weight gradient: this unit is the only share of its tile
-    int unused;
 };
 
 // n / d for 0 <= n < 2^31, 0 < d < 2^31, from r = 1 / d, off by a unit of fp32's last place or less, and the rest of the
@@ -140,7 +139,6 @@ __host__ __device__ __forceinline__ LinUnit lin_unit(const LinParams& p, const i
     }
     LinUnit r;
     r.u = u;
-    r.unused = 0;
     r.g = lo;
     const int rows = row[lo + 1] - row[lo];
     const int nt = p.wgrad ? p.n_tiles : (rows + p.bn - 1) >> p.bn_log;

@@ -381,7 +381,7 @@ int kdw_linear_f16(int op, const void* a, const void* b, void* out, const int32_
     args.out = out;
     args.ends = ends;
     if (is_few(args)) return linear_few(args, dtype, (cudaStream_t)stream);
-    // 16-byte stores: an output that does not allow them takes the other path, whose workspace must then be given
+    // 16-byte stores: an output that does not allow them takes the other path, which copies nothing of operands like these
     if (is_narrow(args) && ((uintptr_t)out & 15) == 0) return linear_narrow(args, (cudaStream_t)stream);
     return plan_and_run(&args, workspace, workspace_bytes, stream);
 }
@@ -399,8 +399,8 @@ int64_t kdw_linear_grads_f16_workspace_bytes(const void* x, const void* w, const
     d.ends = g.ends = has_ends ? &any : nullptr;
     int64_t bytes = 0;
     if (!rc && is_narrow_grads(d, g)) rc = linear_narrow_grads(d, g, nullptr, 0, &bytes, nullptr);
-    for (const LinArgs* a : {&d, &g})  // (these too: an unaligned dx takes them)
-        if (!rc && !is_narrow(*a)) {
+    for (const LinArgs* a : {&d, &g})  // (also where both gradients go in one pass: an unaligned dx takes two products)
+        if (!rc && !is_narrow(*a)) {  // (a narrow product needs none on either path)
             rc = linear_plan(&pl, *a, sms);
             bytes = std::max<int64_t>(bytes, rc ? 0 : pl.bytes);
         }
