@@ -109,8 +109,9 @@ __host__ __device__ __forceinline__ long long lin_out_offset(long long row, int 
 // and rs 2^-32 < 2^96 stay inside, and no product comes near fp32's smallest (2^58 2^-149).
 struct RowScale {
     float s, back;
+    __host__ __device__ static __forceinline__ bool is_large(float rs) { return fabsf(rs) >= 1.2379400392853803e27f; }  // 2^90
     __host__ __device__ __forceinline__ explicit RowScale(float rs) {
-        const bool large = fabsf(rs) >= 1.2379400392853803e27f;  // 2^90
+        const bool large = is_large(rs);
         s = large ? rs * 2.3283064365386963e-10f : rs;
         back = large ? 4294967296.f : 1.f;
     }
