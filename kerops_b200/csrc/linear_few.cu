@@ -8,8 +8,8 @@
 // eight warps in pieces of 64 bytes, so that it reads runs of 512 bytes, or 32 channels with four warps to each half and runs
 // of 256 bytes; the warps' sums are added in shared memory.
 //
-// One row of 4096 x 4096 takes 7.6 us in bf16 and 4.4 us in 8 bits (0.68 and 0.59 of the measured bandwidth: some 2 us are
-// the launch, the first load's latency and the last sums), 8192 x 16384 in bf16 51 us (0.80).
+// One row of 4096 x 4096 takes 6.7 us in bf16 and 4.2-4.5 us in 8 bits, 5.1 with its quantisation (0.77 and 0.6 of the measured
+// bandwidth: some 2 us are the launch, the first load's latency and the last sums), 8192 x 16384 in bf16 48 us (0.86).
 //
 // 8-bit products of 16-bit rows: with at most eight rows every CTA quantises the rows it needs itself (they come from L2),
 // which is cheaper than a kernel in front.
@@ -316,8 +316,8 @@ static int few_warps(const FewParams& p, cudaStream_t st) {
 }
 template <bool I8, bool BF16, bool QUANT, int NT, bool VEC>
 static int few_launch(const FewParams& p, cudaStream_t st) {
-    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four (7.6 us
-    // since a piece's successor is loaded as soon as it has been used).
+    // Pieces in flight per lane and weight row.  One row of 4096 x 4096 in bf16: 8.2 us with eight, 10.5 us with four (6.7 us
+    // now that a piece's successor is loaded as soon as it has been used).
     constexpr int U = (NT == 1 ? 8 : 4) / (VEC ? 1 : 4);
     int sms = 0;
     int rc = device_facts(nullptr, &sms);

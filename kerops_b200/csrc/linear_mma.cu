@@ -27,10 +27,10 @@ namespace kdw {
 //         one CTA is bound by shared memory: 768 cycles to a stage where the products take 512).  CTA 0 waits for the
 //         loads of both and issues the products.
 // Large products are bound by the tensor cores (87 % of their cycles busy on 16384 rows of 8 groups, 2048 -> 4096): 18944 x
-// 4096 -> 2048 in bf16 takes 204-212 us on different boards, 1500-1560 TFLOP/s (the library's product beside the 212: 205);
+// 4096 -> 2048 in bf16 takes 204-212 us on different boards, 1500-1560 TFLOP/s (the library's product beside 209 and 212: 204, 205);
 // 8192 x 4096 -> 8192 in 8-bit integers 165-173 us, 3180-3330 TOP/s.
 // Many small groups are bound by their weights' bytes (64 groups of about 8 rows, 2048 -> 1024: 46 us,
-// 0.90 of the measured bandwidth), short contractions by bringing the results to memory (18944 x 64 -> 2048: 22 us; with
+// 0.90 of the measured bandwidth), short contractions by bringing the results to memory (18944 x 64 -> 2048: 21 us; with
 // eight warps instead of sixteen and 16-byte pieces instead of transposing matrix stores 26 us).
 // Tried and left: asking L2 for the next unit's boxes ahead of their loads (the TMA unit does twice the work: 430 instead of
 // 385 us on 32768 rows of 16 groups, 2048 -> 4096), or for its first blocks alone (no difference).

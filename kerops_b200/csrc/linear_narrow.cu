@@ -7,8 +7,8 @@
 // columns inside a fragment is free: a lane's words of a 16-byte piece of a row are the operands of two products as they
 // come, and the columns are dealt to the fragments so that a lane's results are 16 contiguous bytes of an output row.
 //
-// 4.48 M rows, fp16: 32 -> 32 channels 95 us, 128 -> 8 186 us (0.93 and 1.00 of the measured copy bandwidth), 64 -> 64, whose
-// weights fill the registers, 200 us (0.87); the tensor-core kernel of linear_mma.cu took 295 us for 64 -> 32 (now 139 us).
+// 4.48 M rows, fp16: 32 -> 32 channels 95 us, 128 -> 8 184 us (0.92 and 1.01 of the measured copy bandwidth), 64 -> 64, whose
+// weights fill the registers, 181 us (0.97); the tensor-core kernel of linear_mma.cu took 295 us for 64 -> 32 (now 137 us).
 #include "../../include/kdw.h"
 #include "linear_core.cuh"
 #include "linear_plan.h"
@@ -66,9 +66,9 @@ struct NCfg {
     static constexpr int COLS = NP >= 32 ? 32 : NP;             // columns whose results a lane stores as one piece
     static constexpr int GROUPS = NP / COLS, TILES = COLS / 8;  // of eight columns, per piece
     static constexpr int AHEAD = PIECES >= 4 ? 1 : PIECES == 2 ? 2 : 4;  // row tiles whose loads are in flight
-    // The tiles of a warp in flight are neighbours, or spread over the warps' tiles where rows of 256 bytes are written.
-    // 4.48 M rows, us, neighbours and spread: 64 -> 64 200 and 207, 32 -> 64 158 and 163, 8 -> 128 212 and 220, but 16 -> 128
-    // 270 and 241, 32 -> 128 291 and 247.
+    // The tiles of a warp in flight are neighbours, or spread over the warps' tiles where rows of 256 bytes are written and those
+    // read have 32 bytes and more.  4.48 M rows, us, neighbours and spread: 64 -> 64 181 and 187, 32 -> 64 149 and 154, 8 -> 128
+    // 212 and 208, 16 -> 128 255 and 231, 32 -> 128 257 and 254.
     static constexpr bool SPREAD = NP == 128 && KP >= 16;
     static constexpr int THREADS = 128;
     static constexpr int CTAS = KP * NP >= 4096 ? 3 : 4;        // to an SM at least: what the registers have to allow

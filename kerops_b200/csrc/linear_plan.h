@@ -43,7 +43,7 @@ constexpr int kFewRows = 16;
 constexpr int kFewQuantRows = 8, kFewQuantPitch = 128 * 96 + 64;  // rows and bytes of a row that a CTA quantises itself
 int linear_few(const LinArgs& a, int x_type, cudaStream_t st);
 // Output channels of a CTA: 32 where CTAs of 16 would not all be resident at once (two to an SM; `groups` at most that have
-// rows).  8 rows of 8 groups, 2048 -> 1024, 9.1 us instead of 10.3 (8.3 now that pieces run ahead); with fewer CTAs the
+// rows).  8 rows of 8 groups, 2048 -> 1024, 9.1 us instead of 10.3 (7.0 now that pieces run ahead); with fewer CTAs the
 // contraction is better split further (4096 x 4096: 8.5 and 11.2 us, measured before that too).
 inline int few_channels(int64_t N, int64_t groups, int sms) { return (N + 15) / 16 * groups > 2 * (int64_t)sms ? 32 : 16; }
 

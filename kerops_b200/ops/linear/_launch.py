@@ -12,8 +12,8 @@ INT8 = 2  # KDW_I8
 FWD, DGRAD, WGRAD = 0, 1, 2
 MAX_GROUPS = 1024
 
-# of a device index, and the current one: torch.cuda.current_stream and torch.cuda.device cost 3 us more, a quarter of a
-# small call
+# of a device index, and the current one: torch.cuda.current_stream and torch.cuda.device cost 3 us more, beside
+# some 10 us that a small call takes
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)  # (absent from builds of torch without CUDA)
 _current_device = getattr(torch._C, '_cuda_getDevice', None)
 

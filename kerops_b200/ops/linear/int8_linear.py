@@ -42,7 +42,8 @@ def Int8Linear(x, weight, w_scale, ends=None, *, x_scale=None, dtype=None):
     weight   [E, N, K] (or [N, K]) int8 contiguous and w_scale [E, N] (or [N]) fp32 contiguous: QuantRows(weights)
     ends     [E] int32 cumulative row counts, as for GroupedLinear; None: one group
     dtype    torch.float16 or torch.bfloat16, the result's; x's own by default, needed for int8 x
-    Returns [T, N], or a channels_last_3d volume with N channels.  K at most 131071."""
+    Returns [T, N], or a channels_last_3d volume with N channels.  K at most 131071.  Pays with long rows; on volumes of up
+    to some 128 channels GroupedLinear on 16-bit weights is faster (8 M voxels, 64 -> 64: 319 and 877 us)."""
     assert weight.ndim in (2, 3) and weight.dtype == torch.int8 and weight.is_contiguous(), \
         'weight: contiguous int8 [groups, out_channels, in_channels] or [out_channels, in_channels] expected'
     E, N, K = weight.shape if weight.ndim == 3 else (1,) + tuple(weight.shape)
