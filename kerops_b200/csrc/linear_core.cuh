@@ -286,6 +286,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();  // the barrier is executed by converged warps, whatever their lanes did before
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Arrivals on another CTA's barrier.  Only the first makes this thread's writes to memory visible to the CTA that waits by

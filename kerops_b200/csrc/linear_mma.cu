@@ -640,8 +640,11 @@ __global__ __launch_bounds__(C::THREADS, 1) void linear_kernel(const __grid_cons
     if (C::PAIR || shared_tile) cluster_sync();
     tc_fence_after();
     // CTA 0's last report goes to both CTAs, and it has waited for its own: CTA 1 leaves when the other has arrived too
-    if (C::PAIR && rank != 0 && warp == 1 && !mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
-    if (warp == 1) tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
+    if (warp == 1) {
+        if (C::PAIR && rank != 0 && !mbar_wait_bounded(drain, 0, p.limit_ns)) atomicExch(p.status, (int)KDW_STATUS_TMA_TIMEOUT);
+        __syncwarp();  // (lanes may leave the wait one after the other; what follows is executed by the warp as one)
+        tmem_free<C::PAIR>(tmem, C::TMEM_COLS);
+    }
     if (shared_tile) {
         if (early) grid_dependency_wait();  // (of the warps that have not waited)
         w = ring[0];
